@@ -54,8 +54,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // One 16-byte chunk of a row centred on the codebook mean and scaled by -2: fma(-2, x, 2 m) rounds
-// once, exactly like x - m, and doubling is exact.  Two components per instruction (v_pk_fma_f32);
-// sq gathers the squares, even components in one half and odd ones in the other.
+// once, exactly like x - m, and doubling is exact.  sq gathers the squares, even components in one
+// half and odd ones in the other.
 __device__ __forceinline__ void centre_chunk(const f32x4 x, const f32x4 mu2, float* out, f32x2& sq) {
   const f32x2 m2 = {-2.0f, -2.0f};
   const f32x2 a = __builtin_elementwise_fma(m2, x.lo, mu2.lo);
