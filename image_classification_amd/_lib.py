@@ -23,6 +23,10 @@ NORM_MODES = {"none": IC_NORM_NONE, "l1": IC_NORM_L1, "l2": IC_NORM_L2,
 METRICS = {"euclidean": 0, "l2": 0, "sqeuclidean": 1, "manhattan": 2, "cityblock": 2, "l1": 2,
            "intersection": 3, "chisqr": 4}
 
+# element types and the block of 8-bit optimizer states, as in include/ic_hip.h
+IC_F32, IC_BF16, IC_F16 = 0, 1, 2
+IC_ADAMW_BLOCK = 256
+
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
 _c_f = ctypes.c_float
@@ -64,9 +68,29 @@ _SIGNATURES = {
     "ic_ransac_homography": [_p, _p, _p, _c_i64, _c_int, _p, ctypes.c_uint64, _c_d, _c_int, _c_int,
                              _p, _p, _p, _p, _p, _p],
     "ic_host_gather_f32": [_p, _p, _p, _p, _c_i64, _c_int],
+    "ic_group_rows_scratch": [_c_i64, _c_i64],
+    "ic_group_rows": [_p, _p, _c_i64, _c_i64, _p, _p, _p, _c_i64, _p],
+    "ic_grouped_matmul": [_p, _p, _c_i64, _p, _p, _c_i64, _p, _p, _c_i64, _c_i64, _c_int, _c_int,
+                          _c_int, _c_int, _p],
+    "ic_grouped_matmul_dx": [_p, _p, _c_i64, _p, _p, _c_i64, _p, _p, _c_i64, _c_i64, _c_int, _c_int,
+                             _c_int, _c_int, _p],
+    "ic_grouped_matmul_dw_scratch": [_c_i64, _c_int, _c_int],
+    "ic_grouped_matmul_dw": [_p, _p, _c_i64, _p, _c_i64, _p, _p, _p, _c_i64, _c_i64, _c_int, _c_int,
+                             _c_int, _c_int, _p, _c_i64, _p],
+    "ic_label_logprobs_scratch": [_c_i64, _c_i64, _c_int, _c_int],
+    "ic_label_logprobs": [_p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _c_int, _c_f, _c_int, _p, _p, _p,
+                          _p, _p, _p, _c_i64, _p],
+    "ic_label_logprobs_grad": [_p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _c_int, _c_f, _p, _p, _p, _p,
+                               _p, _c_i64, _p],
+    "ic_adamw_step": [_p, _p, _c_i64, _c_int, _p, _p, _p, _c_i64, _c_d, _p, _c_d, _c_d, _c_d, _c_d,
+                      _c_i64, _p, _c_f, _p],
+    "ic_adamw_state_values": [_p, _p, _p, _p, _c_i64, _p, _p, _p],
 }
 _RESTYPES = {"ic_last_error": ctypes.c_char_p, "ic_codebook_aux_floats": ctypes.c_int64,
-             "ic_codebook_aux_floats_d": ctypes.c_int64}
+             "ic_codebook_aux_floats_d": ctypes.c_int64,
+             "ic_group_rows_scratch": ctypes.c_int64,
+             "ic_grouped_matmul_dw_scratch": ctypes.c_int64,
+             "ic_label_logprobs_scratch": ctypes.c_int64}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

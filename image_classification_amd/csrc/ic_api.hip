@@ -353,6 +353,7 @@ int ic_create(int device, void** handle) {
   // copy of the static scratch array
   e = ic::assign_init();
   if (e == hipSuccess) e = ic::reduce_init();
+  if (e == hipSuccess) e = ic::grouped_init();
   if (e != hipSuccess) {
     (void)hipEventDestroy(c->done);
     delete c;
@@ -876,6 +877,276 @@ int ic_ransac_homography(void* handle, const double* pts, const int64_t* offsets
                            best_err, best_iter, inlier_mask, s),
          "homography RANSAC kernels");
   return scope.finish();
+}
+
+// ---- what is learned on top of the codes: launches only, no handle state ------------------------
+
+namespace {
+
+bool bad_type(int t) { return t != IC_F32 && t != IC_BF16 && t != IC_F16; }
+int type_bytes(int t) { return t == IC_F32 ? 4 : 2; }
+
+int check_scratch(const char* who, const void* scratch, int64_t have, size_t need) {
+  if (need == 0) return IC_OK;
+  if (!scratch || have < 0 || (size_t)have < need)
+    return fail(IC_EINVAL, "%s: needs %zu bytes of scratch, got %lld", who, need,
+                (long long)(scratch ? have : 0));
+  if (reinterpret_cast<uintptr_t>(scratch) & 15)
+    return fail(IC_EINVAL, "%s: scratch must be 16-byte aligned", who);
+  return IC_OK;
+}
+
+int check_grouped(const char* who, int64_t n, int64_t groups, int k, int out, int dtype, int y_dtype) {
+  if (n < 0 || n >= 0x7fffffffLL || groups < 1 || groups > ((int64_t)1 << 26))
+    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 and 1 <= n_groups <= 2^26 (n=%lld n_groups=%lld)", who,
+                (long long)n, (long long)groups);
+  if (k < 1 || out < 1 || k > (1 << 24) || out > (1 << 24))
+    return fail(IC_EINVAL, "%s: widths must be in [1, 2^24] (k=%d out=%d)", who, k, out);
+  if (bad_type(dtype) || (y_dtype != dtype && y_dtype != IC_F32))
+    return fail(IC_EINVAL, "%s: unsupported element types %d -> %d", who, dtype, y_dtype);
+  return IC_OK;
+}
+
+int misaligned(const char* who, const void* p, int type) {
+  if (reinterpret_cast<uintptr_t>(p) % type_bytes(type))
+    return fail(IC_EINVAL, "%s: a pointer is not aligned to its element type", who);
+  return IC_OK;
+}
+
+int grouped_rows_call(void* handle, const char* who, bool dx, const void* x, int64_t ld_x, const void* w,
+                      void* y, int64_t ld_y, const int64_t* offsets, const int32_t* order, int64_t n,
+                      int64_t groups, int k, int out, int dtype, int y_dtype, void* stream) {
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  int rc = check_grouped(who, n, groups, k, out, dtype, y_dtype);
+  if (rc) return rc;
+  if (n == 0) return IC_OK;
+  if (!x || !w || !y || !offsets) return fail(IC_EINVAL, "%s: NULL pointer", who);
+  if (ld_x < (dx ? out : k) || ld_y < (dx ? k : out))
+    return fail(IC_EINVAL, "%s: rows overlap (row strides %lld, %lld)", who, (long long)ld_x, (long long)ld_y);
+  if ((rc = misaligned(who, x, dtype)) || (rc = misaligned(who, w, dtype)) ||
+      (rc = misaligned(who, y, y_dtype)))
+    return rc;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  const ic::GroupedCall c{x, w, y, offsets, order, n, groups, k, out, ld_x, 0, ld_y, dtype,
+                          y_dtype == IC_F32};
+  IC_HIP(ic::launch_grouped_rows(c, dx, static_cast<hipStream_t>(stream)), who);
+  return IC_OK;
+}
+
+int check_scores(const char* who, int64_t n, int64_t v, int dtype, int64_t ld, float inv_t) {
+  if (n < 0 || n >= 0x7fffffffLL || v < 1 || v > 0x7fffff00LL)
+    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 and 1 <= v <= 2^31 - 256 (n=%lld v=%lld)", who,
+                (long long)n, (long long)v);
+  if (bad_type(dtype)) return fail(IC_EINVAL, "%s: unknown element type %d", who, dtype);
+  if (ld < v) return fail(IC_EINVAL, "%s: rows overlap (row stride %lld)", who, (long long)ld);
+  if (!(inv_t > 0.0f) || inv_t > 3.0e38f)
+    return fail(IC_EINVAL, "%s: the temperature must be positive and finite", who);
+  return IC_OK;
+}
+
+}  // namespace
+
+int64_t ic_group_rows_scratch(int64_t n, int64_t n_groups) {
+  if (n < 0 || n_groups < 1) return 0;
+  return (int64_t)ic::group_rows_scratch(n, n_groups);
+}
+
+int ic_group_rows(void* handle, const int32_t* codes, int64_t n, int64_t n_groups, int32_t* order,
+                  int64_t* offsets, void* scratch, int64_t scratch_bytes, void* stream) {
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "ic_group_rows: invalid handle");
+  int rc = check_grouped("ic_group_rows", n, n_groups, 1, 1, IC_F32, IC_F32);
+  if (rc) return rc;
+  if (!offsets || (n > 0 && (!codes || !order))) return fail(IC_EINVAL, "ic_group_rows: NULL pointer");
+  rc = check_scratch("ic_group_rows", scratch, scratch_bytes, ic::group_rows_scratch(n, n_groups));
+  if (rc) return rc;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  IC_HIP(ic::launch_group_rows(codes, n, n_groups, order, offsets, scratch,
+                               static_cast<hipStream_t>(stream)),
+         "row grouping kernels");
+  return IC_OK;
+}
+
+int ic_grouped_matmul(void* handle, const void* x, int64_t ld_x, const void* w, void* y, int64_t ld_y,
+                      const int64_t* offsets, const int32_t* order, int64_t n, int64_t n_groups, int k,
+                      int out, int dtype, int y_dtype, void* stream) {
+  return grouped_rows_call(handle, "ic_grouped_matmul", false, x, ld_x, w, y, ld_y, offsets, order, n,
+                           n_groups, k, out, dtype, y_dtype, stream);
+}
+
+int ic_grouped_matmul_dx(void* handle, const void* dy, int64_t ld_dy, const void* w, void* dx,
+                         int64_t ld_dx, const int64_t* offsets, const int32_t* order, int64_t n,
+                         int64_t n_groups, int k, int out, int dtype, int y_dtype, void* stream) {
+  return grouped_rows_call(handle, "ic_grouped_matmul_dx", true, dy, ld_dy, w, dx, ld_dx, offsets, order,
+                           n, n_groups, k, out, dtype, y_dtype, stream);
+}
+
+int64_t ic_grouped_matmul_dw_scratch(int64_t n, int k, int out) {
+  if (n < 0 || k < 1 || out < 1) return 0;
+  return (int64_t)ic::grouped_dw_scratch(n, out, k);
+}
+
+int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                         void* dw, const int64_t* offsets, const int32_t* order, int64_t n,
+                         int64_t n_groups, int k, int out, int dtype, int y_dtype, void* scratch,
+                         int64_t scratch_bytes, void* stream) {
+  const char* who = "ic_grouped_matmul_dw";
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  int rc = check_grouped(who, n, n_groups, k, out, dtype, y_dtype);
+  if (rc) return rc;
+  if (!dw || !offsets || (n > 0 && (!x || !dy))) return fail(IC_EINVAL, "%s: NULL pointer", who);
+  if (ld_x < k || ld_dy < out) return fail(IC_EINVAL, "%s: rows overlap", who);
+  if ((rc = misaligned(who, x, dtype)) || (rc = misaligned(who, dy, dtype)) ||
+      (rc = misaligned(who, dw, y_dtype)))
+    return rc;
+  rc = check_scratch(who, scratch, scratch_bytes, ic::grouped_dw_scratch(n, out, k));
+  if (rc) return rc;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  const ic::GroupedCall c{x, dy, dw, offsets, order, n, n_groups, k, out, ld_x, ld_dy, 0, dtype,
+                          y_dtype == IC_F32};
+  IC_HIP(ic::launch_grouped_dw(c, scratch, static_cast<hipStream_t>(stream)), who);
+  return IC_OK;
+}
+
+int64_t ic_label_logprobs_scratch(int64_t n, int64_t v, int dtype, int top) {
+  if (n < 0 || v < 1 || bad_type(dtype) || top < 0) return 0;
+  return (int64_t)ic::score_scratch_bytes(n, ic::score_pieces(n, v, dtype), top);
+}
+
+int ic_label_logprobs(void* handle, const void* logits, int64_t ld, int64_t n, int64_t v, int dtype,
+                      const void* labels, int labels64, float inv_temperature, int top, float* logp,
+                      float* entropy, float* lse, float* top_logp, int32_t* top_idx, void* scratch,
+                      int64_t scratch_bytes, void* stream) {
+  const char* who = "ic_label_logprobs";
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  int rc = check_scores(who, n, v, dtype, ld, inv_temperature);
+  if (rc) return rc;
+  if (top < 0 || top > ic::kMaxTop || top > v)
+    return fail(IC_EINVAL, "%s: top must be in [0, min(%d, v)], got %d", who, ic::kMaxTop, top);
+  if (n == 0) return IC_OK;
+  if (!logits || !entropy || !lse || (top > 0 && (!top_logp || !top_idx)))
+    return fail(IC_EINVAL, "%s: NULL pointer", who);
+  rc = misaligned(who, logits, dtype);
+  if (rc) return rc;
+  const int pieces = ic::score_pieces(n, v, dtype);
+  rc = check_scratch(who, scratch, scratch_bytes, ic::score_scratch_bytes(n, pieces, top));
+  if (rc) return rc;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  IC_HIP(ic::launch_label_logprobs(logits, dtype, ld, n, v, labels, labels64 != 0, inv_temperature, top,
+                                   logp, entropy, lse, top_logp, top_idx, pieces, scratch,
+                                   static_cast<hipStream_t>(stream)),
+         who);
+  return IC_OK;
+}
+
+int ic_label_logprobs_grad(void* handle, const void* logits, int64_t ld, int64_t n, int64_t v, int dtype,
+                           const void* labels, int labels64, float inv_temperature, const float* lse,
+                           const float* entropy, const float* d_logp, const float* d_entropy, void* out,
+                           int64_t ld_out, void* stream) {
+  const char* who = "ic_label_logprobs_grad";
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  int rc = check_scores(who, n, v, dtype, ld, inv_temperature);
+  if (rc) return rc;
+  if (ld_out < v) return fail(IC_EINVAL, "%s: output rows overlap (row stride %lld)", who, (long long)ld_out);
+  if (n == 0) return IC_OK;
+  if (!logits || !out || !lse || (d_entropy && !entropy) || (d_logp && !labels))
+    return fail(IC_EINVAL, "%s: NULL pointer", who);
+  if ((rc = misaligned(who, logits, dtype)) || (rc = misaligned(who, out, dtype))) return rc;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  IC_HIP(ic::launch_label_logprobs_grad(logits, dtype, ld, n, v, labels, labels64 != 0, inv_temperature,
+                                        lse, entropy, d_logp, d_entropy, out, ld_out,
+                                        static_cast<hipStream_t>(stream)),
+         who);
+  return IC_OK;
+}
+
+int ic_adamw_step(void* handle, const ic_adamw_tensor* tensors, int64_t count, int state_bits,
+                  void* exp_avg, void* exp_avg_sq, float* scales, int64_t state_elements, double lr,
+                  const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,
+                  int64_t step, const int64_t* step_dev, float grad_scale, void* stream) {
+  const char* who = "ic_adamw_step";
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  if (count < 0 || (count > 0 && !tensors)) return fail(IC_EINVAL, "%s: no tensors", who);
+  if (state_bits != 32 && state_bits != 8)
+    return fail(IC_EINVAL, "%s: states have 32 or 8 bits, not %d", who, state_bits);
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
+    return fail(IC_EINVAL, "%s: betas must be in [0, 1)", who);
+  if (!(eps >= 0.0)) return fail(IC_EINVAL, "%s: eps must not be negative", who);
+  if (!step_dev && step < 1) return fail(IC_EINVAL, "%s: step counts from 1, got %lld", who, (long long)step);
+  if (state_elements < 0 || state_elements % IC_ADAMW_BLOCK)
+    return fail(IC_EINVAL, "%s: state_elements must be a multiple of %d", who, IC_ADAMW_BLOCK);
+  if (((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq)) & 15) ||
+      (reinterpret_cast<uintptr_t>(scales) & 3))
+    return fail(IC_EINVAL, "%s: states must be 16-byte aligned", who);
+  std::vector<ic::AdamTensor> list;
+  try {
+    list.reserve((size_t)count);
+  } catch (...) {
+    return fail(IC_ENOMEM, "%s: no memory for a list of %lld tensors", who, (long long)count);
+  }
+  for (int64_t i = 0; i < count; ++i) {
+    const ic_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || t.n > ((int64_t)1 << 33)) return fail(IC_EINVAL, "%s: tensor %lld has a bad size", who, (long long)i);
+    if (t.n == 0) continue;
+    if (!t.param || !t.grad || !exp_avg || !exp_avg_sq || (state_bits == 8 && !scales))
+      return fail(IC_EINVAL, "%s: NULL pointer (tensor %lld)", who, (long long)i);
+    if (bad_type(t.param_dtype) || bad_type(t.grad_dtype))
+      return fail(IC_EINVAL, "%s: tensor %lld has an unknown element type", who, (long long)i);
+    int rc = misaligned(who, t.param, t.param_dtype);
+    if (!rc) rc = misaligned(who, t.grad, t.grad_dtype);
+    if (rc) return rc;
+    const int64_t padded = (t.n + IC_ADAMW_BLOCK - 1) / IC_ADAMW_BLOCK * IC_ADAMW_BLOCK;
+    if (t.state_offset < 0 || t.state_offset % IC_ADAMW_BLOCK || t.state_offset > state_elements - padded)
+      return fail(IC_EINVAL, "%s: the states of tensor %lld lie outside the state arrays", who, (long long)i);
+    ic::AdamTensor d = {};
+    d.p = t.param;
+    d.g = t.grad;
+    d.n = t.n;
+    d.state0 = t.state_offset;
+    d.p_type = (unsigned char)t.param_dtype;
+    d.g_type = (unsigned char)t.grad_dtype;
+    list.push_back(d);
+  }
+  if (list.empty()) return IC_OK;
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  IC_HIP(ic::launch_adamw(list.data(), (int64_t)list.size(), state_bits, exp_avg, exp_avg_sq, scales,
+                          state_elements, lr, lr_dev, beta1, beta2, eps, weight_decay, step, step_dev,
+                          grad_scale, static_cast<hipStream_t>(stream)),
+         who);
+  return IC_OK;
+}
+
+int ic_adamw_state_values(void* handle, const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                          const float* scales, int64_t state_elements, float* out_avg,
+                          float* out_avg_sq, void* stream) {
+  const char* who = "ic_adamw_state_values";
+  Ctx* ctx = as_ctx(handle);
+  if (!ctx) return fail(IC_EHANDLE, "%s: invalid handle", who);
+  if (state_elements < 0 || state_elements % IC_ADAMW_BLOCK)
+    return fail(IC_EINVAL, "%s: state_elements must be a multiple of %d", who, IC_ADAMW_BLOCK);
+  if (state_elements == 0) return IC_OK;
+  if (!exp_avg || !exp_avg_sq || !scales || !out_avg || !out_avg_sq)
+    return fail(IC_EINVAL, "%s: NULL pointer", who);
+  if ((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq) |
+       reinterpret_cast<uintptr_t>(out_avg) | reinterpret_cast<uintptr_t>(out_avg_sq)) & 15)
+    return fail(IC_EINVAL, "%s: states and outputs must be 16-byte aligned", who);
+  DeviceGuard guard(ctx->device);
+  if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");
+  IC_HIP(ic::launch_adamw_values(exp_avg, exp_avg_sq, scales, state_elements, out_avg, out_avg_sq,
+                                 static_cast<hipStream_t>(stream)),
+         who);
+  return IC_OK;
 }
 
 }  // extern "C"

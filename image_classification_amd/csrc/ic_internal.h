@@ -11,6 +11,7 @@ namespace ic {
 
 constexpr int kD = 128;      // padded descriptor dimension the MFMA kernel contracts over
 constexpr int kStageK = 128;  // codebook norms are padded to a multiple of this (the largest stage)
+constexpr int kCUs = 256;    // compute units of the one GPU this library is built for
 constexpr int kMaxShards = 64;  // shard bases of ic_top2_merge travel as a kernel argument
 
 static_assert(sizeof(ic_top2_rec) == 16, "ic_top2_rec must be 16 bytes");
@@ -218,5 +219,61 @@ hipError_t launch_ransac(const double* pts, const int64_t* off, int64_t n_cand, 
                          const int32_t* samples, uint64_t seed, double th, int min_inliers,
                          int flags, int32_t* n_inl_ws, double* H, int32_t* n_inliers,
                          double* best_err, int32_t* best_it, uint8_t* mask, hipStream_t s);
+
+// ---- ic_score.hip -----------------------------------------------------------------------------
+constexpr int kMaxTop = 32;   // alternatives of a row: a wave's lanes hold them
+// pieces a row is cut into (more than 1: a second launch joins them through scratch)
+int score_pieces(int64_t n, int64_t v, int dtype);
+size_t score_scratch_bytes(int64_t n, int pieces, int top);
+hipError_t launch_label_logprobs(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v,
+                                 const void* labels, int labels64, float inv_t, int top, float* logp,
+                                 float* entropy, float* lse, float* top_logp, int32_t* top_idx,
+                                 int pieces, void* scratch, hipStream_t s);
+hipError_t launch_label_logprobs_grad(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v,
+                                      const void* labels, int labels64, float inv_t, const float* lse,
+                                      const float* entropy, const float* d_logp,
+                                      const float* d_entropy, void* out, int64_t ld_out, hipStream_t s);
+
+// ---- ic_optim.hip -----------------------------------------------------------------------------
+constexpr int kStateBlock = IC_ADAMW_BLOCK;   // state elements that share a scale
+constexpr int kTensorsPerLaunch = 64;         // their table is a kernel argument of 2.5 KB
+constexpr int64_t kMaxChunks = (int64_t)1 << 23;   // workgroups of a launch
+struct AdamTensor {
+  void* p;
+  const void* g;
+  int64_t n;
+  int64_t state0;   // where its states begin (a multiple of kStateBlock)
+  int chunk0;       // set by the launcher
+  unsigned char p_type, g_type, p_vec, g_vec;
+};
+// m, v: float32 (bits 32) or codes (bits 8, with scales [2][state_elements / kStateBlock])
+hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int bits, void* m, void* v,
+                        float* scales, int64_t state_elements, double lr, const float* lr_dev,
+                        double b1, double b2, double eps, double wd, int64_t step,
+                        const int64_t* step_dev, float grad_scale, hipStream_t s);
+hipError_t launch_adamw_values(const unsigned char* m, const unsigned char* v, const float* scales,
+                               int64_t n, float* out_m, float* out_v, hipStream_t s);
+
+// ---- ic_grouped.hip ---------------------------------------------------------------------------
+hipError_t grouped_init();   // once per device: function attributes
+// order int32 [n], offsets int64 [groups + 1] <- codes int32 [n], stable; scratch: group_rows_scratch
+size_t group_rows_scratch(int64_t n, int64_t groups);
+hipError_t launch_group_rows(const int32_t* codes, int64_t n, int64_t groups, int32_t* order,
+                             int64_t* offsets, void* scratch, hipStream_t s);
+struct GroupedCall {
+  const void* x;          // rows (forward: x, dx: dy, dw: x)
+  const void* w;          // forward, dx: the groups' matrices [groups][out][k]; dw: dy
+  void* y;
+  const int64_t* offsets;
+  const int32_t* order;   // may be NULL
+  int64_t n, groups;
+  int k, out;             // W_e is out x k
+  int64_t ld_x, ld_w, ld_y;   // row strides in elements (ld_w: dw's dy)
+  int type;
+  int y_f32;              // the result is float32 whatever the type
+};
+hipError_t launch_grouped_rows(const GroupedCall& c, bool dx, hipStream_t s);
+size_t grouped_dw_scratch(int64_t n, int out, int k);
+hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s);
 
 }  // namespace ic

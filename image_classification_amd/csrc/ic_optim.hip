@@ -1,0 +1,350 @@
+// One AdamW step over many tensors, with optimizer states in 32 or in 8 bits.
+//
+//     m <- b1 m + (1 - b1) g          v <- b2 v + (1 - b2) g^2
+//     p <- p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// The tensors' addresses travel as kernel arguments, kTensorsPerLaunch a launch, so that a step is
+// launches only: nothing is uploaded, and a captured graph holds the addresses it was captured with.
+// States lie in flat arrays in which every tensor starts at a multiple of kStateBlock elements.
+//
+// States in 8 bits: kStateBlock elements share two float32 scales.
+//   m: sign, 4-bit exponent, 3-bit mantissa of m / scale_m, with scale_m = max |m| / 448 (448 is
+//      the largest finite code, 126; 127 marks a value that is not finite);
+//   v: an unsigned 4-bit exponent, 4-bit mantissa code of sqrt(v) / scale_v, scale_v = max / 491520
+//      (code 254; 255 marks a value that is not finite).  sqrt(v) rather than v: the step divides
+//      by it, and its range is half as many octaves.  A state above zero keeps a code above zero,
+//      so the step never divides by eps alone where a gradient was seen.
+// Both roundings are to nearest, an exact middle to the even code, at most 2^-4 (m) and 2^-5
+// (sqrt v) of the value, and the codes are decided in float64 (see k_adamw8): which of two codes a
+// value takes then does not depend on the last bit of a float32 evaluation.
+// The update uses the new m and v before they are rounded.
+//
+// What bounds it: memory.  See the figures at each kernel.
+#include "ic_wave.h"
+
+namespace ic {
+
+namespace {
+
+struct AdamTable {
+  AdamTensor t[kTensorsPerLaunch];
+  int count;
+};
+
+struct AdamArgs {
+  void* m;
+  void* v;
+  float* scale_m;
+  float* scale_v;
+  double lr, b1, b2, omb1, omb2, eps, wd, c1, c2;   // omb = 1 - b; c = 1 - b^t
+  const float* lr_dev;       // not NULL: the learning rate is read here
+  const int64_t* step_dev;   // not NULL: t is read here
+  float grad_scale;
+};
+
+constexpr int kChunk = 2048;   // elements of a workgroup's pass: 256 lanes x 8
+
+__device__ __forceinline__ int find_tensor(const AdamTable& tab, int chunk) {
+  int lo = 0, hi = tab.count;   // the last tensor whose chunk0 <= chunk
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.t[mid].chunk0 <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// b^t for t >= 0 by squaring
+__device__ double power(double b, int64_t t) {
+  double r = 1.0;
+  for (; t > 0; t >>= 1) {
+    if (t & 1) r *= b;
+    b *= b;
+  }
+  return r;
+}
+
+// eight consecutive elements at p + i; those at and behind n are 0
+template <typename T>
+__device__ __forceinline__ void get8(const T* p, int64_t i, int64_t n, bool vec, float* x) {
+  constexpr int kV = Elem<T>::kVec;
+  if (vec && i + 8 <= n) {
+#pragma unroll
+    for (int q = 0; q < 8; q += kV) Elem<T>::unpack(*reinterpret_cast<const u32x4*>(p + i + q), x + q);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) x[q] = i + q < n ? Elem<T>::load(p + i + q) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* p, int64_t i, int64_t n, bool vec, const float* x) {
+  constexpr int kV = Elem<T>::kVec;
+  if (vec && i + 8 <= n) {
+#pragma unroll
+    for (int q = 0; q < 8; q += kV) *reinterpret_cast<u32x4*>(p + i + q) = Elem<T>::pack(x + q);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (i + q < n) Elem<T>::store(p + i + q, x[q]);
+  }
+}
+__device__ __forceinline__ void get_typed(const void* p, int type, int64_t i, int64_t n, bool vec,
+                                          float* x) {
+  if (type == IC_F32) get8(static_cast<const float*>(p), i, n, vec, x);
+  else if (type == IC_BF16) get8(static_cast<const bf16_t*>(p), i, n, vec, x);
+  else get8(static_cast<const f16_t*>(p), i, n, vec, x);
+}
+__device__ __forceinline__ void put_typed(void* p, int type, int64_t i, int64_t n, bool vec,
+                                          const float* x) {
+  if (type == IC_F32) put8(static_cast<float*>(p), i, n, vec, x);
+  else if (type == IC_BF16) put8(static_cast<bf16_t*>(p), i, n, vec, x);
+  else put8(static_cast<f16_t*>(p), i, n, vec, x);
+}
+
+__device__ __forceinline__ void corrections(const AdamArgs& a, double* lr, double* c1, double* c2) {
+  *lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+  if (a.step_dev) {
+    const int64_t t = *a.step_dev;
+    *c1 = 1.0 - power(a.b1, t);
+    *c2 = 1.0 - power(a.b2, t);
+  } else {
+    *c1 = a.c1;
+    *c2 = a.c2;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_adamw32(AdamTable tab, AdamArgs a) {
+  const int chunk = blockIdx.x;
+  const AdamTensor& t = tab.t[find_tensor(tab, chunk)];
+  const int64_t i = (int64_t)(chunk - t.chunk0) * kChunk + (int64_t)threadIdx.x * 8;
+  if (i >= t.n) return;
+  double lr, c1, c2;
+  corrections(a, &lr, &c1, &c2);
+  const float b1 = (float)a.b1, b2 = (float)a.b2, omb1 = (float)a.omb1, omb2 = (float)a.omb2;
+  const float eps = (float)a.eps, lrwd = (float)(lr * a.wd), lr1 = (float)(lr / c1);
+  const float ic2 = (float)(1.0 / c2);
+  float p[8], g[8], m[8], v[8];
+  float* mp = static_cast<float*>(a.m) + t.state0;
+  float* vp = static_cast<float*>(a.v) + t.state0;
+  get_typed(t.g, t.g_type, i, t.n, t.g_vec, g);
+  get_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
+  get8(mp, i, t.n, true, m);
+  get8(vp, i, t.n, true, v);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float gq = g[q] * a.grad_scale;
+    m[q] = fmaf(b1, m[q], omb1 * gq);
+    v[q] = fmaf(b2, v[q], omb2 * gq * gq);
+    const float den = __builtin_sqrtf(v[q] * ic2) + eps;
+    p[q] = fmaf(-lrwd, p[q], p[q]) - m[q] * lr1 / den;
+  }
+  put8(mp, i, t.n, true, m);
+  put8(vp, i, t.n, true, v);
+  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
+}
+
+// -- 8-bit codes -----------------------------------------------------------------------------------
+// An unsigned float code of MANT mantissa bits stands for the integer
+//     (e ? 2^MANT + f : f) << max(e - 1, 0),   e = c >> MANT, f = c & (2^MANT - 1).
+template <int MANT>
+__device__ __forceinline__ unsigned code_value(unsigned c) {
+  const unsigned e = c >> MANT, f = c & ((1u << MANT) - 1u);
+  return (e ? (f | (1u << MANT)) : f) << (e ? e - 1u : 0u);
+}
+// The code nearest to q >= 0 (in the same units), a middle to the even one, at most `top`.
+// float64 bits: the exponent and the 20 mantissa bits of the upper word, the rest folded into a
+// sticky bit, so that "exactly the middle" is told from "a little above it".
+template <int MANT>
+__device__ __forceinline__ unsigned nearest_code(double q, unsigned top) {
+  // below 2^(MANT+1) the grid is 1: adding 2^52 rounds to an integer, to nearest even
+  constexpr double kOne52 = 4503599627370496.0;
+  if (q < (double)(2 << MANT)) return (unsigned)(int)((q + kOne52) - kOne52);
+  const unsigned long long bits = __double_as_longlong(q);
+  unsigned hi = (unsigned)(bits >> 32);
+  hi |= (unsigned)((unsigned)bits != 0u);            // sticky
+  constexpr int kDrop = 20 - MANT;
+  const unsigned r = hi + ((1u << (kDrop - 1)) - 1u) + ((hi >> kDrop) & 1u);
+  // r >> kDrop = biased exponent and MANT bits; exponent MANT is code exponent 1
+  const unsigned c = (r >> kDrop) - ((1023u + MANT - 1u) << MANT);
+  return c < top ? c : top;
+}
+
+__device__ __forceinline__ double m_value(unsigned c, double scale) {   // scale / 512 as argument
+  const unsigned mag = c & 127u;
+  const double v = (double)code_value<3>(mag) * scale;
+  const double s = (c & 128u) ? -v : v;
+  return mag == 127u ? __builtin_nan("") : s;
+}
+__device__ __forceinline__ double r_value(unsigned c, double scale) {
+  return c == 255u ? __builtin_nan("") : (double)code_value<4>(c) * scale;
+}
+
+// largest over the 32 lanes that hold one block of 256 elements (values >= 0, compared as bits)
+__device__ __forceinline__ double half_wave_max(double v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double w = __shfl_xor(v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+__global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
+  const int chunk = blockIdx.x;
+  const AdamTensor& t = tab.t[find_tensor(tab, chunk)];
+  const int64_t i = (int64_t)(chunk - t.chunk0) * kChunk + (int64_t)threadIdx.x * 8;
+  const int64_t padded = (t.n + kStateBlock - 1) / kStateBlock * kStateBlock;
+  if (i >= padded) return;   // whole blocks: their 32 lanes stay together
+  double lr, c1, c2;
+  corrections(a, &lr, &c1, &c2);
+  // (the step itself is float32: only what becomes a code has to be decided in float64)
+  const float lr1 = (float)(lr / c1), lrwd = (float)(lr * a.wd), eps = (float)a.eps;
+  const double root = sqrt(1.0 / c2);
+  unsigned char* mp = static_cast<unsigned char*>(a.m) + t.state0 + i;
+  unsigned char* vp = static_cast<unsigned char*>(a.v) + t.state0 + i;
+  const int64_t block = (t.state0 + i) / kStateBlock;
+  const u32x2 mc = *reinterpret_cast<const u32x2*>(mp);
+  const u32x2 vc = *reinterpret_cast<const u32x2*>(vp);
+  const double sm = (double)a.scale_m[block] * (1.0 / 512.0), sv = (double)a.scale_v[block];
+  float p[8], g[8];
+  get_typed(t.g, t.g_type, i, t.n, t.g_vec, g);
+  get_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
+  double m[8], r[8];
+  double top_m = 0.0, top_r = 0.0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const double gq = (double)(g[q] * a.grad_scale);
+    const double m0 = m_value((mc[q >> 2] >> (8 * (q & 3))) & 255u, sm);
+    const double r0 = r_value((vc[q >> 2] >> (8 * (q & 3))) & 255u, sv);
+    const double v = fma(a.b2, r0 * r0, a.omb2 * gq * gq);
+    m[q] = i + q < t.n ? fma(a.b1, m0, a.omb1 * gq) : 0.0;
+    r[q] = i + q < t.n ? sqrt(v) : 0.0;
+    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 / ((float)(r[q] * root) + eps);
+    const double am = fabs(m[q]);
+    if (am > top_m && am < __builtin_inf()) top_m = am;
+    if (r[q] > top_r && r[q] < __builtin_inf()) top_r = r[q];
+  }
+  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
+  const float new_sm = (float)(half_wave_max(top_m) / 448.0);
+  const float new_sv = (float)(half_wave_max(top_r) / 491520.0);
+  const double im = new_sm > 0.0f ? 512.0 / (double)new_sm : 0.0;
+  const double iv = new_sv > 0.0f ? 1.0 / (double)new_sv : 0.0;
+  u32x2 mo = {0u, 0u}, vo = {0u, 0u};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const double am = fabs(m[q]);
+    unsigned cm = am < __builtin_inf() ? nearest_code<3>(am * im, 126u) : 127u;
+    cm |= m[q] < 0.0 ? 128u : 0u;
+    unsigned cv = 255u;
+    if (r[q] < __builtin_inf()) {
+      cv = nearest_code<4>(r[q] * iv, 254u);
+      if (cv == 0u && r[q] * iv > 0.0) cv = 1u;
+    }
+    mo[q >> 2] |= cm << (8 * (q & 3));
+    vo[q >> 2] |= cv << (8 * (q & 3));
+  }
+  *reinterpret_cast<u32x2*>(mp) = mo;
+  *reinterpret_cast<u32x2*>(vp) = vo;
+  if ((threadIdx.x & 31) == 0) {
+    a.scale_m[block] = new_sm;
+    a.scale_v[block] = new_sv;
+  }
+}
+
+// The float32 values that 8-bit states stand for.
+__global__ __launch_bounds__(256) void k_adamw_values(const unsigned char* mc, const unsigned char* vc,
+                                                      const float* scale_m, const float* scale_v,
+                                                      int64_t n, float* m, float* v) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const unsigned cm = *reinterpret_cast<const unsigned*>(mc + i);
+  const unsigned cv = *reinterpret_cast<const unsigned*>(vc + i);
+  const float sm = scale_m[i / kStateBlock], sv = scale_v[i / kStateBlock];
+  f32x4 om, ov;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const unsigned c = (cm >> (8 * q)) & 255u, d = (cv >> (8 * q)) & 255u;
+    const float x = (float)code_value<3>(c & 127u) * (1.0f / 512.0f) * sm;
+    om[q] = (c & 127u) == 127u ? __builtin_nanf("") : (c & 128u) ? -x : x;
+    const float y = (float)code_value<4>(d) * sv;
+    ov[q] = d == 255u ? __builtin_nanf("") : y * y;
+  }
+  *reinterpret_cast<f32x4*>(m + i) = om;
+  *reinterpret_cast<f32x4*>(v + i) = ov;
+}
+
+}  // namespace
+
+hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int bits, void* m, void* v,
+                        float* scales, int64_t state_elements, double lr, const float* lr_dev,
+                        double b1, double b2, double eps, double wd, int64_t step,
+                        const int64_t* step_dev, float grad_scale, hipStream_t s) {
+  AdamArgs a;
+  a.m = m;
+  a.v = v;
+  a.scale_m = scales;
+  a.scale_v = scales ? scales + state_elements / kStateBlock : nullptr;
+  a.lr = lr;
+  a.b1 = b1;
+  a.b2 = b2;
+  a.omb1 = 1.0 - b1;
+  a.omb2 = 1.0 - b2;
+  a.eps = eps;
+  a.wd = wd;
+  double p1 = 1.0, p2 = 1.0;
+  double q1 = b1, q2 = b2;
+  for (int64_t t = step; t > 0; t >>= 1) {
+    if (t & 1) {
+      p1 *= q1;
+      p2 *= q2;
+    }
+    q1 *= q1;
+    q2 *= q2;
+  }
+  a.c1 = 1.0 - p1;
+  a.c2 = 1.0 - p2;
+  a.lr_dev = lr_dev;
+  a.step_dev = step_dev;
+  a.grad_scale = grad_scale;
+  AdamTable tab;
+  int64_t i = 0;
+  while (i < count) {
+    tab.count = 0;
+    int64_t chunks = 0;
+    for (; i < count && tab.count < kTensorsPerLaunch; ++i) {
+      if (tensors[i].n == 0) continue;
+      const int64_t more = (tensors[i].n + kChunk - 1) / kChunk;
+      if (chunks + more > kMaxChunks) {
+        if (tab.count) break;              // the next launch begins with it
+        return hipErrorInvalidValue;       // (refused by the caller's checks)
+      }
+      AdamTensor& d = tab.t[tab.count++];
+      d = tensors[i];
+      d.chunk0 = (int)chunks;
+      d.p_vec = (reinterpret_cast<uintptr_t>(d.p) & 15) == 0;
+      d.g_vec = (reinterpret_cast<uintptr_t>(d.g) & 15) == 0;
+      chunks += more;
+    }
+    if (!tab.count) break;
+    if (bits == 8) hipLaunchKernelGGL(k_adamw8, dim3((unsigned)chunks), dim3(256), 0, s, tab, a);
+    else hipLaunchKernelGGL(k_adamw32, dim3((unsigned)chunks), dim3(256), 0, s, tab, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_adamw_values(const unsigned char* m, const unsigned char* v, const float* scales,
+                               int64_t n, float* out_m, float* out_v, hipStream_t s) {
+  const int64_t per = (int64_t)1 << 32;   // elements of a launch (a multiple of kStateBlock)
+  for (int64_t i = 0; i < n; i += per) {
+    const int64_t k = n - i < per ? n - i : per;
+    hipLaunchKernelGGL(k_adamw_values, dim3((unsigned)((k + 1023) / 1024)), dim3(256), 0, s, m + i,
+                       v + i, scales + i / kStateBlock, scales + (n + i) / kStateBlock, k, out_m + i,
+                       out_v + i);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace ic

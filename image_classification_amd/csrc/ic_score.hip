@@ -1,0 +1,628 @@
+// Log probabilities of labels over rows of scores, their entropy and best alternatives, and the
+// gradient of the first two.
+//
+// With z_j = x_j / T for the V scores of a row:
+//     M = max_j x_j,   s = sum_j e^{(x_j - M)/T},   u = sum_j e^{(x_j - M)/T} (x_j - M)
+//     lse = M/T + ln s,   log p_j = (x_j - M)/T - ln s,   H = -sum_j p_j log p_j = ln s - u/(T s)
+// so one pass over the row gives everything: (M, s, u) of two pieces of a row join as
+//     M = max(M1, M2),  s = s1 f1 + s2 f2,  u = (u1 + s1 (M1 - M)) f1 + ...,  f = e^{(M1 - M)/T}.
+// Both terms of H are >= 0, so a peaked row's small entropy does not come out of a cancellation.
+// All sums are float32 over float32 terms, added as a tree of 64 lanes x waves x pieces.
+//
+// Special rows: scores of -inf have p = 0 and add nothing (the product 0 * (x - M) is kept finite
+// by clamping x - M); a row of nothing but -inf has lse = -inf, H = 0, log p = -inf and gradient 0;
+// a row with NaN or +inf has NaN results (its alternatives are still ranked, NaN above +inf).
+//
+// The best alternatives: values are ranked as integers (a monotone map of the float bits, -0 as
+// +0), ties to the lowest index.  A lane keeps its own two best while it streams; the t best of a
+// wave are then t rounds of a 64-lane maximum, in which only the winner moves on.  A lane that has
+// given away both of its two looks for its next ones in its part of the row again (seldom: three
+// of the t best in one of 64 lanes).
+//
+// What bounds it: reading the row once.  See the figures at each kernel.
+#include "ic_wave.h"
+
+namespace ic {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFar = -1.0e30f;      // x - M of a masked score: e^kFar is 0 and 0 * kFar is 0
+constexpr float kLowest = -3.402823466e38f;
+
+// monotone in the value, 0 below everything (an absent element)
+__device__ __forceinline__ unsigned rank_of(float x) {
+  const unsigned b = __float_as_uint(x + 0.0f);
+  const unsigned k = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+  return x != x ? 0xffffffffu : k;
+}
+__device__ __forceinline__ float value_of(unsigned k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+
+struct Stats {
+  float m, s, u;
+};
+
+__device__ __forceinline__ float gap(float x, float m) { return fmaxf(x - m, kFar); }
+
+// c = log2(e) / T
+__device__ __forceinline__ void rescale(Stats& a, float m, float c) {
+  const float d = gap(a.m, m);
+  const float f = __builtin_amdgcn_exp2f(d * c);
+  a.u = (a.u + a.s * d) * f;
+  a.s *= f;
+  a.m = m;
+}
+
+template <int N>
+__device__ __forceinline__ void add_values(Stats& a, const float* x, float c) {
+  float vm = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) vm = fmaxf(vm, x[i]);
+  rescale(a, fmaxf(a.m, vm), c);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - a.m;
+    const float e = __builtin_amdgcn_exp2f(d * c);   // NaN for NaN and for +inf: s carries it on
+    a.s += e;
+    a.u = fmaf(e, fmaxf(d, kFar), a.u);
+  }
+}
+
+// the 64 lanes' pieces as one, in every lane
+__device__ __forceinline__ Stats wave_join(Stats a, float c) {
+  rescale(a, wave_max_f32(a.m), c);
+  a.s = wave_sum_f32(a.s);
+  a.u = wave_sum_f32(a.u);
+  return a;
+}
+
+// A lane's two best: (rank, index) descending by rank, ascending by index.
+struct Best2 {
+  unsigned k1, k2;
+  int i1, i2;
+};
+__device__ __forceinline__ void keep(Best2& b, unsigned k, int i) {   // i ascends within a lane
+  const bool first = k > b.k1, second = k > b.k2;
+  b.i2 = first ? b.i1 : (second ? i : b.i2);
+  b.k2 = first ? b.k1 : (second ? k : b.k2);
+  b.i1 = first ? i : b.i1;
+  b.k1 = first ? k : b.k1;
+}
+__device__ __forceinline__ bool after(unsigned k, int i, unsigned k0, int i0) {
+  return k < k0 || (k == k0 && i > i0);
+}
+
+// The lane that holds the best (rank, index) of all lanes' heads.
+__device__ __forceinline__ int best_lane(unsigned k, int i, unsigned* kb) {
+  const unsigned top = wave_max_u32(k);
+  *kb = top;
+  unsigned long long who = __ballot(k == top);
+  if (who & (who - 1)) {   // equal values: the lowest index
+    const unsigned low = wave_min_u32(k == top ? (unsigned)i : 0xffffffffu);
+    who = __ballot(k == top && (unsigned)i == low);
+  }
+  return __builtin_amdgcn_readfirstlane(__ffsll(who) - 1);
+}
+
+// t rounds over the lanes' lists; lane r returns with the r-th best.  refill(lane, k, i) gives the
+// lane's next element after (k, i) to that lane.
+template <typename Refill>
+__device__ __forceinline__ void take_best(Best2 b, int t, int lane, unsigned* out_k, int* out_i,
+                                          Refill refill) {
+  int left = 2;
+  unsigned rk = 0;
+  int ri = -1;
+  for (int r = 0; r < t; ++r) {
+    unsigned kb;
+    const int w = best_lane(b.k1, b.i1, &kb);
+    const int ib = __builtin_amdgcn_readlane(b.i1, w);
+    if (lane == r) {
+      rk = kb;
+      ri = ib;
+    }
+    if (lane == w) {
+      b.k1 = b.k2;
+      b.i1 = b.i2;
+      b.k2 = 0;
+      --left;
+    }
+    if (r + 1 < t && __builtin_amdgcn_readlane(left, w) == 0) {
+      unsigned nk;
+      int ni;
+      refill(w, kb, ib, &nk, &ni);
+      if (lane == w) {
+        b.k1 = nk;
+        b.i1 = ni;
+        left = 1;
+      }
+    }
+  }
+  *out_k = rk;
+  *out_i = ri;
+}
+
+// Where a row lies: granules of 16 aligned bytes from the one that holds its first element on; a
+// granule that the row fills is loaded whole, one at either end of the row element by element.
+template <typename T>
+struct RowView {
+  const T* row;
+  const char* base;   // row rounded down to 16 bytes
+  int head;           // elements of the first granule that lie before the row
+  int v;
+  __device__ RowView(const T* r, int v_) : row(r), v(v_) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(r);
+    base = reinterpret_cast<const char*>(a & ~(uintptr_t)15);
+    head = (int)((a & 15) / sizeof(T));
+  }
+  __device__ __forceinline__ int granules() const {
+    return (v + head + Elem<T>::kVec - 1) / Elem<T>::kVec;
+  }
+  // x[i] = element g * kVec + i - head of the row, -inf outside it
+  __device__ __forceinline__ void get(int g, float* x) const {
+    constexpr int kV = Elem<T>::kVec;
+    const int j0 = g * kV - head;
+    if (j0 >= 0 && j0 + kV <= v) {
+      Elem<T>::unpack(*reinterpret_cast<const u32x4*>(base + (size_t)g * 16), x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const int j = j0 + i;
+        x[i] = (j >= 0 && j < v) ? Elem<T>::load(row + j) : -__builtin_inff();
+      }
+    }
+  }
+};
+
+struct ScoreArgs {
+  const void* logits;
+  int64_t ld;
+  int64_t row0, n;      // rows [row0, n) are this launch's
+  int v;
+  const void* labels;   // int32 or int64
+  int labels64;
+  float inv_t;
+  int top;
+  float* logp;
+  float* entropy;
+  float* lse;
+  float* top_logp;
+  int32_t* top_idx;
+};
+
+__device__ __forceinline__ int label_of(const ScoreArgs& a, int64_t row) {
+  if (!a.labels) return -1;
+  const int64_t l = a.labels64 ? static_cast<const int64_t*>(a.labels)[row]
+                               : (int64_t) static_cast<const int32_t*>(a.labels)[row];
+  return l >= 0 && l < a.v ? (int)l : -1;
+}
+
+// One lane writes the row's results; lanes 0 .. top-1 its alternatives.
+template <typename T>
+__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const T* x, Stats st,
+                                          int lane, unsigned rk, int ri) {
+  const bool none = st.s == 0.0f;   // nothing but -inf
+  const float ln_s = __builtin_amdgcn_logf(st.s) * kLn2;
+  if (lane == 0) {
+    a.lse[row] = none ? -__builtin_inff() : fmaf(st.m, a.inv_t, ln_s);
+    a.entropy[row] = none ? 0.0f : fmaxf(ln_s - st.u * a.inv_t / st.s, 0.0f) + 0.0f * st.s;
+    if (a.logp) {
+      const int l = label_of(a, row);
+      float lp = 0.0f;
+      if (l >= 0) {
+        const float z = Elem<T>::load(x + l);
+        lp = none ? -__builtin_inff() : (z - st.m) * a.inv_t - ln_s;
+      }
+      a.logp[row] = lp;
+    }
+  }
+  if (lane < a.top) {
+    const float z = value_of(rk);
+    a.top_idx[row * a.top + lane] = ri;
+    a.top_logp[row * a.top + lane] = none ? -__builtin_inff() : (z - st.m) * a.inv_t - ln_s;
+  }
+}
+
+// Rows of up to 64 * NC granules: one wave a row, the row stays in registers between the maximum,
+// the sums and the ranking.
+template <typename T, int NC, bool TOP>
+__global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
+  constexpr int kV = Elem<T>::kVec;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = a.row0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.n) return;
+  const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
+  const RowView<T> rv(xr, a.v);
+  const float c = a.inv_t * kLog2e;
+  float x[NC][kV];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) rv.get(i * 64 + lane, x[i]);
+  float m = kLowest;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < kV; ++j) m = fmaxf(m, x[i][j]);
+  Stats st;
+  st.m = wave_max_f32(m);
+  st.s = 0.0f;
+  st.u = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const float d = x[i][j] - st.m;
+      const float e = __builtin_amdgcn_exp2f(d * c);
+      st.s += e;
+      st.u = fmaf(e, fmaxf(d, kFar), st.u);
+    }
+  st.s = wave_sum_f32(st.s);
+  st.u = wave_sum_f32(st.u);
+  unsigned rk = 0;
+  int ri = -1;
+  if (TOP) {
+    auto index_at = [&](int i, int j) { return (i * 64 + lane) * kV + j - rv.head; };
+    auto inside = [&](int idx) { return idx >= 0 && idx < a.v; };
+    Best2 b = {0u, 0u, -1, -1};
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        const int idx = index_at(i, j);
+        keep(b, inside(idx) ? rank_of(x[i][j]) : 0u, idx);
+      }
+    take_best(b, a.top, lane, &rk, &ri, [&](int, unsigned k0, int i0, unsigned* nk, int* ni) {
+      Best2 q = {0u, 0u, -1, -1};
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+          const int idx = index_at(i, j);
+          const unsigned k = inside(idx) ? rank_of(x[i][j]) : 0u;
+          if (after(k, idx, k0, i0)) keep(q, k, idx);
+        }
+      *nk = q.k1;
+      *ni = q.i1;
+    });
+  }
+  write_row<T>(a, row, xr, st, lane, rk, ri);
+}
+
+// A piece of a row as k_score_pieces leaves it: 4 words, then top (rank, index) pairs
+__host__ __device__ inline size_t piece_words(int top) { return 4 + 2 * (size_t)top; }
+
+constexpr int kPieceThreads = 256;
+constexpr int kPieceWaves = kPieceThreads / 64;
+
+// Longer rows: a workgroup streams one of `pieces` pieces of a row (pieces > 1 where there are too
+// few rows to fill the card; k_score_join then joins them).
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kPieceThreads) void k_score_pieces(ScoreArgs a, int pieces,
+                                                                unsigned* part) {
+  constexpr int kV = Elem<T>::kVec;
+  __shared__ float sm[kPieceWaves][4];
+  __shared__ unsigned lk[kPieceWaves][32];
+  __shared__ int li[kPieceWaves][32];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = a.row0 + blockIdx.x;
+  const int piece = blockIdx.y;
+  const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
+  const RowView<T> rv(xr, a.v);
+  const float c = a.inv_t * kLog2e;
+  const int64_t total = rv.granules();
+  const int g0 = (int)(total * piece / pieces), g1 = (int)(total * (piece + 1) / pieces);
+  Stats st = {kLowest, 0.0f, 0.0f};
+  Best2 b = {0u, 0u, -1, -1};
+  auto take = [&](const float* x, int g) {
+    if (TOP) {
+      const int j0 = g * kV - rv.head;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        const int idx = j0 + j;
+        keep(b, idx >= 0 && idx < a.v ? rank_of(x[j]) : 0u, idx);
+      }
+    }
+  };
+  int g = g0 + (int)threadIdx.x;
+  // two granules per lane and step: their loads are in flight together
+  for (; g + kPieceThreads < g1; g += 2 * kPieceThreads) {
+    float x[2 * kV];
+    rv.get(g, x);
+    rv.get(g + kPieceThreads, x + kV);
+    add_values<2 * kV>(st, x, c);
+    take(x, g);
+    take(x + kV, g + kPieceThreads);
+  }
+  if (g < g1) {
+    float x[kV];
+    rv.get(g, x);
+    add_values<kV>(st, x, c);
+    take(x, g);
+  }
+  st = wave_join(st, c);
+  if (lane == 0) {
+    sm[wave][0] = st.m;
+    sm[wave][1] = st.s;
+    sm[wave][2] = st.u;
+  }
+  if (TOP) {
+    unsigned rk;
+    int ri;
+    const int t0 = g0 + (wave << 6);
+    take_best(b, a.top, lane, &rk, &ri, [&](int w, unsigned k0, int i0, unsigned* nk, int* ni) {
+      // lane w's granules are t0 + w, + kPieceThreads, ...: the 64 lanes look through them
+      Best2 q = {0u, 0u, -1, -1};
+      for (int64_t h = (int64_t)t0 + w + (int64_t)lane * kPieceThreads; h < g1;
+           h += 64 * kPieceThreads) {
+        float x[kV];
+        rv.get((int)h, x);
+        const int j0 = (int)h * kV - rv.head;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+          const int idx = j0 + j;
+          const unsigned k = idx >= 0 && idx < a.v ? rank_of(x[j]) : 0u;
+          if (after(k, idx, k0, i0)) keep(q, k, idx);
+        }
+      }
+      unsigned kb;
+      const int from = best_lane(q.k1, q.i1, &kb);
+      *nk = kb;
+      *ni = __builtin_amdgcn_readlane(q.i1, from);
+    });
+    if (lane < a.top) {
+      lk[wave][lane] = rk;
+      li[wave][lane] = ri;
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  Stats j = {kLowest, 0.0f, 0.0f};
+  if (lane < kPieceWaves) {
+    j.m = sm[lane][0];
+    j.s = sm[lane][1];
+    j.u = sm[lane][2];
+  }
+  j = wave_join(j, c);
+  unsigned rk = 0;
+  int ri = -1;
+  if (TOP) {
+    // lane w walks wave w's list
+    int at = 0;
+    unsigned k = lane < kPieceWaves ? lk[lane][0] : 0u;
+    int i = lane < kPieceWaves ? li[lane][0] : 0x7fffffff;
+    for (int r = 0; r < a.top; ++r) {
+      unsigned kb;
+      const int w = best_lane(k, i, &kb);
+      const int ib = __builtin_amdgcn_readlane(i, w);
+      if (lane == r) {
+        rk = kb;
+        ri = ib;
+      }
+      if (lane == w) {
+        ++at;
+        k = at < a.top ? lk[w][at] : 0u;
+        i = at < a.top ? li[w][at] : 0x7fffffff;
+      }
+    }
+  }
+  if (pieces == 1) {
+    write_row<T>(a, row, xr, j, lane, rk, ri);
+    return;
+  }
+  unsigned* out = part + ((size_t)row * pieces + piece) * piece_words(a.top);
+  if (lane == 0) {
+    out[0] = __float_as_uint(j.m);
+    out[1] = __float_as_uint(j.s);
+    out[2] = __float_as_uint(j.u);
+  }
+  if (lane < a.top) {
+    out[4 + 2 * lane] = rk;
+    out[5 + 2 * lane] = (unsigned)ri;
+  }
+}
+
+// One wave a row: lane p holds piece p (at most 64 pieces).
+template <typename T>
+__global__ __launch_bounds__(64) void k_score_join(ScoreArgs a, int pieces, const unsigned* part) {
+  const int lane = threadIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
+  const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
+  const bool mine = lane < pieces;
+  const unsigned* in = part + ((size_t)row * pieces + (mine ? lane : 0)) * piece_words(a.top);
+  Stats j = {kLowest, 0.0f, 0.0f};
+  if (mine) {
+    j.m = __uint_as_float(in[0]);
+    j.s = __uint_as_float(in[1]);
+    j.u = __uint_as_float(in[2]);
+  }
+  j = wave_join(j, a.inv_t * kLog2e);
+  unsigned rk = 0;
+  int ri = -1;
+  int at = 0;
+  unsigned k = mine && a.top > 0 ? in[4] : 0u;
+  int i = mine && a.top > 0 ? (int)in[5] : 0x7fffffff;
+  for (int r = 0; r < a.top; ++r) {
+    unsigned kb;
+    const int w = best_lane(k, i, &kb);
+    const int ib = __builtin_amdgcn_readlane(i, w);
+    if (lane == r) {
+      rk = kb;
+      ri = ib;
+    }
+    if (lane == w) {
+      ++at;
+      k = at < a.top ? in[4 + 2 * at] : 0u;
+      i = at < a.top ? (int)in[5 + 2 * at] : 0x7fffffff;
+    }
+  }
+  write_row<T>(a, row, xr, j, lane, rk, ri);
+}
+
+struct GradArgs {
+  const void* logits;
+  int64_t ld;
+  int64_t row0, n;
+  int v;
+  const void* labels;
+  int labels64;
+  float inv_t;
+  const float* lse;
+  const float* entropy;
+  const float* d_logp;      // may be NULL: no gradient through log p
+  const float* d_entropy;   // may be NULL
+  void* out;
+  int64_t ld_out;
+};
+
+// dL/dx_j = ( g (delta_{j,label} - p_j) - h p_j (log p_j + H) ) / T with g = dL/dlogp (0 for a row
+// without a label) and h = dL/dH.  One read of the scores, one write of the gradient (out may be
+// the scores themselves: an element is read before it is written, by the same lane).  A row of few
+// granules is taken by 2^lanes_log2 lanes, 256 >> lanes_log2 rows a workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, int span) {
+  constexpr int kV = Elem<T>::kVec;
+  const int lanes = 1 << lanes_log2;
+  const int64_t row = a.row0 + ((int64_t)blockIdx.x << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+  if (row >= a.n) return;
+  const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
+  T* yr = static_cast<T*>(a.out) + row * a.ld_out;
+  const float lse = a.lse[row];
+  int64_t l = -1;
+  if (a.labels && a.d_logp)
+    l = a.labels64 ? static_cast<const int64_t*>(a.labels)[row]
+                   : (int64_t) static_cast<const int32_t*>(a.labels)[row];
+  const int label = l >= 0 && l < a.v ? (int)l : -1;
+  const float g = label >= 0 ? a.d_logp[row] : 0.0f;
+  const float h = a.d_entropy ? a.d_entropy[row] : 0.0f;
+  const float H = a.d_entropy ? a.entropy[row] : 0.0f;
+  const bool none = lse == -__builtin_inff();
+  const RowView<T> rv(xr, a.v);
+  const int total = rv.granules();
+  const int g0 = (int)blockIdx.y * span;
+  const int g1 = total - g0 < span ? total : g0 + span;
+  // the output row starts at the same place of a granule as the input row
+  const bool same = (reinterpret_cast<uintptr_t>(yr) & 15) == (reinterpret_cast<uintptr_t>(xr) & 15);
+  char* yb = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(yr) & ~(uintptr_t)15);
+  for (int q = g0 + ((int)threadIdx.x & (lanes - 1)); q < g1; q += lanes) {
+    float x[kV];
+    rv.get(q, x);
+    const int j0 = q * kV - rv.head;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const float lq = fmaxf(fmaf(x[i], a.inv_t, -lse), kFar) + 0.0f * lse;
+      const float p = __builtin_amdgcn_exp2f(lq * kLog2e);
+      float d = -p * fmaf(h, lq + H, g);
+      d = (j0 + i == label ? d + g : d) * a.inv_t;
+      x[i] = none ? 0.0f : d;
+    }
+    if (same && j0 >= 0 && j0 + kV <= a.v) {
+      *reinterpret_cast<u32x4*>(yb + (size_t)q * 16) = Elem<T>::pack(x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        if (j0 + i >= 0 && j0 + i < a.v) Elem<T>::store(yr + j0 + i, x[i]);
+    }
+  }
+}
+
+// rows of one launch: the launch's threads are counted in 32 bits
+constexpr int64_t kRowsPerLaunch = (int64_t)1 << 22;
+
+template <typename T, bool TOP>
+hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) {
+  // the longest row a wave keeps in registers: 8 granules a lane (one more than the row's length
+  // asks for, because a row may start inside a granule)
+  const int64_t granules = ((int64_t)a.v + 2 * Elem<T>::kVec - 2) / Elem<T>::kVec;
+  const int64_t n = a.n;
+  for (a.row0 = 0; a.row0 < n; a.row0 += kRowsPerLaunch) {
+    const int64_t rows = n - a.row0 < kRowsPerLaunch ? n - a.row0 : kRowsPerLaunch;
+    a.n = a.row0 + rows;
+    const dim3 by4((unsigned)((rows + 3) / 4));
+    if (granules <= 64) {
+      hipLaunchKernelGGL((k_score_wave<T, 1, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 128) {
+      hipLaunchKernelGGL((k_score_wave<T, 2, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 256) {
+      hipLaunchKernelGGL((k_score_wave<T, 4, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 512) {
+      hipLaunchKernelGGL((k_score_wave<T, 8, TOP>), by4, dim3(256), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((k_score_pieces<T, TOP>), dim3((unsigned)rows, (unsigned)pieces),
+                         dim3(kPieceThreads), 0, s, a, pieces, part);
+      if (pieces > 1)
+        hipLaunchKernelGGL(k_score_join<T>, dim3((unsigned)rows), dim3(64), 0, s, a, pieces, part);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T>
+hipError_t grad_launch(GradArgs a, hipStream_t s) {
+  const int64_t granules = ((int64_t)a.v + 2 * Elem<T>::kVec - 2) / Elem<T>::kVec;
+  int lanes_log2 = 1;
+  while (lanes_log2 < 8 && (1 << lanes_log2) < granules) ++lanes_log2;
+  // a workgroup takes 2048 granules of a row, fewer when that leaves CUs without work
+  int64_t span = 2048;
+  while (span > 256 && a.n * ((granules + span - 1) / span) < 8 * (int64_t)kCUs) span /= 2;
+  while ((granules + span - 1) / span > 65535) span *= 2;
+  const unsigned y = (unsigned)((granules + span - 1) / span);
+  const int64_t n = a.n;
+  for (a.row0 = 0; a.row0 < n; a.row0 += kRowsPerLaunch) {
+    const int64_t rows = n - a.row0 < kRowsPerLaunch ? n - a.row0 : kRowsPerLaunch;
+    a.n = a.row0 + rows;
+    const int64_t per_wg = 256 >> lanes_log2;
+    hipLaunchKernelGGL(k_score_grad<T>, dim3((unsigned)((rows + per_wg - 1) / per_wg), y), dim3(256), 0,
+                       s, a, lanes_log2, (int)span);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+int score_pieces(int64_t n, int64_t v, int dtype) {
+  const int vec = dtype == IC_F32 ? 4 : 8;
+  const int64_t granules = (v + 2 * vec - 2) / vec;
+  if (granules <= 64 * 8 || n == 0) return 1;
+  // four workgroups a CU, and at least two granules a lane in a piece
+  int64_t p = (4 * (int64_t)kCUs + n - 1) / n;
+  const int64_t most = granules / (2 * kPieceThreads);
+  if (p > most) p = most;
+  return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
+}
+
+size_t score_scratch_bytes(int64_t n, int pieces, int top) {
+  return pieces > 1 ? (size_t)n * pieces * piece_words(top) * 4 : 0;
+}
+
+hipError_t launch_label_logprobs(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v,
+                                 const void* labels, int labels64, float inv_t, int top, float* logp,
+                                 float* entropy, float* lse, float* top_logp, int32_t* top_idx,
+                                 int pieces, void* scratch, hipStream_t s) {
+  const ScoreArgs a{logits, ld, 0, n, (int)v, labels, labels64, inv_t, top, logp, entropy, lse, top_logp,
+                    top_idx};
+  unsigned* part = static_cast<unsigned*>(scratch);
+  if (dtype == IC_F32)
+    return top ? score_launch<float, true>(a, pieces, part, s) : score_launch<float, false>(a, pieces, part, s);
+  if (dtype == IC_BF16)
+    return top ? score_launch<bf16_t, true>(a, pieces, part, s) : score_launch<bf16_t, false>(a, pieces, part, s);
+  return top ? score_launch<f16_t, true>(a, pieces, part, s) : score_launch<f16_t, false>(a, pieces, part, s);
+}
+
+hipError_t launch_label_logprobs_grad(const void* logits, int dtype, int64_t ld, int64_t n, int64_t v,
+                                      const void* labels, int labels64, float inv_t, const float* lse,
+                                      const float* entropy, const float* d_logp,
+                                      const float* d_entropy, void* out, int64_t ld_out, hipStream_t s) {
+  const GradArgs a{logits, ld, 0, n, (int)v, labels, labels64, inv_t, lse, entropy, d_logp, d_entropy, out,
+                   ld_out};
+  if (dtype == IC_F32) return grad_launch<float>(a, s);
+  if (dtype == IC_BF16) return grad_launch<bf16_t>(a, s);
+  return grad_launch<f16_t>(a, s);
+}
+
+}  // namespace ic

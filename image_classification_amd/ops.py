@@ -909,6 +909,393 @@ def ransac_homography(pts, offsets, n_iter, th, samples=None, seed=0, min_inlier
     return H, n_inl, err, best_it, mask
 
 
+# -- what is learned on top of the codes -------------------------------------------------------------
+# Launches only: memory a call needs for itself is allocated here, from torch's allocator on the
+# current stream, so these calls may be captured into a graph and used on any stream.
+_TYPE_NUMBER = {torch.float32: _lib.IC_F32, torch.bfloat16: _lib.IC_BF16, torch.float16: _lib.IC_F16}
+MAX_TOP = 32                 # alternatives label_logprobs returns per row
+MAX_GROUPS = 1 << 26
+
+
+def _type_number(t, name):
+    code = _TYPE_NUMBER.get(t.dtype)
+    if code is None:
+        raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return code
+
+
+def _check_rows(t, name):
+    """A matrix of unit-stride rows (a slice of a wider one is fine); returns its row stride."""
+    if t.dim() != 2:
+        raise ValueError("%s must be 2-D, got shape %s" % (name, tuple(t.shape)))
+    n, d = t.shape
+    if n <= 1 or d == 0:
+        if d > 1 and t.stride(1) != 1:
+            raise ValueError("the elements of a row of %s must be adjacent" % name)
+        return max(d, 1)
+    if (d > 1 and t.stride(1) != 1) or t.stride(0) < d:
+        raise ValueError("%s must have adjacent elements in a row and rows that do not overlap "
+                         "(strides %s)" % (name, tuple(t.stride())))
+    return t.stride(0)
+
+
+def _check_same_device(dev, *named):
+    for t, name in named:
+        if t is not None and t.device != dev:
+            raise ValueError("%s lives on %s, expected %s" % (name, t.device, dev))
+
+
+def _scratch(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def group_rows(codes, n_groups):
+    """(order int32 [n], offsets int64 [n_groups + 1]): the rows of each code one after the other,
+    in their order; group g is order[offsets[g]:offsets[g + 1]].  Rows whose code is outside
+    [0, n_groups) (-1: no codeword) belong to no group and come last.  codes int32 [n]."""
+    if codes.dtype != torch.int32 or codes.dim() != 1:
+        raise ValueError("codes must be int32 with one entry per row")
+    n_groups = int(n_groups)
+    if not 1 <= n_groups <= MAX_GROUPS:
+        raise ValueError("n_groups must be in [1, %d], got %d" % (MAX_GROUPS, n_groups))
+    dev = _dev_index(codes)
+    codes = codes.contiguous()
+    n = codes.shape[0]
+    order = torch.empty(n, dtype=torch.int32, device=codes.device)
+    offsets = torch.empty(n_groups + 1, dtype=torch.int64, device=codes.device)
+    lib = _lib.load()
+    nbytes = lib.ic_group_rows_scratch(n, n_groups)
+    scratch = _scratch(nbytes, codes.device)
+    rc = lib.ic_group_rows(_lib.handle(dev), _ptr(codes), n, n_groups, _ptr(order), _ptr(offsets),
+                           _ptr(scratch), nbytes, _stream_ptr(dev))
+    _lib.check(rc, "ic_group_rows")
+    return order, offsets
+
+
+def _check_groups(offsets, order, n, n_groups, device):
+    if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] != n_groups + 1 \
+            or not offsets.is_contiguous():
+        raise ValueError("offsets must be contiguous int64 [n_groups + 1] = [%d]" % (n_groups + 1))
+    if order is not None and (order.dtype != torch.int32 or order.dim() != 1 or order.shape[0] != n
+                              or not order.is_contiguous()):
+        raise ValueError("order must be contiguous int32 with one entry per row")
+    _check_same_device(device, (offsets, "offsets"), (order, "order"))
+
+
+def _check_group_matrices(w):
+    if w.dim() != 3 or not w.is_contiguous():
+        raise ValueError("w must be contiguous [n_groups, out, k], got shape %s" % (tuple(w.shape),))
+    if w.shape[0] < 1 or w.shape[1] < 1 or w.shape[2] < 1:
+        raise ValueError("w must not be empty, got shape %s" % (tuple(w.shape),))
+    if w.shape[0] > MAX_GROUPS:
+        raise ValueError("at most %d groups, got %d" % (MAX_GROUPS, w.shape[0]))
+
+
+def _result(out, out_dtype, shape, like, name):
+    """(tensor, its type number) for a result of `shape`: `out`, or a new one."""
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or like.dtype, device=like.device)
+    elif tuple(out.shape) != tuple(shape) or out.device != like.device or \
+            (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("out must be a %s tensor on %s" % (tuple(shape), like.device))
+    if out.dtype != like.dtype and out.dtype != torch.float32:
+        raise ValueError("%s is %s or float32, not %s" % (name, like.dtype, out.dtype))
+    return out, _type_number(out, name)
+
+
+def _grouped_rows(fn_name, x, w, offsets, order, out, out_dtype, dx):
+    _check_group_matrices(w)
+    groups, o, k = w.shape
+    ld_x = _check_rows(x, "dy" if dx else "x")
+    width, cols = (o, k) if dx else (k, o)
+    if x.shape[1] != width:
+        raise ValueError("dimension mismatch: rows have %d columns, w is %s"
+                         % (x.shape[1], tuple(w.shape)))
+    if x.dtype != w.dtype:
+        raise ValueError("rows are %s, w is %s" % (x.dtype, w.dtype))
+    t = _type_number(x, "rows")
+    dev = _dev_index(x)
+    _check_same_device(x.device, (w, "w"))
+    n = x.shape[0]
+    _check_groups(offsets, order, n, groups, x.device)
+    y, yt = _result(out, out_dtype, (n, cols), x, "the result")
+    ld_y = _check_rows(y, "out")
+    lib = _lib.load()
+    rc = getattr(lib, fn_name)(_lib.handle(dev), _ptr(x), ld_x, _ptr(w), _ptr(y), ld_y, _ptr(offsets),
+                               _ptr(order), n, groups, k, o, t, yt, _stream_ptr(dev))
+    _lib.check(rc, fn_name)
+    return y
+
+
+def grouped_matmul(x, w, offsets, order=None, out=None, out_dtype=None):
+    """y[i] = w[g] @ x[i] for every row i of group g, zeros for rows of no group.
+
+    x [n, k], w [n_groups, out, k] of the same type (float32, bfloat16, float16; sums are float32);
+    (order, offsets) as group_rows returns them -- order=None: the rows lie group by group, row i in
+    group g when offsets[g] <= i < offsets[g + 1].  Returns y [n, out] of x's type or `out_dtype`
+    (float32); `out`: a tensor to write to, which must share no memory with x or w.  Rows may lie
+    apart (a column slice of a wider matrix); order must name every row once."""
+    return _grouped_rows("ic_grouped_matmul", x, w, offsets, order, out, out_dtype, False)
+
+
+def grouped_matmul_dx(dy, w, offsets, order=None, out=None, out_dtype=None):
+    """dx[i] = w[g].T @ dy[i]: the gradient of grouped_matmul with respect to x.  dy [n, out]."""
+    return _grouped_rows("ic_grouped_matmul_dx", dy, w, offsets, order, out, out_dtype, True)
+
+
+def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
+    """dw[g] = sum of outer(dy[i], x[i]) over the rows i of group g (zeros for a group without
+    rows): the gradient of grouped_matmul with respect to w.  dy [n, out], x [n, k] of one type;
+    returns [n_groups, out, k] of that type or `out_dtype` (float32).  The same inputs give the
+    same bits."""
+    ld_dy, ld_x = _check_rows(dy, "dy"), _check_rows(x, "x")
+    if dy.shape[0] != x.shape[0]:
+        raise ValueError("dy has %d rows, x %d" % (dy.shape[0], x.shape[0]))
+    if dy.dtype != x.dtype:
+        raise ValueError("dy is %s, x is %s" % (dy.dtype, x.dtype))
+    if dy.shape[1] < 1 or x.shape[1] < 1:
+        raise ValueError("rows must not be empty")
+    t = _type_number(x, "rows")
+    dev = _dev_index(x)
+    _check_same_device(x.device, (dy, "dy"))
+    groups = offsets.shape[0] - 1 if offsets.dim() == 1 else 0
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError("offsets must be int64 [n_groups + 1]")
+    n, o, k = x.shape[0], dy.shape[1], x.shape[1]
+    _check_groups(offsets, order, n, groups, x.device)
+    dw, yt = _result(out, out_dtype, (groups, o, k), x, "the result")
+    if not dw.is_contiguous():
+        raise ValueError("out must be contiguous")
+    lib = _lib.load()
+    nbytes = lib.ic_grouped_matmul_dw_scratch(n, k, o)
+    scratch = _scratch(nbytes, x.device)
+    rc = lib.ic_grouped_matmul_dw(_lib.handle(dev), _ptr(dy), ld_dy, _ptr(x), ld_x, _ptr(dw),
+                                  _ptr(offsets), _ptr(order), n, groups, k, o, t, yt, _ptr(scratch),
+                                  nbytes, _stream_ptr(dev))
+    _lib.check(rc, "ic_grouped_matmul_dw")
+    return dw
+
+
+def _check_labels(labels, n, device):
+    if labels is None:
+        return 0
+    if labels.dtype not in (torch.int32, torch.int64) or labels.dim() != 1 or labels.shape[0] != n \
+            or not labels.is_contiguous():
+        raise ValueError("labels must be contiguous int32 or int64 with one entry per row")
+    _check_same_device(device, (labels, "labels"))
+    return 1 if labels.dtype == torch.int64 else 0
+
+
+def _inverse_temperature(temperature):
+    temperature = float(temperature)
+    if not 1e-30 < temperature < 1e30:
+        raise ValueError("temperature must be positive and finite, got %r" % temperature)
+    return 1.0 / temperature
+
+
+def label_logprobs(logits, labels=None, top=0, temperature=1.0):
+    """(logp, entropy, lse, top_logp, top_idx) of every row of scores, one read of them.
+
+    With z = logits / temperature: lse = log(sum(exp(z))), p = exp(z - lse), entropy =
+    -sum(p log p), logp = log p of the row's label (0 where the label is outside [0, v): no label;
+    None without labels), all float32 [n]; top_logp float32 / top_idx int32 [n, top] = the `top`
+    largest scores' log p and index, descending, equal scores by ascending index (None for top=0,
+    at most 32).  logits [n, v] float32, bfloat16 or float16, rows may lie apart.
+
+    Scores of -inf have probability 0; a row of nothing else gives lse = -inf, logp = -inf and
+    entropy = 0.  NaN or +inf in a row makes its results NaN."""
+    ld = _check_rows(logits, "logits")
+    n, v = logits.shape
+    t = _type_number(logits, "logits")
+    if v < 1:
+        raise ValueError("logits have no columns")
+    top = int(top)
+    if not 0 <= top <= min(MAX_TOP, v):
+        raise ValueError("top must be in [0, min(%d, %d columns)], got %d" % (MAX_TOP, v, top))
+    inv = _inverse_temperature(temperature)
+    dev = _dev_index(logits)
+    device = logits.device
+    l64 = _check_labels(labels, n, device)
+    stats = torch.empty((3, n), dtype=torch.float32, device=device)
+    logp = stats[2] if labels is not None else None
+    top_logp = top_idx = None
+    if top:
+        top_logp = torch.empty((n, top), dtype=torch.float32, device=device)
+        top_idx = torch.empty((n, top), dtype=torch.int32, device=device)
+    lib = _lib.load()
+    nbytes = lib.ic_label_logprobs_scratch(n, v, t, top)
+    scratch = _scratch(nbytes, device)
+    rc = lib.ic_label_logprobs(_lib.handle(dev), _ptr(logits), ld, n, v, t, _ptr(labels), l64, inv, top,
+                               _ptr(logp), _ptr(stats[0]), _ptr(stats[1]), _ptr(top_logp),
+                               _ptr(top_idx), _ptr(scratch), nbytes, _stream_ptr(dev))
+    _lib.check(rc, "ic_label_logprobs")
+    return logp, stats[0], stats[1], top_logp, top_idx
+
+
+def _check_vector(t, name, n, device):
+    if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n
+                          or not t.is_contiguous() or t.device != device):
+        raise ValueError("%s must be contiguous float32 with one entry per row, on %s" % (name, device))
+
+
+def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=None, temperature=1.0,
+                        out=None):
+    """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to logits, in logits'
+    type.  lse and entropy are what label_logprobs returned for the same logits and temperature;
+    d_logp / d_entropy float32 [n] (None: zeros).  `out` may be logits itself.  Rows without a
+    label have no gradient through logp; rows of nothing but -inf have none at all."""
+    ld = _check_rows(logits, "logits")
+    n, v = logits.shape
+    t = _type_number(logits, "logits")
+    if v < 1:
+        raise ValueError("logits have no columns")
+    inv = _inverse_temperature(temperature)
+    dev = _dev_index(logits)
+    device = logits.device
+    l64 = _check_labels(labels, n, device)
+    if d_logp is not None and labels is None:
+        raise ValueError("d_logp needs labels")
+    for q, name in ((lse, "lse"), (entropy, "entropy"), (d_logp, "d_logp"), (d_entropy, "d_entropy")):
+        _check_vector(q, name, n, device)
+    if lse is None or (d_entropy is not None and entropy is None):
+        raise ValueError("lse is needed, and entropy where d_entropy is given")
+    if out is None:
+        out = torch.empty((n, v), dtype=logits.dtype, device=device)
+    elif out.dtype != logits.dtype or tuple(out.shape) != (n, v) or out.device != device:
+        raise ValueError("out must be a %s %s tensor on %s" % (logits.dtype, (n, v), device))
+    ld_out = _check_rows(out, "out")
+    rc = _lib.load().ic_label_logprobs_grad(
+        _lib.handle(dev), _ptr(logits), ld, n, v, t, _ptr(labels), l64, inv, _ptr(lse), _ptr(entropy),
+        _ptr(d_logp), _ptr(d_entropy), _ptr(out), ld_out, _stream_ptr(dev))
+    _lib.check(rc, "ic_label_logprobs_grad")
+    return out
+
+
+# one row of the table adamw_step hands over: struct ic_adamw_tensor
+_ADAMW_TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("n", "<i8"), ("state_offset", "<i8"),
+                          ("param_dtype", "<i4"), ("grad_dtype", "<i4")])
+ADAMW_BLOCK = _lib.IC_ADAMW_BLOCK
+
+
+def adamw_state_size(params):
+    """Elements of the flat optimizer states of these tensors: each starts at a multiple of
+    ADAMW_BLOCK, in the order of the list."""
+    return sum((p.numel() + ADAMW_BLOCK - 1) // ADAMW_BLOCK * ADAMW_BLOCK for p in params)
+
+
+def adamw_states(params, bits=32):
+    """(exp_avg, exp_avg_sq, scales) for a first step: zeros.  bits=32: float32, scales None;
+    bits=8: uint8 codes with float32 scales [2, size / ADAMW_BLOCK]."""
+    if bits not in (8, 32):
+        raise ValueError("states have 8 or 32 bits, not %r" % (bits,))
+    size = adamw_state_size(params)
+    device = params[0].device if params else None
+    dtype = torch.float32 if bits == 32 else torch.uint8
+    m, v = (torch.zeros(size, dtype=dtype, device=device) for _ in range(2))
+    scales = None if bits == 32 else torch.zeros((2, size // ADAMW_BLOCK), dtype=torch.float32,
+                                                 device=device)
+    return m, v, scales
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=0.01, scales=None, grad_scale=1.0):
+    """One AdamW step (decoupled weight decay) over all tensors of the lists, in place:
+
+        g = grad_scale * grad
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        p -= lr * weight_decay * p + lr * (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)
+
+    params / grads: contiguous float32, bfloat16 or float16 tensors in any mix, one gradient per
+    parameter of the same number of elements; no two parameters may share memory.  exp_avg,
+    exp_avg_sq, scales: flat states as adamw_states makes them, for this list in this order.  With
+    uint8 states, ADAMW_BLOCK elements share a scale (adamw_state_values gives their values).
+    lr: a number, or a float32 device tensor of one element; step: a number counted from 1, or an
+    int64 device tensor of one element -- a captured step reads them at every replay."""
+    count = len(params)
+    if len(grads) != count:
+        raise ValueError("%d parameters, %d gradients" % (count, len(grads)))
+    if exp_avg.dtype == torch.float32:
+        bits = 32
+        if scales is not None:
+            raise ValueError("float32 states have no scales")
+    elif exp_avg.dtype == torch.uint8:
+        bits = 8
+    else:
+        raise ValueError("states are float32 or uint8, not %s" % exp_avg.dtype)
+    device = exp_avg.device
+    dev = _dev_index(exp_avg)
+    if exp_avg_sq.dtype != exp_avg.dtype or exp_avg_sq.device != device or exp_avg.dim() != 1 \
+            or exp_avg_sq.shape != exp_avg.shape or not exp_avg.is_contiguous() \
+            or not exp_avg_sq.is_contiguous():
+        raise ValueError("exp_avg and exp_avg_sq must be flat, contiguous and alike")
+    table = np.empty(count, dtype=_ADAMW_TENSOR)
+    rows = []
+    at = 0
+    types = _TYPE_NUMBER
+    for p, g in zip(params, grads):
+        n = p.numel()
+        if g.numel() != n or p.device != device or g.device != device:
+            raise ValueError("a gradient must match its parameter, on the states' device")
+        if not (p.is_contiguous() and g.is_contiguous()):
+            raise ValueError("parameters and gradients must be contiguous")
+        try:
+            rows.append((p.data_ptr(), g.data_ptr(), n, at, types[p.dtype], types[g.dtype]))
+        except KeyError:
+            raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
+        at += (n + ADAMW_BLOCK - 1) // ADAMW_BLOCK * ADAMW_BLOCK
+    size = exp_avg.shape[0]
+    if at != size:
+        raise ValueError("the states have %d elements, these tensors need %d" % (size, at))
+    if bits == 8 and (scales is None or scales.dtype != torch.float32 or scales.device != device
+                      or tuple(scales.shape) != (2, size // ADAMW_BLOCK) or not scales.is_contiguous()):
+        raise ValueError("uint8 states need contiguous float32 scales [2, %d]" % (size // ADAMW_BLOCK))
+    if count == 0:
+        return
+    table[:] = rows
+    lr_t = step_t = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
+            raise ValueError("lr must be a number or a float32 tensor of one element on %s" % device)
+        lr_t, lr = lr, 0.0
+    if isinstance(step, torch.Tensor):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.device != device:
+            raise ValueError("step must be a number or an int64 tensor of one element on %s" % device)
+        step_t, step = step, 1
+    if step < 1:
+        raise ValueError("step counts from 1, got %r" % (step,))
+    b1, b2 = float(betas[0]), float(betas[1])
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not eps >= 0:
+        raise ValueError("betas must be in [0, 1) and eps must not be negative")
+    rc = _lib.load().ic_adamw_step(
+        _lib.handle(dev), table.ctypes.data, count, bits, _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(scales),
+        size, float(lr), _ptr(lr_t), b1, b2, float(eps), float(weight_decay), int(step), _ptr(step_t),
+        float(grad_scale), _stream_ptr(dev))
+    _lib.check(rc, "ic_adamw_step")
+
+
+def adamw_state_values(exp_avg, exp_avg_sq, scales=None):
+    """(m, v) float32: the values that 8-bit states stand for (32-bit states are returned as they
+    are)."""
+    if exp_avg.dtype == torch.float32:
+        return exp_avg, exp_avg_sq
+    size = exp_avg.shape[0]
+    if exp_avg.dtype != torch.uint8 or exp_avg_sq.dtype != torch.uint8 \
+            or exp_avg.shape != exp_avg_sq.shape or exp_avg.dim() != 1 or size % ADAMW_BLOCK \
+            or not exp_avg.is_contiguous() or not exp_avg_sq.is_contiguous():
+        raise ValueError("states must be flat uint8 of a multiple of %d elements" % ADAMW_BLOCK)
+    if scales is None or scales.dtype != torch.float32 or not scales.is_contiguous() \
+            or tuple(scales.shape) != (2, size // ADAMW_BLOCK):
+        raise ValueError("uint8 states need contiguous float32 scales [2, %d]" % (size // ADAMW_BLOCK))
+    dev = _dev_index(exp_avg)
+    _check_same_device(exp_avg.device, (exp_avg_sq, "exp_avg_sq"), (scales, "scales"))
+    m = torch.empty(size, dtype=torch.float32, device=exp_avg.device)
+    v = torch.empty(size, dtype=torch.float32, device=exp_avg.device)
+    rc = _lib.load().ic_adamw_state_values(_lib.handle(dev), _ptr(exp_avg), _ptr(exp_avg_sq),
+                                           _ptr(scales), size, _ptr(m), _ptr(v), _stream_ptr(dev))
+    _lib.check(rc, "ic_adamw_state_values")
+    return m, v
+
+
 def reserve_workspace(device_index, nbytes):
     """Grow the handle's device workspace to at least `nbytes` now, so that later calls of known
     size do not allocate."""

@@ -60,6 +60,14 @@ extern "C" {
 #define IC_METRIC_INTERSECTION 3 /* sum min(a,b)             model/clustering.py:309-310        */
 #define IC_METRIC_CHISQR 4       /* sum (a-b)^2/a over a!=0  model/clustering.py:305-306        */
 
+/* element types of the entry points that take more than float32 */
+#define IC_F32 0
+#define IC_BF16 1
+#define IC_F16 2
+
+/* 8-bit optimizer states: elements that share one scale */
+#define IC_ADAMW_BLOCK 256
+
 /* per-row partial result exchanged between shards / K-splits (16 bytes) */
 typedef struct ic_top2_rec {
   float d1;   /* best distance (Euclidean, not squared) */
@@ -307,6 +315,99 @@ int ic_ransac_homography(void* handle, const double* pts, const int64_t* offsets
  * float32) or float64 when kind[j] == 1 (converted to float32).  All pointers are HOST memory. */
 int ic_host_gather_f32(float* dst, const void* const* src, const int64_t* elems,
                        const int32_t* kind, int64_t n_jobs, int threads);
+
+/* ---- products grouped by codeword, label log probabilities, AdamW --------------------------------
+ * What is learned on top of the codes: a matrix per codeword (a projection per visual word, a linear
+ * classifier per pyramid cell), probabilities over a vocabulary or a label set, and the optimizer
+ * step that trains both.  The reference leaves this to libsvm (model/classifiers.py:218,
+ * vision/utils/bovw_functions.py:133-159) and external binaries; these entry points have no one
+ * call there that they replace.
+ *
+ * All of them consist of kernel launches on `stream` only: no allocation, no event, no
+ * synchronisation, no state in the handle, so they may be captured into a graph and called from
+ * several threads at once.  Where a call needs memory of its own the caller passes `scratch` (device,
+ * 16-byte aligned) of at least the size that the *_scratch function of the same arguments returns;
+ * two calls that may run at the same time need a scratch each.  Sums are float32. */
+
+/* Groups rows by code: order [n] int32 = the rows with codes[i] == 0, then 1, ..., ascending inside a
+ * group; rows whose code is outside [0, n_groups) come last.  offsets [n_groups + 1] int64: group g is
+ * order[offsets[g]] .. order[offsets[g + 1] - 1].  0 <= n < 2^31, 1 <= n_groups <= 2^26. */
+int64_t ic_group_rows_scratch(int64_t n, int64_t n_groups);
+int ic_group_rows(void* handle, const int32_t* codes, int64_t n, int64_t n_groups, int32_t* order,
+                  int64_t* offsets, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* y_i = W_g x_i for every row i of group g; rows of no group get zeros.
+ *   x [n][k] with rows ld_x elements apart, w [n_groups][out][k], y [n][out] with rows ld_y apart.
+ *   offsets [n_groups + 1] ascending from 0 (device); order [n] (device) holds every row once, as
+ *   ic_group_rows writes it, or is NULL: the rows lie group by group.  An entry of order that is no
+ *   row is passed over; offsets are used as if clamped to [0, n].
+ *   dtype: of x and w; y_dtype: the same, or IC_F32.
+ * 1 <= k, out; 0 <= n < 2^31.  Rows and matrices that are 16-byte aligned, with widths of a
+ * multiple of 16 bytes, take the fast path. */
+int ic_grouped_matmul(void* handle, const void* x, int64_t ld_x, const void* w, void* y, int64_t ld_y,
+                      const int64_t* offsets, const int32_t* order, int64_t n, int64_t n_groups, int k,
+                      int out, int dtype, int y_dtype, void* stream);
+/* dx_i = W_g^T dy_i (zeros for rows of no group): the gradient of ic_grouped_matmul with respect to x.
+ *   dy [n][out], dx [n][k]. */
+int ic_grouped_matmul_dx(void* handle, const void* dy, int64_t ld_dy, const void* w, void* dx,
+                         int64_t ld_dx, const int64_t* offsets, const int32_t* order, int64_t n,
+                         int64_t n_groups, int k, int out, int dtype, int y_dtype, void* stream);
+/* dW_g = sum over the rows i of group g of dy_i x_i^T (zeros for a group without rows): the gradient
+ * with respect to w.  dw [n_groups][out][k].  The order of every sum is fixed. */
+int64_t ic_grouped_matmul_dw_scratch(int64_t n, int k, int out);
+int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                         void* dw, const int64_t* offsets, const int32_t* order, int64_t n,
+                         int64_t n_groups, int k, int out, int dtype, int y_dtype, void* scratch,
+                         int64_t scratch_bytes, void* stream);
+
+/* Per row of scores, with z = logits * inv_temperature: lse = log sum_j e^{z_j}, entropy =
+ * -sum_j p_j log p_j (natural logarithm), logp = log p of the row's label, and the `top` best
+ * alternatives by descending score, ties by ascending index (0 <= top <= 32, top <= v).
+ *   logits [n][v] with rows ld elements apart, labels [n] int32 (labels64 == 0) or int64, or NULL;
+ *   a label outside [0, v) marks a row without one: logp = 0.  logp may be NULL.
+ *   lse, entropy, logp [n] f32, top_logp [n][top] f32, top_idx [n][top] int32 (NULL when top == 0).
+ * Scores of -inf have probability 0; a row of nothing else has lse = -inf, entropy = 0, logp = -inf.
+ * A row that holds NaN or +inf has NaN results (its alternatives' indices are still ranked, NaN
+ * first). */
+int64_t ic_label_logprobs_scratch(int64_t n, int64_t v, int dtype, int top);
+int ic_label_logprobs(void* handle, const void* logits, int64_t ld, int64_t n, int64_t v, int dtype,
+                      const void* labels, int labels64, float inv_temperature, int top, float* logp,
+                      float* entropy, float* lse, float* top_logp, int32_t* top_idx, void* scratch,
+                      int64_t scratch_bytes, void* stream);
+/* dlogits = the gradient of sum_i d_logp[i] logp[i] + d_entropy[i] entropy[i], in the scores' type.
+ * lse and entropy are what ic_label_logprobs returned; d_logp or d_entropy may be NULL (zeros).
+ * out [n][v] with rows ld_out apart may be the scores themselves (same pointer and ld). */
+int ic_label_logprobs_grad(void* handle, const void* logits, int64_t ld, int64_t n, int64_t v, int dtype,
+                           const void* labels, int labels64, float inv_temperature, const float* lse,
+                           const float* entropy, const float* d_logp, const float* d_entropy, void* out,
+                           int64_t ld_out, void* stream);
+
+/* One tensor of an AdamW step.  Its states begin at element state_offset (a multiple of
+ * IC_ADAMW_BLOCK) of the flat state arrays and take n elements rounded up to that. */
+typedef struct ic_adamw_tensor {
+  void* param;          /* device, updated in place */
+  const void* grad;     /* device */
+  int64_t n;
+  int64_t state_offset;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+} ic_adamw_tensor;
+
+/* AdamW with decoupled weight decay over all tensors:
+ *   g' = grad_scale g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2;
+ *   p -= lr weight_decay p + lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ *   tensors [count] (HOST).  state_bits 32: exp_avg, exp_avg_sq [state_elements] f32.  state_bits 8:
+ *   they are codes [state_elements] uint8 with scales [2][state_elements / IC_ADAMW_BLOCK] f32
+ *   (all zeros to begin with); ic_adamw_state_values gives the values that they stand for.
+ *   lr_dev (f32) and step_dev (int64), device, are read instead of lr and step when they are not NULL
+ *   (a captured step then follows them).  step >= 1.  No two tensors may share memory. */
+int ic_adamw_step(void* handle, const ic_adamw_tensor* tensors, int64_t count, int state_bits,
+                  void* exp_avg, void* exp_avg_sq, float* scales, int64_t state_elements, double lr,
+                  const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,
+                  int64_t step, const int64_t* step_dev, float grad_scale, void* stream);
+int ic_adamw_state_values(void* handle, const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                          const float* scales, int64_t state_elements, float* out_avg,
+                          float* out_avg_sq, void* stream);
 
 #ifdef __cplusplus
 }

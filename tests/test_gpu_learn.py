@@ -1,0 +1,715 @@
+"""Products grouped by codeword, label log probabilities and the AdamW step against their formulas in
+float64.  Tolerances count roundings: u = 2^-24 per float32 operation, finfo(t).eps / 2 for a result
+stored in type t."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from image_classification_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda:0"
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+# -- group_rows ---------------------------------------------------------------------------------------
+def grouping(codes, groups):
+    c = np.asarray(codes)
+    key = np.where((c >= 0) & (c < groups), c, groups)
+    order = np.argsort(key, kind="stable")
+    return order.astype(np.int32), np.searchsorted(key[order], np.arange(groups + 1))
+
+
+@pytest.mark.parametrize("n,groups", [
+    (0, 1), (0, 5000), (1, 1), (1, 70000), (2, 3), (63, 7), (64, 64), (65, 1000), (511, 2), (512, 9),
+    (513, 300), (2047, 5), (4096, 4096), (4096, 1), (4097, 1), (4097, 511), (5000, 512), (8192, 70000),
+    (12289, 10000), (100003, 37), (300000, 300000), (70000, 1 << 20)])
+@pytest.mark.parametrize("kind", ["even", "skewed", "one", "none"])
+def test_group_rows(n, groups, kind):
+    rng = np.random.default_rng(n * 31 + groups)
+    if kind == "even":
+        c = rng.integers(-2, groups + 2, n)
+    elif kind == "skewed":
+        c = np.minimum((rng.random(n) ** 6 * groups).astype(np.int64), groups - 1)
+        c[rng.random(n) < 0.1] = -1
+    elif kind == "one":
+        c = np.full(n, groups - 1)
+    else:
+        c = rng.choice([-1, groups, 2 ** 31 - 1, -2 ** 31], n)
+    c = c.astype(np.int32)
+    order, offsets = ops.group_rows(torch.from_numpy(c).to(DEV), groups)
+    ro, rf = grouping(c, groups)
+    assert order.dtype == torch.int32 and offsets.dtype == torch.int64
+    assert np.array_equal(order.cpu().numpy(), ro)
+    assert np.array_equal(offsets.cpu().numpy(), rf)
+
+
+# -- grouped products ------------------------------------------------------------------------------------
+def group_case(n, groups, k, out, t, seed, kind="ragged"):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "ragged":
+        w = torch.randn(groups, generator=g).mul(1.2).exp()
+        codes = torch.multinomial(w, n, replacement=True, generator=g) if n else torch.empty(0)
+        codes = codes.to(torch.int32)
+        if n > 4:
+            codes[torch.rand(n, generator=g) < 0.1] = -1
+    elif kind == "last":
+        codes = torch.full((n,), groups - 1, dtype=torch.int32)
+    else:
+        codes = torch.full((n,), -1, dtype=torch.int32)
+    x = torch.randn(n, k, generator=g).to(t)
+    dy = torch.randn(n, out, generator=g).to(t)
+    w = (torch.randn(groups, out, k, generator=g) / math.sqrt(k)).to(t)
+    return codes, x, dy, w
+
+
+def reference(codes, x, dy, w):
+    """(value, sum of the terms' magnitudes) of y, dx, dw in float64."""
+    n, k = x.shape
+    groups, out, _ = w.shape
+    r = {q: [torch.zeros(s, dtype=torch.float64) for _ in range(2)]
+         for q, s in (("y", (n, out)), ("dx", (n, k)), ("dw", (groups, out, k)))}
+    xd, dd, wd = x.double(), dy.double(), w.double()
+    for e in codes.unique().tolist():
+        if e < 0 or e >= groups:
+            continue
+        at = torch.nonzero(codes == e)[:, 0]
+        for i, f in enumerate((lambda q: q, torch.abs)):
+            r["y"][i][at] = f(xd[at]) @ f(wd[e]).t()
+            r["dx"][i][at] = f(dd[at]) @ f(wd[e])
+            r["dw"][i][e] = f(dd[at]).t() @ f(xd[at])
+    return r
+
+
+def close(got, want, mags, depth, name):
+    """Each product is exact or rounded once, each of at most depth sums once, the result once more
+    (16-bit subnormals: half of 2^-24, what float16 keeps of the smallest values)."""
+    t = got.dtype
+    tol = (depth + 2) * U * mags + half_step(t) * want.abs() + (2.0 ** -25 if t == torch.float16 else 1e-37)
+    bad = (got.double().cpu() - want).abs() > tol
+    assert not bool(bad.any()), "%s: %d of %d off, worst %g" % (
+        name, int(bad.sum()), bad.numel(), float(((got.double().cpu() - want).abs() / tol).max()))
+
+
+SHAPES = [
+    # n, groups, k, out
+    (1, 1, 1, 1), (1, 3, 8, 8), (3, 5, 7, 9), (16, 64, 256, 128), (17, 4, 64, 64), (63, 1, 128, 64),
+    (64, 1, 65, 33), (128, 2, 72, 136), (129, 2, 128, 128), (257, 9, 193, 31), (1000, 1000, 128, 64),
+    (700, 3, 40, 264), (1500, 21, 1000, 104), (2300, 2, 31, 320), (5003, 37, 193, 317), (900, 70, 264, 520),
+    (4000, 5, 128, 130), (1, 2, 2048, 24), (33, 2, 24, 2048), (40, 7, 2056, 64)]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n,groups,k,out", SHAPES)
+def test_grouped_products(n, groups, k, out, t):
+    codes, x, dy, w = group_case(n, groups, k, out, t, seed=n * 7 + k)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    xd, dd, wd = x.to(DEV), dy.to(DEV), w.to(DEV)
+    for odt in ([t] if t == torch.float32 else [t, torch.float32]):
+        y = ops.grouped_matmul(xd, wd, offsets, order, out_dtype=odt)
+        dx = ops.grouped_matmul_dx(dd, wd, offsets, order, out_dtype=odt)
+        dw = ops.grouped_matmul_dw(dd, xd, offsets, order, out_dtype=odt)
+        assert y.dtype == dx.dtype == dw.dtype == odt
+        close(y, *ref["y"], k, "y")
+        close(dx, *ref["dx"], out, "dx")
+        close(dw, *ref["dw"], n, "dw")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("kind", ["last", "none"])
+def test_grouped_products_of_one_long_group_and_of_none(kind, t):
+    n, groups, k, out = 3001, 6, 72, 40
+    codes, x, dy, w = group_case(n, groups, k, out, t, 5, kind)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    # what is left in the buffers must not shine through where a row or a group is empty
+    y = torch.full((n, out), float("nan"), dtype=t, device=DEV)
+    dx = torch.full((n, k), float("nan"), dtype=t, device=DEV)
+    dw = torch.full((groups, out, k), float("nan"), dtype=t, device=DEV)
+    ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out=y)
+    ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order, out=dx)
+    ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out=dw)
+    close(y, *ref["y"], k, "y")
+    close(dx, *ref["dx"], out, "dx")
+    close(dw, *ref["dw"], n, "dw")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_long_groups_are_cut_and_joined(t):
+    # one group of 9000 rows is cut into chunks, its neighbours are not; the bits repeat
+    g = torch.Generator().manual_seed(3)
+    codes = torch.cat([torch.zeros(9000), torch.ones(3), torch.full((700,), 3.0)]).to(torch.int32)
+    codes = codes[torch.randperm(codes.numel(), generator=g)]
+    n = codes.numel()
+    x = torch.randn(n, 48, generator=g).to(t)
+    dy = torch.randn(n, 136, generator=g).to(t)
+    w = torch.zeros(5, 136, 48).to(t)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), 5)
+    a = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+    close(a, *ref["dw"], n, "dw")
+    for _ in range(3):
+        b = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_rows_in_group_order_and_rows_that_lie_apart(t):
+    n, groups, k, out = 517, 6, 64, 72
+    g = torch.Generator().manual_seed(9)
+    codes = torch.randint(0, groups, (n,), generator=g).sort()[0].to(torch.int32)
+    wide = torch.randn(n, k + 40, generator=g).to(t)
+    wide_dy = torch.randn(n, out + 3, generator=g).to(t)
+    w = torch.randn(groups, out, k, generator=g).to(t)
+    offsets = torch.searchsorted(codes, torch.arange(groups + 1, dtype=torch.int32)).to(DEV)
+    xs, ds = wide.to(DEV), wide_dy.to(DEV)
+    for at in (0, 8, 5):
+        x, dy = xs[:, at:at + k], ds[:, 1:1 + out]
+        ref = reference(codes, x.cpu(), dy.cpu(), w)
+        host = torch.full((n, out + 20), 7.0, dtype=t, device=DEV)
+        y = ops.grouped_matmul(x, w.to(DEV), offsets, out=host[:, 4:4 + out])
+        close(y, *ref["y"], k, "y")
+        assert bool((host[:, :4] == 7).all()) and bool((host[:, 4 + out:] == 7).all())
+        close(ops.grouped_matmul_dx(dy, w.to(DEV), offsets), *ref["dx"], out, "dx")
+        close(ops.grouped_matmul_dw(dy, x, offsets), *ref["dw"], n, "dw")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_values_of_other_groups_do_not_leak(t):
+    # NaN and infinity in one group's rows and matrix, and in rows of no group, stay there
+    n, groups, k, out = 300, 4, 72, 56
+    codes, x, dy, w = group_case(n, groups, k, out, t, 11)
+    codes[:3] = torch.tensor([0, 1, 2], dtype=torch.int32)
+    poisoned = (codes == 2) | (codes < 0)
+    clean = reference(codes, x, dy, w)
+    x[poisoned] = float("nan")
+    dy[poisoned] = float("inf")
+    w[2] = float("nan")
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    y = ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order).cpu()
+    dx = ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order).cpu()
+    dw = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order).cpu()
+    keep = ~(codes == 2)
+    close(y[keep], clean["y"][0][keep], clean["y"][1][keep], k, "y")
+    close(dx[keep], clean["dx"][0][keep], clean["dx"][1][keep], out, "dx")
+    rest = [0, 1, 3]
+    close(dw[rest], clean["dw"][0][rest], clean["dw"][1][rest], n, "dw")
+    assert bool(torch.isnan(y[codes == 2]).all()) and bool(torch.isnan(dw[2]).all())
+
+
+def test_grouped_gradients_against_differences():
+    # y is linear in x and in w, so central differences are exact but for rounding
+    n, groups, k, out = 40, 3, 24, 16
+    codes, x, dy, w = group_case(n, groups, k, out, torch.float32, 21)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    xd, dd, wd = x.to(DEV), dy.to(DEV), w.to(DEV)
+    dx = ops.grouped_matmul_dx(dd, wd, offsets, order)
+    dw = ops.grouped_matmul_dw(dd, xd, offsets, order)
+    g = torch.Generator().manual_seed(1)
+
+    def loss(xx, ww):
+        return float((ops.grouped_matmul(xx, ww, offsets, order).double() * dd.double()).sum())
+
+    for _ in range(4):
+        vx, vw = torch.randn(n, k, generator=g).to(DEV), torch.randn(groups, out, k, generator=g).to(DEV)
+        # |loss| terms: n * out sums of k products, each of a few units, u each: 1e-3 is 10 times that
+        assert abs((loss(xd + vx, wd) - loss(xd - vx, wd)) / 2 - float((dx.double() * vx.double()).sum())) < 1e-3
+        assert abs((loss(xd, wd + vw) - loss(xd, wd - vw)) / 2 - float((dw.double() * vw.double()).sum())) < 1e-3
+
+
+def test_bad_orders_and_offsets_stay_inside():
+    # entries that are no rows are passed over; offsets that lie outside are used as if clamped
+    n, groups, k, out = 200, 3, 32, 48
+    codes, x, dy, w = group_case(n, groups, k, out, torch.float32, 2)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    good = ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order)
+    bad = order.clone()
+    hit = bad[5:9].long()
+    bad[5:9] = torch.tensor([-1, n, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=DEV)
+    y = torch.full((n, out), 3.0, device=DEV)
+    ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, bad, out=y)
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[hit] = False
+    assert torch.equal(y[keep], good[keep]) and bool((y[~keep] == 3).all())
+    far = offsets.clone()
+    far[-1] = 10 ** 12
+    all_rows = ops.grouped_matmul(x.to(DEV), w.to(DEV), far, order)
+    assert torch.equal(all_rows[codes.to(DEV) >= 0], good[codes.to(DEV) >= 0])
+    for off in ([0, 150, 20, 200], [-5, -9, 300, 100], [10 ** 15, 0, 0, -10 ** 15]):
+        o = torch.tensor(off, device=DEV)
+        ops.grouped_matmul(x.to(DEV), w.to(DEV), o, order)
+        ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), o, order)
+        ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), o, order)
+    torch.cuda.synchronize()
+
+
+# -- label_logprobs ---------------------------------------------------------------------------------------
+def score_reference(z, labels, temperature):
+    z = z.double() / temperature
+    lse = torch.logsumexp(z, 1)
+    lq = z - lse[:, None]
+    p = lq.exp()
+    h = -torch.where(p > 0, p * lq, torch.zeros_like(p)).sum(1)
+    empty = lse == -math.inf
+    h[empty] = 0.0
+    ok = (labels >= 0) & (labels < z.shape[1])
+    logp = torch.where(ok, lq.gather(1, labels.clamp(0, z.shape[1] - 1).long()[:, None])[:, 0],
+                       torch.zeros_like(lse))
+    logp[empty & ok] = -math.inf
+    return lse, h, logp, lq, p
+
+
+def score_tolerance(z, temperature):
+    """Absolute tolerance of lse, entropy and logp for scores of |z / T| <= a: the exponent of a term
+    carries 3 roundings of at most 130 (smaller terms vanish), a sum at most 300 roundings in a row
+    and 2 more per join, and the outer operations 4 roundings of values up to a + 20.  The entropy
+    sums terms up to 130 times smaller in their own factor: 130 times the sum's relative error is
+    avoided because e^-d d <= 1, so the same count covers it with |H| <= 20."""
+    finite = z[torch.isfinite(z)].abs().double() / temperature
+    a = float(finite.max()) if finite.numel() else 0.0
+    return U * (3 * 130 + 300 + 30 + 4 * (a + 20))
+
+
+def masked_scores(n, v, t, seed, masked, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(n, v, generator=g) * spread
+    if masked:
+        z[torch.rand(n, v, generator=g) < masked] = -math.inf
+    labels = torch.randint(-2, v + 2, (n,), generator=g)
+    return z.to(t), labels
+
+
+def check_scores(z, labels, top, temperature, zd=None, ld=None):
+    n, v = z.shape
+    zd = z.to(DEV) if zd is None else zd
+    ld = labels.to(DEV) if ld is None else ld
+    logp, ent, lse, tl, ti = ops.label_logprobs(zd, ld, top=top, temperature=temperature)
+    rl, rh, rp, lq, _ = score_reference(z, labels, temperature)
+    tol = score_tolerance(z, temperature)
+    for got, want, name in ((lse, rl, "lse"), (ent, rh, "entropy"), (logp, rp, "logp")):
+        got = got.double().cpu()
+        fine = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(got), fine), name
+        assert torch.equal(got[~fine], want[~fine]), name
+        assert float((got - want)[fine].abs().max() if fine.any() else 0) <= tol, name
+    if top:
+        # descending by score, equal scores by ascending index
+        order = torch.sort(z.double(), dim=1, descending=True, stable=True)[1][:, :top]
+        assert ti.dtype == torch.int32 and torch.equal(ti.cpu().long(), order)
+        want = lq.gather(1, order)
+        want[rl == -math.inf] = -math.inf
+        got = tl.double().cpu()
+        fine = torch.isfinite(want)
+        assert torch.equal(got[~fine], want[~fine])
+        assert float((got - want)[fine].abs().max() if fine.any() else 0) <= tol
+    else:
+        assert tl is None and ti is None
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n,v", [(1, 1), (5, 2), (3, 7), (9, 64), (4, 255), (7, 257), (33, 1000), (5, 1023),
+                                 (3, 2041), (2, 4090), (5, 4099), (3, 10007), (1, 65536), (2, 100001)])
+@pytest.mark.parametrize("top,masked,temperature", [(0, 0.0, 1.0), (1, 0.3, 0.7), (5, 0.0, 1.0), (32, 0.9, 2.0)])
+def test_label_logprobs(n, v, t, top, masked, temperature):
+    z, labels = masked_scores(n, v, t, n * 13 + v, masked)
+    check_scores(z, labels.int() if v % 2 else labels, min(top, v), temperature)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("v", [3, 300, 3001, 20000])
+def test_label_logprobs_special_rows(t, v):
+    g = torch.Generator().manual_seed(v)
+    lowest = torch.finfo(t).min
+    z = torch.randn(9, v, generator=g)
+    z[0] = -math.inf                              # nothing left
+    z[1] = -math.inf
+    z[1, v // 2] = 4.0                            # one left
+    z[2] = lowest                                 # masked with the type's lowest value
+    z[2, 1] = 3.0
+    z[3] = lowest                                 # ... everywhere
+    z[4] = 1.5                                    # all equal
+    z[5, ::2], z[5, 1::2] = 0.0, -0.0             # +0 and -0 are the same score
+    z[6] = -math.inf
+    z[6, -1] = lowest
+    z = z.to(t)
+    labels = torch.tensor([1, v // 2, 0, 2, 0, 1, v - 1, 0, -1])
+    check_scores(z, labels, min(7, v), 1.0)
+    bad = z.clone()
+    bad[7, 1] = math.inf
+    bad[8, 2] = math.nan
+    logp, ent, lse, tl, ti = ops.label_logprobs(bad.to(DEV), labels.to(DEV), top=2)
+    for q in (ent, lse, tl[:, 0], tl[:, 1]):
+        assert bool(torch.isnan(q[7:]).all()) and not bool(torch.isnan(q[:7]).any())
+    assert bool(torch.isnan(logp[7]))
+    assert int(ti[7, 0]) == 1 and int(ti[8, 0]) == 2
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_best_alternatives_that_lie_in_one_lane(t):
+    # the best scores 64 or 256 granules apart, and ties everywhere: a lane gives away many
+    vec = 4 if t == torch.float32 else 8
+    for v, apart in ((60 * 64 * vec, 64 * vec), (40 * 256 * vec, 256 * vec), (7 * 64 * vec, 64 * vec)):
+        z = torch.zeros(3, v)
+        z[0, 3::apart] = 2.0 + torch.arange(len(z[0, 3::apart])) * 0.25
+        z[1, 5::apart] = 9.0
+        z[2] = (torch.arange(v) % 3).float()
+        check_scores(z.to(t), torch.zeros(3, dtype=torch.int64), 32, 1.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("v", [37, 1000, 5001])
+def test_label_logprobs_of_rows_that_lie_apart(t, v):
+    z, labels = masked_scores(11, v + 9, t, v, 0.1)
+    zd = z.to(DEV)
+    for at in (0, 1, 3, 8):
+        check_scores(z[:, at:at + v], labels % v, 6, 1.0, zd[:, at:at + v])
+
+
+def check_grad(z, labels, d_logp, d_ent, temperature, got):
+    rl, rh, _, lq, p = score_reference(z, labels, temperature)
+    n, v = z.shape
+    ok = (labels >= 0) & (labels < v)
+    g = torch.where(ok, d_logp.double(), torch.zeros(n, dtype=torch.float64))
+    h = d_ent.double() if d_ent is not None else torch.zeros(n, dtype=torch.float64)
+    lqf = torch.where(p > 0, lq, torch.zeros_like(lq))
+    want = -p * (g[:, None] + h[:, None] * (lqf + rh[:, None]))
+    at = torch.nonzero(ok)[:, 0]
+    want[at, labels[at].long()] += g[at]
+    want[rl == -math.inf] = 0.0
+    want = want / temperature
+    # p = e^(z - lse): z - lse within score_tolerance, 3 roundings; the factor as many times |h|; a sum
+    # of g and -g p cancels to at most |g| roundings
+    eps = 2 * score_tolerance(z, temperature) + 8 * U
+    size = p * (g.abs()[:, None] + h.abs()[:, None] * (lqf.abs() + rh[:, None] + 1))
+    size[at, labels[at].long()] += g[at].abs()
+    size = torch.nan_to_num(size)
+    tol = eps * size / temperature + half_step(got.dtype) * want.abs() + \
+        (2.0 ** -25 if got.dtype == torch.float16 else 1e-37)
+    off = (got.double().cpu() - want).abs()
+    assert bool(torch.isfinite(got).all())
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n,v", [(1, 1), (300, 2), (7, 33), (64, 1000), (3, 4099), (2, 70001)])
+@pytest.mark.parametrize("temperature,masked", [(1.0, 0.0), (0.5, 0.3)])
+def test_label_logprobs_grad(n, v, t, temperature, masked):
+    z, labels = masked_scores(n, v, t, n + v, masked)
+    if n > 2:
+        z[1] = -math.inf
+    g = torch.Generator().manual_seed(4)
+    d_logp, d_ent = torch.randn(n, generator=g), torch.randn(n, generator=g)
+    zd, ld = z.to(DEV), labels.to(DEV)
+    _, ent, lse, _, _ = ops.label_logprobs(zd, ld, temperature=temperature)
+    got = ops.label_logprobs_grad(zd, ld, lse, ent, d_logp.to(DEV), d_ent.to(DEV), temperature)
+    check_grad(z, labels, d_logp, d_ent, temperature, got)
+    got = ops.label_logprobs_grad(zd, ld.int(), lse, ent, d_logp.to(DEV), None, temperature)
+    check_grad(z, labels, d_logp, None, temperature, got)
+    # in place, and rows that lie apart: the same bits
+    wide = torch.zeros(n, v + 5, dtype=t, device=DEV)
+    ops.label_logprobs_grad(zd, ld, lse, ent, d_logp.to(DEV), None, temperature, out=wide[:, 3:3 + v])
+    assert torch.equal(wide[:, 3:3 + v], got) and bool((wide[:, :3] == 0).all()) and bool((wide[:, 3 + v:] == 0).all())
+    ops.label_logprobs_grad(zd, ld, lse, ent, d_logp.to(DEV), None, temperature, out=zd)
+    assert torch.equal(zd, got)
+
+
+def test_label_logprobs_gradient_against_differences():
+    g = torch.Generator().manual_seed(8)
+    n, v = 6, 50
+    z = torch.randn(n, v, generator=g)
+    labels = torch.randint(0, v, (n,), generator=g).to(DEV)
+    a, b = torch.randn(n, generator=g), torch.randn(n, generator=g)
+    zd = z.to(DEV)
+    _, ent, lse, _, _ = ops.label_logprobs(zd, labels)
+    grad = ops.label_logprobs_grad(zd, labels, lse, ent, a.to(DEV), b.to(DEV)).double().cpu()
+
+    def loss(q):
+        logp, e, _, _, _ = ops.label_logprobs(q.to(DEV), labels)
+        return float((logp.double().cpu() * a.double() + e.double().cpu() * b.double()).sum())
+
+    step = 2.0 ** -6
+    for _ in range(5):
+        d = torch.randn(n, v, generator=g).mul(16).round() / 16
+        fd = (loss(z + step * d) - loss(z - step * d)) / (2 * step)
+        # third differences: step^2 / 6 * |d|^3 * 50 terms; rounding: 12 values of 5 u each / step
+        assert abs(fd - float((grad * d.double()).sum())) < 2e-3
+
+
+# -- adamw -------------------------------------------------------------------------------------------------
+HYPER = dict(lr=3e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+
+
+def adam_values(m_codes, v_codes, scales):
+    """The values of 8-bit states, float64 numpy, from the format's definition."""
+    c = m_codes.cpu().numpy().astype(np.int64)
+    d = v_codes.cpu().numpy().astype(np.int64)
+    s = scales.double().cpu().numpy().repeat(256, axis=1)
+
+    def value(code, mant):
+        e, f = code >> mant, code & ((1 << mant) - 1)
+        return np.where(e > 0, (f + (1 << mant)) * 2.0 ** (e - 1), f * 1.0)
+
+    m = np.where(c & 128, -1.0, 1.0) * value(c & 127, 3) / 512 * s[0]
+    r = value(d, 4) * s[1]
+    m[(c & 127) == 127] = np.nan
+    r[d == 255] = np.nan
+    return m, r * r
+
+
+def adam_reference(p, g, m, v, step, lr, betas, eps, weight_decay, grad_scale=1.0):
+    """float64 numpy; g is scaled in float32 as the step does."""
+    b1, b2 = betas
+    g = (g.astype(np.float32) * np.float32(grad_scale)).astype(np.float64)
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    upd = lr * (m / (1 - b1 ** step)) / (np.sqrt(v / (1 - b2 ** step)) + eps)
+    return p * (1 - lr * weight_decay) - upd, m, v, np.abs(upd)
+
+
+SIZES = [1, 255, 256, 257, 4099, 2048, 7, 0, 100_003]
+
+
+def adam_tensors(p_t, g_t, seed, align=1):
+    g = torch.Generator().manual_seed(seed)
+    ps, gs = [], []
+    for i, n in enumerate(SIZES):
+        # views at odd places of larger buffers too
+        pad = i % 3 if align == 1 else 0
+        p = torch.empty(n + pad, dtype=p_t, device=DEV)[pad:]
+        q = torch.empty(n + pad, dtype=g_t, device=DEV)[pad:]
+        p.copy_(torch.randn(n, generator=g))
+        q.copy_(torch.randn(n, generator=g) * 10.0 ** (i % 5 - 3))
+        ps.append(p)
+        gs.append(q)
+    return ps, gs
+
+
+def flat_f64(ts):
+    parts = []
+    for t in ts:
+        a = t.double().cpu().numpy().reshape(-1)
+        parts.append(np.pad(a, (0, -a.size % 256)))
+    return np.concatenate(parts)
+
+
+@pytest.mark.parametrize("p_t", TYPES, ids=str)
+@pytest.mark.parametrize("g_t", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps(p_t, g_t, bits):
+    ps, gs = adam_tensors(p_t, g_t, 17)
+    m, v, scales = ops.adamw_states(ps, bits)
+    rng = np.random.default_rng(3)
+    inside = np.concatenate([np.pad(np.ones(n, bool), (0, -n % 256)) for n in SIZES])
+    for step in (1, 2, 3, 40):
+        for q in gs:
+            q.mul_(float(rng.uniform(-1.5, 1.5)))
+        before = flat_f64(ps), flat_f64(gs)
+        if bits == 32:
+            m0, v0 = m.double().cpu().numpy(), v.double().cpu().numpy()
+        else:
+            m0, v0 = adam_values(m, v, scales)
+        scale = 1.0 if step < 3 else 0.37
+        ops.adamw_step(ps, gs, m, v, step=step, scales=scales, grad_scale=scale, **HYPER)
+        rp, rm, rv, upd = adam_reference(before[0], before[1], m0, v0, step, grad_scale=scale, **HYPER)
+        got = flat_f64(ps)
+        # the decay and the difference round twice, the step's factors about ten times
+        tol = 2 * U * (np.abs(before[0]) + upd) + 12 * U * upd + half_step(p_t) * np.abs(rp) + \
+            (2.0 ** -25 if p_t == torch.float16 else 1e-37)
+        # v = 0 with m = 0: the step is 0 / eps
+        assert (np.abs(got - rp)[inside] <= tol[inside]).all(), step
+        assert (got[~inside] == 0).all()
+        if bits == 32:
+            m1, v1 = m.double().cpu().numpy(), v.double().cpu().numpy()
+            b1, b2 = HYPER["betas"]
+            gq = np.abs(before[1] * scale)
+            assert (np.abs(m1 - rm) <= 4 * U * (np.abs(m0) + gq) + 1e-44)[inside].all()
+            assert (np.abs(v1 - rv) <= 6 * U * rv + 1e-44)[inside].all()
+            assert (m1[~inside] == 0).all() and (v1[~inside] == 0).all()
+        else:
+            check_codes(m, v, scales, rm * inside, np.sqrt(rv) * inside)
+            mv, vv = ops.adamw_state_values(m, v, scales)
+            wm, wv = adam_values(m, v, scales)
+            assert (np.abs(mv.double().cpu().numpy() - wm) <= U * np.abs(wm) + 1e-45).all()
+            assert (np.abs(vv.double().cpu().numpy() - wv) <= 3 * U * wv + 1e-45).all()
+
+
+def check_codes(m, v, scales, rm, rr):
+    """Scales are the rounded maxima, codes the nearest ones (unless float64 itself cannot tell)."""
+    rm, rr = rm.reshape(-1, 256), rr.reshape(-1, 256)
+    s = scales.double().cpu().numpy()
+    for want, got in ((np.abs(rm).max(1) / 448, s[0]), (rr.max(1) / 491520, s[1])):
+        assert (np.abs(want - got) <= U * want * (1 + 1e-9) + 2.0 ** -150).all()
+    mags = np.arange(127)
+    tab_m = np.where(mags >= 8, ((mags & 7) + 8) * 2.0 ** ((mags >> 3) - 1.0), mags) / 512
+    full = np.arange(255)
+    tab_v = np.where(full >= 16, ((full & 15) + 16) * 2.0 ** ((full >> 4) - 1.0), full)
+    for value, scale, table, codes in ((np.abs(rm), s[0], tab_m, m.cpu().numpy() & 127),
+                                       (rr, s[1], tab_v, v.cpu().numpy())):
+        q = np.divide(value, scale[:, None], out=np.zeros_like(value), where=scale[:, None] > 0)
+        mids = (table[1:] + table[:-1]) / 2
+        c = np.searchsorted(mids, q, side="left")
+        tie = (c < mids.size) & (mids[np.minimum(c, mids.size - 1)] == q)
+        c = np.where(tie & (c % 2 == 1), c + 1, c)
+        if table is tab_v:
+            c = np.where((q > 0) & (c == 0), 1, c)
+        near = np.abs(q - mids[np.clip(np.searchsorted(mids, q), 0, mids.size - 1)]) <= 1e-12 * q
+        got = codes.reshape(-1, 256)
+        assert ((c == got) | near).all(), int(((c != got) & ~near).sum())
+    sign = (m.cpu().numpy().reshape(-1, 256) & 128) != 0
+    assert (sign == (rm < 0)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_tensors_and_device_scalars(bits):
+    # more tensors than one launch's table holds; lr and step read from the device
+    g = torch.Generator().manual_seed(1)
+    sizes = [int(q) for q in torch.randint(1, 700, (200,), generator=g)]
+    ps = [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    gs = [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    ps2 = [p.clone() for p in ps]
+    a = ops.adamw_states(ps, bits)
+    b = ops.adamw_states(ps, bits)
+    for step in (1, 2):
+        ops.adamw_step(ps, gs, a[0], a[1], lr=0.01, step=step, scales=a[2])
+        ops.adamw_step(ps2, gs, b[0], b[1], lr=torch.tensor([0.01], device=DEV),
+                       step=torch.tensor([step], device=DEV), scales=b[2])
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for p, q, n in zip(ps, ps2, sizes):
+        # the device's lr is the float32 nearest to 0.01
+        assert float((p - q).abs().max()) <= 4 * U * float(p.abs().max() + 0.02)
+    rp, rm, rv = flat_f64([t.cpu() for t in ps2]) * 0, 0, 0
+    assert rp.size == a[0].numel()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_a_gradient_that_is_not_finite_stays_where_it_is(bits):
+    p = torch.randn(600, device=DEV)
+    g = torch.randn(600, device=DEV)
+    g[3], g[300], g[301] = math.nan, math.inf, -math.inf
+    m, v, s = ops.adamw_states([p], bits)
+    ops.adamw_step([p], [g], m, v, lr=1e-3, step=1, scales=s)
+    mv, vv = ops.adamw_state_values(m, v, s)
+    hit = torch.zeros(600, dtype=torch.bool)
+    hit[[3, 300, 301]] = True
+    for q in (p, mv[:600], vv[:600]):
+        assert torch.equal(~torch.isfinite(q.cpu()), hit)
+    if bits == 8:
+        assert bool(torch.isnan(mv[:600].cpu()[hit]).all())
+
+
+def test_adamw_zero_and_tiny_gradients_in_8_bits():
+    # nothing seen: nothing moves; 12 decades in one block: v stays above zero where g was not zero
+    p = torch.ones(512, device=DEV)
+    g = torch.zeros(512, device=DEV)
+    m, v, s = ops.adamw_states([p], 8)
+    ops.adamw_step([p], [g], m, v, lr=1e-3, step=1, weight_decay=0.0, scales=s)
+    assert bool((p == 1).all()) and int(m.sum()) == 0 and int(v.sum()) == 0
+    g[:256] = 10.0 ** torch.linspace(-12, 0, 256, device=DEV)
+    ops.adamw_step([p], [g], m, v, lr=1e-3, step=2, weight_decay=0.0, scales=s)
+    assert bool((v[:256] > 0).all()) and int(v[256:].sum()) == 0
+    assert bool(torch.isfinite(p).all()) and bool((p[256:] == 1).all())
+
+
+# -- together, on other streams, captured ---------------------------------------------------------------
+def _train_pass(x, codes, w, labels, step, state, groups):
+    order, offsets = ops.group_rows(codes, groups)
+    z = ops.grouped_matmul(x, w, offsets, order)
+    logp, ent, lse, _, _ = ops.label_logprobs(z, labels)
+    d = torch.full_like(logp, -1.0 / x.shape[0])
+    dz = ops.label_logprobs_grad(z, labels, lse, ent, d, out=z)
+    dw = ops.grouped_matmul_dw(dz, x, offsets, order)
+    dx = ops.grouped_matmul_dx(dz, w, offsets, order)
+    ops.adamw_step([w], [dw], state[0], state[1], lr=1e-2, step=step, weight_decay=0.0, scales=state[2])
+    return logp, dx
+
+
+def _train_inputs(seed, n=3000, groups=7, k=64, classes=40):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, k, generator=g).to(DEV),
+            torch.randint(-1, groups, (n,), generator=g, dtype=torch.int32).to(DEV),
+            (torch.randn(groups, classes, k, generator=g) * 0.1).to(DEV),
+            torch.randint(-1, classes, (n,), generator=g).to(DEV))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_training_pass_matches_its_formulas(bits):
+    x, codes, w, labels = _train_inputs(1)
+    w0 = w.double().cpu()
+    state = ops.adamw_states([w], bits)
+    logp, dx = _train_pass(x, codes, w, labels, 1, state, 7)
+    xd, c, y = x.double().cpu(), codes.cpu().long(), labels.cpu()
+    leaf, xl = w0.clone().requires_grad_(), xd.clone().requires_grad_()
+    member = c >= 0
+    z = torch.zeros(x.shape[0], 40, dtype=torch.float64)
+    z = torch.where(member[:, None], torch.einsum("nck,nk->nc", leaf[c.clamp(min=0)], xl), z)
+    lq = torch.log_softmax(z, 1)
+    has = y >= 0
+    picked = torch.where(has, lq.gather(1, y.clamp(min=0)[:, None])[:, 0], torch.zeros(1, dtype=torch.float64))
+    (-picked.mean()).backward()
+    # 64-term products, one log-softmax over 40: all well below 1e-5 of values up to 10
+    assert float((logp.double().cpu() - picked.detach()).abs().max()) < 1e-5
+    assert float((dx.double().cpu() - xl.grad).abs().max()) < 1e-6 / x.shape[0] ** 0.5
+    rp, _, _, upd = adam_reference(w0.numpy(), leaf.grad.numpy().astype(np.float32).astype(np.float64), 0.0, 0.0, 1,
+                                   1e-2, (0.9, 0.999), 1e-8, 0.0)
+    # the first step is lr * g / (|g| + eps): a gradient entry of size s off by 1e-9 moves it by lr * 1e-9 *
+    # eps / s^2, so entries above 1e-6 are compared
+    big = np.abs(leaf.grad.numpy()) > 1e-6
+    assert np.abs(w.double().cpu().numpy() - rp)[big].max() < 1e-5
+    assert big.mean() > 0.9
+
+
+def test_a_captured_training_pass_is_replayed():
+    x, codes, w, labels = _train_inputs(2)
+    step = torch.ones(1, dtype=torch.int64, device=DEV)
+    state = ops.adamw_states([w], 8)
+    w1, state1 = w.clone(), ops.adamw_states([w], 8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _train_pass(x, codes, w.clone(), labels, 1, ops.adamw_states([w], 8), 7)   # warm
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logp, dx = _train_pass(x, codes, w, labels, step, state, 7)
+    for i in range(4):
+        # other inputs, through the captured addresses; eager work in between
+        nx, nc, _, nl = _train_inputs(10 + i)
+        x.copy_(nx)
+        codes.copy_(nc)
+        labels.copy_(nl)
+        step.fill_(i + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        elogp, edx = _train_pass(nx, nc, w1, nl, i + 1, state1, 7)
+        torch.cuda.synchronize()
+        assert torch.equal(logp, elogp) and torch.equal(dx, edx)
+        assert torch.equal(w, w1) and torch.equal(state[0], state1[0]) and torch.equal(state[1], state1[1])
+
+
+def test_two_streams_at_once():
+    cases = [_train_inputs(30 + i, n=20_000, groups=30) for i in range(2)]
+    want = []
+    for x, codes, w, labels in cases:
+        s = ops.adamw_states([w], 32)
+        q = w.clone()
+        want.append(_train_pass(x, codes, q, labels, 1, s, 30) + (q,))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for (x, codes, w, labels), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                q = w.clone()
+                got.append(_train_pass(x, codes, q, labels, 1, ops.adamw_states([w], 32), 30) + (q,))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, r) for p, r in zip(a, b))

@@ -1,0 +1,116 @@
+"""What the grouped products, label log probabilities and the AdamW step refuse, on any machine."""
+import ctypes
+
+import pytest
+import torch
+
+from image_classification_amd import _lib, ops
+
+
+def z(*shape, **kw):
+    return torch.zeros(*shape, **kw)
+
+
+I32 = dict(dtype=torch.int32)
+I64 = dict(dtype=torch.int64)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.group_rows(z(4, **I64), 3),
+    lambda: ops.group_rows(z(4, 2, **I32), 3),
+    lambda: ops.group_rows(z(4, **I32), 0),
+    lambda: ops.group_rows(z(4, **I32), (1 << 26) + 1),
+    lambda: ops.group_rows(z(4, **I32), 3),                                    # not on a GPU
+    lambda: ops.grouped_matmul(z(4, 8), z(2, 3, 9), z(3, **I64)),              # widths
+    lambda: ops.grouped_matmul(z(4, 8), z(3, 8), z(3, **I64)),                 # w not 3-D
+    lambda: ops.grouped_matmul(z(4, 8), z(2, 8, 3).transpose(1, 2), z(3, **I64)),
+    lambda: ops.grouped_matmul(z(4, 8), z(0, 3, 8), z(1, **I64)),
+    lambda: ops.grouped_matmul(z(4), z(2, 3, 8), z(3, **I64)),
+    lambda: ops.grouped_matmul(z(8, 4).t(), z(2, 3, 8), z(3, **I64)),          # columns adjacent, not rows
+    lambda: ops.grouped_matmul(z(1, 8).expand(4, 8), z(2, 3, 8), z(3, **I64)),  # rows overlap
+    lambda: ops.grouped_matmul(z(4, 8), z(2, 3, 8, dtype=torch.float16), z(3, **I64)),
+    lambda: ops.grouped_matmul(z(4, 8, dtype=torch.float64), z(2, 3, 8, dtype=torch.float64), z(3, **I64)),
+    lambda: ops.grouped_matmul(z(4, 8), z(2, 3, 8), z(3, **I64)),              # not on a GPU
+    lambda: ops.grouped_matmul_dx(z(4, 8), z(2, 3, 8), z(3, **I64)),           # dy has `out` columns
+    lambda: ops.grouped_matmul_dw(z(4, 3), z(5, 8), z(3, **I64)),
+    lambda: ops.grouped_matmul_dw(z(4, 3), z(4, 8, dtype=torch.float16), z(3, **I64)),
+    lambda: ops.grouped_matmul_dw(z(4, 0), z(4, 8), z(3, **I64)),
+    lambda: ops.label_logprobs(z(4)),
+    lambda: ops.label_logprobs(z(4, 0)),
+    lambda: ops.label_logprobs(z(4, 5, dtype=torch.float64)),
+    lambda: ops.label_logprobs(z(4, 5), top=6),
+    lambda: ops.label_logprobs(z(4, 50), top=33),
+    lambda: ops.label_logprobs(z(4, 5), top=-1),
+    lambda: ops.label_logprobs(z(4, 5), temperature=0.0),
+    lambda: ops.label_logprobs(z(4, 5), temperature=float("inf")),
+    lambda: ops.label_logprobs(z(4, 5), temperature=float("nan")),
+    lambda: ops.label_logprobs(z(4, 5)),                                       # not on a GPU
+    lambda: ops.label_logprobs_grad(z(4, 5), None, z(4), z(4), z(4)),
+    lambda: ops.label_logprobs_grad(z(4, 5), z(4, **I64), None, z(4), z(4)),
+    lambda: ops.adamw_states([z(3)], 16),
+    lambda: ops.adamw_step([z(3)], [], z(256), z(256), lr=1e-3, step=1),
+    lambda: ops.adamw_step([z(3)], [z(3)], z(256), z(256), lr=1e-3, step=1, scales=z(2, 1)),
+    lambda: ops.adamw_step([z(3)], [z(3)], z(256, dtype=torch.float16), z(256), lr=1e-3, step=1),
+    lambda: ops.adamw_step([z(3)], [z(3)], z(256), z(256), lr=1e-3, step=1),   # not on a GPU
+    lambda: ops.adamw_state_values(z(300, dtype=torch.uint8), z(300, dtype=torch.uint8), z(2, 1)),
+    lambda: ops.adamw_state_values(z(256, dtype=torch.uint8), z(256, dtype=torch.uint8), z(1, 1)),
+    lambda: ops.adamw_state_values(z(256, dtype=torch.uint8), z(256, dtype=torch.uint8), z(2, 1)),
+])
+def test_refused_before_anything_is_launched(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_a_handle_is_asked_for():
+    lib = _lib.load()
+    for name, args in (("ic_group_rows", 9), ("ic_grouped_matmul", 15), ("ic_grouped_matmul_dx", 15),
+                       ("ic_grouped_matmul_dw", 17), ("ic_label_logprobs", 18),
+                       ("ic_label_logprobs_grad", 16), ("ic_adamw_step", 18), ("ic_adamw_state_values", 8)):
+        fn = getattr(lib, name)
+        assert len(fn.argtypes) == args
+        zeros = [None if t is ctypes.c_void_p else 0 for t in fn.argtypes]
+        assert fn(*zeros) == 10003, name
+        assert "invalid handle" in _lib.last_error()
+
+
+def test_scratch_sizes():
+    lib = _lib.load()
+    assert lib.ic_group_rows_scratch(4096, 1000) == 0
+    assert lib.ic_group_rows_scratch(1_000_000, 10_000) >= 12_000_000   # pairs and sorted codes
+    assert lib.ic_grouped_matmul_dw_scratch(500, 128, 64) == 0
+    # chunks of at least 512 rows, at most two partial results a chunk, 256 MB in all
+    for n, k, out in ((1_000_000, 128, 64), (65536, 2048, 2048), (3_000_000, 2048, 16), (4097, 8, 8)):
+        assert 0 <= lib.ic_grouped_matmul_dw_scratch(n, k, out) <= max(1 << 28, 2 * (n // 512) * k * out * 4)
+    assert lib.ic_label_logprobs_scratch(100_000, 1000, 1, 5) == 0
+    assert lib.ic_label_logprobs_scratch(4, 65536, 0, 5) > 0
+    assert lib.ic_label_logprobs_scratch(4, 65536, 9, 5) == 0
+
+
+# -- host arithmetic of the tile numbering (what find_group and the grids rely on) ---------------------------
+def test_every_tile_of_ragged_groups_has_a_number():
+    import numpy as np
+    rng = np.random.default_rng(0)
+    for trial in range(300):
+        groups = int(rng.integers(1, 12))
+        bm = int(rng.choice([16, 64, 128, 512]))
+        sizes = rng.choice([0, 0, 1, bm - 1, bm, bm + 1, 3 * bm, int(rng.integers(0, 5 * bm))], groups)
+        off = np.concatenate([[0], np.cumsum(sizes)])
+        n = int(off[-1] + rng.integers(0, 3 * bm))
+        first = np.array([off[e] // bm + e for e in range(groups + 1)])
+        total = n // bm + groups + 1
+        assert (np.diff(first) >= 1).all()
+        ends = np.append(off[1:], n)
+        for e in range(groups + 1):
+            tiles = -(-(ends[e] - off[e]) // bm)
+            nxt = first[e + 1] if e < groups else total
+            assert first[e] + tiles <= nxt
+        # partial results of groups of more than one chunk
+        used = set()
+        for e in range(groups):
+            rows = off[e + 1] - off[e]
+            if rows > bm:
+                slots = range(2 * (off[e] // bm), 2 * (off[e] // bm) + -(-rows // bm))
+                assert not used & set(slots) and max(slots) < 2 * (n // bm)
+                used |= set(slots)
+                j = -(-off[e] // bm)
+                assert off[e] <= j * bm < off[e] + bm and j * bm < off[e + 1] and j <= (n - 1) // bm
