@@ -74,7 +74,7 @@ _SIGNATURES = {
                           _c_int, _c_int, _p],
     "ic_grouped_matmul_dx": [_p, _p, _c_i64, _p, _p, _c_i64, _p, _p, _c_i64, _c_i64, _c_int, _c_int,
                              _c_int, _c_int, _p],
-    "ic_grouped_matmul_dw_scratch": [_c_i64, _c_int, _c_int],
+    "ic_grouped_matmul_dw_scratch": [_c_i64, _c_i64, _c_int, _c_int, _c_int],
     "ic_grouped_matmul_dw": [_p, _p, _c_i64, _p, _c_i64, _p, _p, _p, _c_i64, _c_i64, _c_int, _c_int,
                              _c_int, _c_int, _p, _c_i64, _p],
     "ic_label_logprobs_scratch": [_c_i64, _c_i64, _c_int, _c_int],

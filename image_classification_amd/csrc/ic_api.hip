@@ -984,9 +984,9 @@ int ic_grouped_matmul_dx(void* handle, const void* dy, int64_t ld_dy, const void
                            n, n_groups, k, out, dtype, y_dtype, stream);
 }
 
-int64_t ic_grouped_matmul_dw_scratch(int64_t n, int k, int out) {
-  if (n < 0 || k < 1 || out < 1) return 0;
-  return (int64_t)ic::grouped_dw_scratch(n, out, k);
+int64_t ic_grouped_matmul_dw_scratch(int64_t n, int64_t n_groups, int k, int out, int dtype) {
+  if (n < 0 || n_groups < 1 || k < 1 || out < 1 || bad_type(dtype)) return 0;
+  return (int64_t)ic::grouped_dw_scratch(n, n_groups, k, out, dtype);
 }
 
 int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
@@ -1003,7 +1003,7 @@ int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void
   if ((rc = misaligned(who, x, dtype)) || (rc = misaligned(who, dy, dtype)) ||
       (rc = misaligned(who, dw, y_dtype)))
     return rc;
-  rc = check_scratch(who, scratch, scratch_bytes, ic::grouped_dw_scratch(n, out, k));
+  rc = check_scratch(who, scratch, scratch_bytes, ic::grouped_dw_scratch(n, n_groups, k, out, dtype));
   if (rc) return rc;
   DeviceGuard guard(ctx->device);
   if (!guard.ok) return fail_hip(guard.err, "hipSetDevice");

@@ -25,6 +25,8 @@
 // the lane, so the layouts are not padded: 16-byte granules are exchanged inside a row by an
 // exclusive-or with bits of the row number, chosen so that the lanes of one LDS access fall into
 // different banks.  Granules outside the operands are fetched from a granule of zeros.
+#include <type_traits>
+
 #include "ic_wave.h"
 
 namespace ic {
@@ -284,6 +286,13 @@ struct Groups {
   }
 };
 
+// A value that is the same in every lane, kept in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const unsigned low = __builtin_amdgcn_readfirstlane((unsigned)v);
+  const unsigned high = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)v >> 32));
+  return (int64_t)(((uint64_t)high << 32) | low);
+}
+
 // The last e in [0, groups] whose first tile, at(e) / bm + e, is <= tile.  Every lane of the wave
 // takes part and gets the answer.
 __device__ __forceinline__ int64_t find_group(const Groups& g, int64_t tile, int64_t bm, int lane) {
@@ -297,9 +306,7 @@ __device__ __forceinline__ int64_t find_group(const Groups& g, int64_t tile, int
     lo += c * step;
     hi = lo + step < hi ? lo + step : hi;
   }
-  const unsigned low = __builtin_amdgcn_readfirstlane((unsigned)lo);
-  const unsigned high = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)lo >> 32));
-  return (int64_t)(((uint64_t)high << 32) | low);
+  return uniform(lo);
 }
 
 // Workgroup numbers are dealt to the 8 XCDs in turn; this gives each XCD a run of neighbours, whose
@@ -313,10 +320,25 @@ __device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total) {
 // ---- tiles in LDS ----------------------------------------------------------------------------------
 constexpr int kStageBytes = 128;   // of the contraction
 
+// 16 bytes a lane from memory to LDS at a wave-uniform address + 16 * lane.  Written as an instruction
+// of its own, without results: the compiler, which cannot tell the stage being filled from the one
+// being read by the transposing loads, would wait for it in front of every one of those.  The kernels
+// wait themselves (all_landed) before the barrier that hands a stage over.
 __device__ __forceinline__ void lds_load16(const void* src, char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+  const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds_wave_base;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(to))
+               : "memory", "m0");
 }
+__device__ __forceinline__ void lds_load4(const void* src, char* lds_wave_base) {
+  const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds_wave_base;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+               :
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(to))
+               : "memory", "m0");
+}
+__device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <typename T> struct Mma;
 template <> struct Mma<float> {
@@ -348,28 +370,64 @@ template <> struct Mma<f16_t> {
   }
 };
 
-// Tile "along": [rows][128 bytes], granule s of row r holds granule s ^ (r & 7) of the stage.
-__device__ __forceinline__ u32x4 read_along(const char* tile, int r0, int step, int lane) {
+// Which columns the lanes of a fragment stand for.  A product of fragment j of the Q side leaves a lane
+// with results 4 (lane >> 4) .. + 3 of its 16; taking column
+//     spread(i, j) = 16 (i >> 2) + 4 j + (i & 3)
+// as result i of fragment j (j = 0 .. 3) makes that 16 neighbouring columns a lane over the four
+// fragments, and 64 neighbouring columns a row: whole cache lines are stored.
+//
+// Tile "along": [rows][128 bytes], granule s of row r holds granule s ^ swap(r) of the stage.  P is
+// read 16 neighbouring rows at a time, Q in the rows spread(0 .. 15, j); 8 lanes of a read reach 8
+// different places of the 256 bytes of the banks in either.
+__device__ __forceinline__ int along_swap_p(int r) { return r & 7; }
+__device__ __forceinline__ int along_swap_q(int r) { return ((r >> 3) & 6) | ((r >> 1) & 1); }
+// A lane's place of fragment 0, step 0 (bytes behind the operand's tile).  Fragment i of P lies 16
+// rows further, fragment j of Q 4 rows; step 1 exchanges the halves of a row (the swaps and the quarter
+// wave's granule share no bit with it).
+__device__ __forceinline__ int along_place_p(int r0, int lane) {
   const int r = r0 + (lane & 15);
-  const int s = (step * 4 + (lane >> 4)) ^ (r & 7);
-  return *reinterpret_cast<const u32x4*>(tile + r * kStageBytes + s * 16);
+  return r * kStageBytes + ((lane >> 4) ^ along_swap_p(r)) * 16;
+}
+__device__ __forceinline__ int along_place_q(int r0, int lane) {
+  const int r = r0 + ((lane & 12) << 2) + (lane & 3);
+  return r * kStageBytes + ((lane >> 4) ^ along_swap_q(r)) * 16;
 }
 
-// Tile "across": [kK rows of the contraction][COLS], granules exchanged by the contraction row.
-template <typename T>
-__device__ __forceinline__ int across_swap(int k) {
-  return sizeof(T) == 2 ? (k & 3) << 1 : ((k >> 2) & 3) << 2;
+// Tile "across": [kK rows of the contraction][COLS], granules exchanged by the contraction row k.  In
+// the transposing load of 16-bit types the 16 lanes of a quarter wave point at 4 rows of the
+// contraction and 4 x 4 columns; lane i is handed column i of the 16, 4 elements of the contraction.
+// float32 needs no transposing: 4-byte loads of rows k, k + 1, ... a lane.
+template <typename T, int COLS>
+__device__ __forceinline__ int across_swap_p(int k) {
+  if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+  return COLS >= 128 ? ((k & 3) | ((k >> 1) & 4)) << 1 : (k & 3) << 1;
 }
 template <typename T, int COLS>
-__device__ __forceinline__ u32x4 read_across(const char* tile, int c0, int step, int lane) {
+__device__ __forceinline__ int across_swap_q(int k) {
+  if (sizeof(T) == 4) return (k >> 2) & 3;
+  return COLS >= 128 ? (k & 1) | ((k & 2) << 2) : k & 1;
+}
+// A lane's place of fragment 0, step 0: the column whose 8 bytes (16-bit types) or 4 bytes (float32) it
+// points at, in its row of the contraction.  The fragments' columns and the swaps only set bits that
+// are clear in the wave's first column, so fragment i of P lies at place ^ 16 i columns and fragment j
+// of Q at place ^ 4 j columns; a step is kK / 2 rows.
+template <typename T, int COLS, bool Q>
+__device__ __forceinline__ int across_place(int c0, int lane) {
+  constexpr int kRow = COLS * (int)sizeof(T), kV = 16 / (int)sizeof(T);
+  const int k = sizeof(T) == 2 ? (lane >> 4) * 8 + ((lane & 15) >> 2) : (lane >> 4) * 4;
+  int c;
+  if (sizeof(T) == 2) c = (lane & 3) * (Q ? 16 : 4);
+  else c = Q ? ((lane & 12) << 2) + (lane & 3) : lane & 15;
+  c += c0;
+  const int swap = Q ? across_swap_q<T, COLS>(k) : across_swap_p<T, COLS>(k);
+  return k * kRow + ((c / kV) ^ swap) * 16 + c % kV * (int)sizeof(T);
+}
+// (rows k .. k + 3 of float32 and k, k + 4 of the 16-bit types have the same swap)
+template <typename T, int COLS>
+__device__ __forceinline__ u32x4 read_across(const char* p) {
   constexpr int kRow = COLS * (int)sizeof(T);
   u32x4 out;
   if constexpr (sizeof(T) == 2) {
-    // the 16 lanes of a quarter wave point at 4 rows of the contraction x 16 columns, 4 columns
-    // each; lane i is handed column i of the 4 rows
-    const int t = lane & 15;
-    const int s = ((c0 >> 3) + ((t & 3) >> 1)) ^ across_swap<T>(t >> 2);
-    const char* p = tile + (step * 32 + (lane >> 4) * 8 + (t >> 2)) * kRow + s * 16 + (t & 1) * 8;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)(p));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -380,13 +438,30 @@ __device__ __forceinline__ u32x4 read_across(const char* tile, int c0, int step,
     out[2] = b[0];
     out[3] = b[1];
   } else {
-    const int t = lane & 15;
-    const int s = ((c0 >> 2) + (t >> 2)) ^ across_swap<T>((lane >> 4) * 4);
-    const char* p = tile + (step * 16 + (lane >> 4) * 4) * kRow + s * 16 + (t & 3) * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = *reinterpret_cast<const unsigned*>(p + j * kRow);
   }
   return out;
+}
+
+// Reads the fragments of one operand for one step: COUNT of them from fragment `first` on.
+template <typename T, int COLS, bool ALONG, bool Q, int COUNT>
+__device__ __forceinline__ void read_fragments(const char* tile, int place, int step, int first, u32x4* out) {
+  // (opaque: the fragments' addresses are worked out here, one instruction each, and not kept in
+  // registers of their own through the loop)
+  asm volatile("" : "+v"(place));
+  if (ALONG) {
+    const char* p = tile + (place ^ (step * 64));
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      out[i] = *reinterpret_cast<const u32x4*>(p + (first + i) * (Q ? 4 : 16) * kStageBytes);
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      out[i] = read_across<T, COLS>(tile + step * (Mma<T>::kK / 2 * COLS * (int)sizeof(T)) +
+                                    (place ^ ((first + i) * (Q ? 4 : 16) * (int)sizeof(T))));
+  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // One granule of an operand: elements [c, c + kVec) of a row of `cols` elements (NULL row: zeros).
@@ -415,6 +490,71 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
   }
 }
 
+// The stages of a tile.  Each is multiplied in two steps, and a step in kHalves parts of the wave's
+// rows (two where there are enough of them: the operands of half a step then fit the registers twice).
+// A part's operands are read from LDS while the part before is multiplied, and the barrier that
+// frees a stage's buffer stands in front of its last part, so that the matrix unit has work on both
+// sides of it:
+//     ... | read the last part | multiply the one before | stage st + 1 has landed, barrier |
+//     read the first part of st + 1 | multiply the last part of st
+// The freed buffer is refilled with stage st + 2 one load per four products, during the last part of
+// st and the first of st + 1: issued in one go behind the barrier, the 8 waves' loads would hold up
+// the products behind them in every wave.
+// LOAD(i, stage, buffer) issues load i of kLoads; with PREPARES, NEXT(stage) fetches what the loads of
+// that stage need, and lands a barrier before them.
+#define MULTIPLY_STAGES(STAGES, LOAD, NEXT, PREPARES)                                          \
+  {                                                                                  \
+    constexpr int kStage = kPBytes + kQBytes, kFirst = kLoads / 2;                   \
+    auto none = [](int) {};                                                          \
+    if (PREPARES) {                                                                  \
+      NEXT(0);                                                                       \
+      NEXT(1);                                                                       \
+      all_landed();                                                                  \
+      __syncthreads();                                                               \
+    }                                                                                \
+    _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0, smem);             \
+    all_landed();                                                                    \
+    __syncthreads();                                                                 \
+    if (STAGES > 1) {                                                                \
+      _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1, smem + kStage);  \
+    }                                                                                \
+    if (PREPARES) NEXT(2);                                                           \
+    read_q(smem, 0, 0);                                                              \
+    read_p(smem, 0, 0, 0);                                                           \
+    for (int st = 0; st < STAGES; ++st) {                                            \
+      char* buf = smem + (st & 1) * kStage;                                          \
+      char* other = smem + ((st + 1) & 1) * kStage;                                  \
+      if (kHalves == 2) {                                                            \
+        read_p(buf, 0, 1, 1);                                                        \
+      } else {                                                                       \
+        read_q(buf, 1, 1);                                                           \
+        read_p(buf, 1, 0, 1);                                                        \
+      }                                                                              \
+      const bool more = st > 0 && st + 1 < STAGES, refill = st + 2 < STAGES;         \
+      mul(0, 0, 0, kLoads - kFirst, [&](int i) {                                     \
+        if (more) LOAD(kFirst + i, st + 1, other);                                   \
+      });                                                                            \
+      if (PREPARES && st > 0) NEXT(st + 2);                                          \
+      if (kHalves == 2) {                                                            \
+        read_q(buf, 1, 1);                                                           \
+        read_p(buf, 1, 0, 0);                                                        \
+        mul(0, 1, 1, 0, none);                                                       \
+        read_p(buf, 1, 1, 1);                                                        \
+        mul(1, 0, 0, 0, none);                                                       \
+      }                                                                              \
+      all_landed();                                                                  \
+      __syncthreads();                                                               \
+      if (st + 1 < STAGES) {                                                         \
+        read_q(other, 0, 0);                                                         \
+        read_p(other, 0, 0, 0);                                                      \
+      }                                                                              \
+      constexpr int kLast = kHalves == 2 ? 1 : 0;                                    \
+      mul(1, kLast, 1, kFirst, [&](int i) {                                          \
+        if (refill) LOAD(i, st + 2, buf);                                            \
+      });                                                                            \
+    }                                                                                \
+  }
+
 struct RowsArgs {
   const void* p;       // rows [n][ld_p], contraction along
   const void* q;       // matrices [groups][...]
@@ -428,30 +568,35 @@ struct RowsArgs {
   int y_f32, y_vec;    // y_vec: four columns can be stored at once
 };
 
-// four neighbouring results of one row
+// Sixteen neighbouring results of one row, v[j] the j-th four of them; `left` columns are left.
+// vec: 16 bytes can be stored at once.
 template <typename T>
-__device__ __forceinline__ void store4(void* y, int64_t at, int left, bool f32, bool vec, f32x4 v) {
+__device__ __forceinline__ void store16(void* y, int64_t at, int left, bool f32, bool vec, const f32x4* v) {
   if (left <= 0) return;
   if (f32 || sizeof(T) == 4) {
     float* d = static_cast<float*>(y) + at;
-    if (vec && left >= 4) {
-      *reinterpret_cast<f32x4*>(d) = v;
+    if (vec && left >= 16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(d + 4 * j) = v[j];
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < left) d[i] = v[i];
+      for (int i = 0; i < 16; ++i)
+        if (i < left) d[i] = v[i >> 2][i & 3];
     }
   } else if constexpr (sizeof(T) == 2) {
     T* d = static_cast<T*>(y) + at;
-    if (vec && left >= 4) {
-      T h[4];
+    if (vec && left >= 16) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) Elem<T>::store(&h[i], v[i]);
-      *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<u32x2*>(h);
+      for (int h = 0; h < 2; ++h) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[2 * h + (i >> 2)][i & 3];
+        *reinterpret_cast<u32x4*>(d + 8 * h) = Elem<T>::pack(f);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < left) Elem<T>::store(d + i, v[i]);
+      for (int i = 0; i < 16; ++i)
+        if (i < left) Elem<T>::store(d + i, v[i >> 2][i & 3]);
     }
   }
 }
@@ -461,6 +606,7 @@ template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static_assert(FN == 4, "a lane's sixteen columns");
   constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
   constexpr int kPBytes = BM * kStageBytes, kQBytes = BN * kStageBytes;
   constexpr int kPLoads = BM * 8 / kThreads, kQLoads = BN * 8 / kThreads;
@@ -474,7 +620,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   const int64_t tile = id / a.col_tiles;
   const int c0 = (int)(id % a.col_tiles) * BN;
   const int64_t e = find_group(a.g, tile, BM, lane);
-  const int64_t o0 = a.g.at(e), o1 = a.g.at(e + 1);
+  const int64_t o0 = uniform(a.g.at(e)), o1 = uniform(a.g.at(e + 1));
   const int64_t t = tile - (o0 / BM + e);
   const int64_t r0 = o0 + t * BM;
   if (t < 0 || r0 >= o1) return;   // (t < 0: only if the offsets do not ascend)
@@ -500,90 +646,94 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   if (e < a.g.groups) {
     const T* qb = static_cast<const T*>(a.q) + e * a.q_stride;
     // this lane's granules: the row and the first element inside the stage
-    const T* prow[kPLoads];
-    const T* qrow[kQLoads];
+    // (its row's distance from the first row in units of kUnit elements, 32 bits; behind the
+    // group's end row 0 stands in: such rows are multiplied and not stored)
+    constexpr int kUnit = ALIGNED ? kV : 1;
+    typedef typename std::conditional<ALIGNED, unsigned, int64_t>::type Off;
+    Off prow[kPLoads];
 #pragma unroll
     for (int i = 0; i < kPLoads; ++i) {
-      const int r = ((i * kWaves + wave) * 64 + lane) >> 3;
-      const int row = rows[r];
-      // (a tile's rows behind the group's end are multiplied too and not stored)
-      prow[i] = row >= 0 ? static_cast<const T*>(a.p) + (int64_t)row * a.ld_p : nullptr;
+      const int row = rows[((i * kWaves + wave) * 64 + lane) >> 3];
+      prow[i] = (Off)((int64_t)(row < 0 ? 0 : row) * (a.ld_p / kUnit));
     }
-#pragma unroll
-    for (int i = 0; i < kQLoads; ++i) {
-      const int q = (i * kWaves + wave) * 64 + lane;
-      if (QALONG) {
-        const int c = c0 + (q >> 3);
-        qrow[i] = c < a.cols ? qb + (int64_t)c * a.ld_q : nullptr;
-      } else {
-        qrow[i] = qb + (int64_t)(q / kQRow) * a.ld_q;
-      }
-    }
-    auto issue = [&](int st, char* buf) {
+    // granule i of this lane lies a fixed number of matrix rows behind granule 0
+    const int lin = wave * 64 + lane;
+    constexpr int kQStep = QALONG ? kThreads / 8 : kThreads / kQRow;
+    const int qfirst = QALONG ? lin >> 3 : lin / kQRow;
+    const T* qrow = qb + (int64_t)(QALONG ? c0 + qfirst : qfirst) * a.ld_q;
+    const int along = ((lin & 7) ^ along_swap_p(lin >> 3)) * kV;   // (a step of i keeps the low bits)
+    constexpr int kLoads = kPLoads + kQLoads;
+    auto load = [&](int i, int st, char* buf) {
       const int64_t k0 = (int64_t)st * kK;
-#pragma unroll
-      for (int i = 0; i < kPLoads; ++i) {
-        const int q0 = (i * kWaves + wave) * 64, q = q0 + lane;
-        fetch<T, ALIGNED>(prow[i], k0 + ((q & 7) ^ ((q >> 3) & 7)) * kV, a.depth, buf + q0 * 16, lane);
+      if (i < kPLoads) {
+        fetch<T, ALIGNED>(static_cast<const T*>(a.p) + (int64_t)prow[i] * kUnit, k0 + along, a.depth,
+                          buf + (i * kWaves + wave) * 1024, lane);
+        return;
       }
-#pragma unroll
-      for (int i = 0; i < kQLoads; ++i) {
-        const int q0 = (i * kWaves + wave) * 64, q = q0 + lane;
-        char* to = buf + kPBytes + q0 * 16;
-        if (QALONG) {
-          fetch<T, ALIGNED>(qrow[i], k0 + ((q & 7) ^ ((q >> 3) & 7)) * kV, a.depth, to, lane);
-        } else {
-          const int k = q / kQRow;
-          const int c = c0 + ((q % kQRow) ^ across_swap<T>(k)) * kV;
-          fetch<T, ALIGNED>(k0 + k < a.depth ? qrow[i] + k0 * a.ld_q : nullptr, c, a.cols, to, lane);
-        }
+      i -= kPLoads;
+      char* to = buf + kPBytes + (i * kWaves + wave) * 1024;
+      if (QALONG) {
+        const bool in = c0 + qfirst + i * kQStep < a.cols;
+        fetch<T, ALIGNED>(in ? qrow + (int64_t)(i * kQStep) * a.ld_q : nullptr,
+                          k0 + ((lin & 7) ^ along_swap_q(qfirst + i * kQStep)) * kV, a.depth, to, lane);
+      } else {
+        const int k = qfirst + i * kQStep;
+        const int c = c0 + ((lin % kQRow) ^ across_swap_q<T, BN>(k)) * kV;
+        fetch<T, ALIGNED>(k0 + k < a.depth ? qrow + (k0 + i * kQStep) * a.ld_q : nullptr, c, a.cols, to, lane);
       }
     };
     const int stages = (int)(((int64_t)a.depth + kK - 1) / kK);
-    issue(0, smem);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-      char* buf = smem + (st & 1) * (kPBytes + kQBytes);
-      if (st + 1 < stages) issue(st + 1, smem + ((st + 1) & 1) * (kPBytes + kQBytes));
+    const bool busy = pr < m;   // a wave whose rows all lie behind the group's end only loads
+    constexpr int kHalves = FM >= 4 ? 2 : 1, kHalf = FM / kHalves;
+    u32x4 pf[2][kHalf], qf[2][FN];
+    const int pplace = along_place_p(pr, lane);
+    const int qplace = kPBytes + (QALONG ? along_place_q(qc, lane) : across_place<T, BN, true>(qc, lane));
+    auto read_p = [&](const char* buf, int step, int half, int to) {
+      if (busy) read_fragments<T, BM, true, false, kHalf>(buf, pplace, step, half * kHalf, pf[to]);
+    };
+    auto read_q = [&](const char* buf, int step, int to) {
+      if (busy) read_fragments<T, BN, QALONG, true, FN>(buf, qplace, step, 0, qf[to]);
+    };
+    // `count` loads are issued between the products
+    auto mul = [&](int q, int half, int p, int count, auto&& issue) {
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        u32x4 pf[FM], qf[FN];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) pf[i] = read_along(buf, pr + i * 16, step, lane);
+      for (int i = 0; i < kHalf; ++i) {
+        if (busy)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          qf[j] = QALONG ? read_along(buf + kPBytes, qc + j * 16, step, lane)
-                         : read_across<T, BN>(buf + kPBytes, qc + j * 16, step, lane);
+          acc[half * kHalf + i][j] = Mma<T>::mul(qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
+        if (count > 0) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::mul(qf[j], pf[i], acc[i][j]);
+          for (int l = 0; l < kLoads; ++l)
+            if (l < count && l * kHalf / count == i) issue(l);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-    }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto next = [](int) {};
+    MULTIPLY_STAGES(stages, load, next, false)
   }
-  // lane: row pr + 16 i + (lane & 15), columns qc + 16 j + 4 (lane >> 4) ..
+  // lane: row pr + 16 i + (lane & 15), 16 columns from qc + 16 (lane >> 4)
+  const int c = c0 + qc + (lane >> 4) * 16;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int row = rows[pr + i * 16 + (lane & 15)];
-    if (row < 0) continue;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int c = c0 + qc + j * 16 + (lane >> 4) * 4;
-      store4<T>(a.y, (int64_t)row * a.ld_y + c, a.cols - c, a.y_f32, a.y_vec, acc[i][j]);
-    }
+    if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y + c, a.cols - c, a.y_f32, a.y_vec, acc[i]);
   }
 }
 
 // ---- dw ---------------------------------------------------------------------------------------------
-// dW_e[o][k] = sum_r dy[r][o] x[r][k]: both operands run across the contraction.  A group's rows are
-// cut into chunks of `chunk` rows (tile numbers as above); a group of one chunk is written at once, the
-// chunks of a longer one go to float32 partial results, which k_grouped_dw_join adds in chunk order.
-// Chunk t of group e has partial result number 2 floor(o_e / chunk) + t: groups of more than one
-// chunk have more than `chunk` rows, so 2 floor(rows / chunk) >= ceil(rows / chunk) numbers lie
-// between their first ones, and 2 floor(n / chunk) of them are enough.
+// dW_e[o][k] = sum_r dy[r][o] x[r][k]: both operands run across the contraction, whose length, the
+// group's rows, is ragged.  All the work is one line of units: group after group, for each tile of
+// its matrix the stages of its rows; a group has floor(o_{e+1} / kK) + 1 - floor(o_e / kK) stages in it
+// (at least as many as it needs, at least one, at most one too many), so that the place of any unit
+// follows from the offsets as for the row tiles above.  The launch's workgroups (as many as fit the
+// card at a time) each take an equal run of the line.  A tile whose stages all fall into one run is
+// stored at once; the pieces of one that is cut go to float32 partial results -- at most two a
+// workgroup: of the tile its run begins inside (number 2 w) and of the one it ends inside (2 w + 1) --
+// and k_grouped_dw_join adds them in the order of the line.
 struct DwArgs {
   const void* dy;
   const void* x;
@@ -592,158 +742,249 @@ struct DwArgs {
   Groups g;
   const int32_t* order;
   int64_t ld_dy, ld_x;
-  int64_t chunk;
   int out, k;
-  int out_tiles, k_tiles;
+  int tiles, k_tiles;
+  int wgs;
   int y_f32, y_vec;
 };
+
+// A place in the line.
+struct DwPlace {
+  int64_t e, o0, o1;   // the group and its rows
+  int tile;            // of its matrix
+  int64_t stage, stages;   // the stage, and how many the line has for each tile of the group
+};
+__device__ __forceinline__ int64_t dw_line(const DwArgs& a, int64_t kk) {
+  return (uniform(a.g.at(a.g.groups)) / kk + a.g.groups) * a.tiles;
+}
+__device__ __forceinline__ DwPlace dw_place(const DwArgs& a, int64_t u, int64_t kk, int lane) {
+  DwPlace p;
+  p.e = find_group(a.g, u / a.tiles, kk, lane);
+  if (p.e >= a.g.groups) p.e = a.g.groups - 1;   // (only if the offsets do not ascend)
+  p.o0 = uniform(a.g.at(p.e));
+  p.o1 = uniform(a.g.at(p.e + 1));
+  if (p.o1 < p.o0) p.o1 = p.o0;
+  p.stages = p.o1 / kk + 1 - p.o0 / kk;
+  int64_t in = u - (p.o0 / kk + p.e) * a.tiles;
+  if (in < 0) in = 0;
+  const int64_t t = in / p.stages;
+  p.tile = t < a.tiles ? (int)t : a.tiles - 1;
+  p.stage = in % p.stages;
+  return p;
+}
 
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static_assert(FN == 4, "a lane's sixteen columns");
+  static_assert(BM == BN, "both operands' granules lie in the same rows");
   constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
   constexpr int kPBytes = BM * kStageBytes, kQBytes = BN * kStageBytes;
-  constexpr int kPLoads = BM * 8 / kThreads, kQLoads = BN * 8 / kThreads;
-  constexpr int kPRow = BM * (int)sizeof(T) / 16, kQRow = BN * (int)sizeof(T) / 16;
+  constexpr int kPLoads = BM * 8 / kThreads;
+  constexpr int kPRow = BM * (int)sizeof(T) / 16;   // granules of a contraction row
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const int tiles = a.out_tiles * a.k_tiles;
-  const int64_t tile = id / tiles;
-  const int in_tile = (int)(id % tiles);
-  const int m0 = in_tile / a.k_tiles * BM, n0 = in_tile % a.k_tiles * BN;
-  const int64_t e = find_group(a.g, tile, a.chunk, lane);
-  if (e >= a.g.groups) return;
-  const int64_t o0 = a.g.at(e), o1 = a.g.at(e + 1);
-  const int64_t t = tile - (o0 / a.chunk + e);
-  const int64_t r0 = o0 + t * a.chunk;
-  if (t < 0 || (r0 >= o1 && t != 0)) return;   // (the first tile of an empty group writes its zeros)
-  const int64_t r1 = r0 + a.chunk < o1 ? r0 + a.chunk : o1;
-  f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // neighbours in the line share rows: they run on one XCD
+  const int64_t w = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t line = dw_line(a, kK);
+  int64_t u = line * w / a.wgs;
+  const int64_t u1 = line * (w + 1) / a.wgs;
   const int wm = wave % WM, wn = wave / WM;
   const int pc = wm * (BM / WM), qc = wn * (BN / WN);
-  if (r0 < r1) {
-    // a position's row: -1 behind the chunk
-    auto row_at = [&](int64_t pos) {
-      if (pos >= r1) return -1;
-      const int64_t r = a.order ? (int64_t)a.order[pos] : pos;
-      return r >= 0 && r < a.g.n ? (int)r : -1;
-    };
-    int prow[kPLoads], qrow[kQLoads];
-    auto look = [&](int st) {
-      const int64_t k0 = r0 + (int64_t)st * kK;
+  const int pplace = across_place<T, BM, false>(pc, lane);
+  const int qplace = kPBytes + across_place<T, BN, true>(qc, lane);
+  int* ids = reinterpret_cast<int*>(smem + 2 * (kPBytes + kQBytes));   // [2][kK] rows of a stage
+  while (u < u1) {
+    const DwPlace pl = dw_place(a, u, kK, lane);
+    const int64_t run = pl.stages - pl.stage < u1 - u ? pl.stages - pl.stage : u1 - u;
+    u += run;
+    const int m0 = pl.tile / a.k_tiles * BM, n0 = pl.tile % a.k_tiles * BN;
+    const int64_t r0 = pl.o0 + pl.stage * kK;
+    int64_t r1 = r0 + run * kK;
+    if (r1 > pl.o1) r1 = pl.o1;
+    f32x4 acc[FM][FN];
 #pragma unroll
-      for (int i = 0; i < kPLoads; ++i) prow[i] = row_at(k0 + ((i * kWaves + wave) * 64 + lane) / kPRow);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < kQLoads; ++i) qrow[i] = row_at(k0 + ((i * kWaves + wave) * 64 + lane) / kQRow);
-    };
-    auto issue = [&](char* buf) {
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r0 < r1) {
+      // The rows of a stage: `order` goes to LDS, one wave's load a stage, two stages ahead of the
+      // loads that need it (without an order the positions are the rows).
+      const int64_t stages = (r1 - r0 + kK - 1) / kK;
+      auto look = [&](int64_t st) {
+        if (!a.order || wave != 0 || st >= stages) return;
+        int64_t pos = r0 + st * kK + (lane < kK ? lane : kK - 1);
+        if (pos >= a.g.n) pos = a.g.n - 1;
+        lds_load4(a.order + pos, reinterpret_cast<char*>(ids + (st & 1) * 64));
+      };
+      constexpr int kLoads = 2 * kPLoads;   // dy's and x's granules of a row in turn
+      auto load = [&](int i, int64_t st, char* buf) {
+        const int q0 = (i / 2 * kWaves + wave) * 64;
+        int q = q0 + lane;
+        asm volatile("" : "+v"(q));   // (worked out at each load: there are no registers to keep it in)
+        const int k = q / kPRow, s = q % kPRow;
+        const int64_t first = r0 + st * kK;
+        int r = (int)first + k;
+        if (a.order) r = ids[(st & 1) * 64 + k];
+        const bool in = k < r1 - first && (unsigned)r < (unsigned)a.g.n;
+        if (i % 2 == 0) {
+          const int c = m0 + (s ^ across_swap_p<T, BM>(k)) * kV;
+          const T* row = static_cast<const T*>(a.dy) + (int64_t)r * a.ld_dy;
+          fetch<T, ALIGNED>(in ? row : nullptr, c, a.out, buf + q0 * 16, lane);
+        } else {
+          const int c = n0 + (s ^ across_swap_q<T, BN>(k)) * kV;
+          const T* row = static_cast<const T*>(a.x) + (int64_t)r * a.ld_x;
+          fetch<T, ALIGNED>(in ? row : nullptr, c, a.k, buf + kPBytes + q0 * 16, lane);
+        }
+      };
+      constexpr int kHalves = FM >= 4 ? 2 : 1, kHalf = FM / kHalves;
+      u32x4 pf[2][kHalf], qf[2][FN];
+      auto read_p = [&](const char* buf, int step, int half, int to) {
+        read_fragments<T, BM, false, false, kHalf>(buf, pplace, step, half * kHalf, pf[to]);
+      };
+      auto read_q = [&](const char* buf, int step, int to) {
+        read_fragments<T, BN, false, true, FN>(buf, qplace, step, 0, qf[to]);
+      };
+      // `count` loads are issued between the products
+      auto mul = [&](int q, int half, int p, int count, auto&& issue) {
 #pragma unroll
-      for (int i = 0; i < kPLoads; ++i) {
-        const int q0 = (i * kWaves + wave) * 64, q = q0 + lane;
-        const int c = m0 + ((q % kPRow) ^ across_swap<T>(q / kPRow)) * kV;
-        const T* row = prow[i] >= 0 ? static_cast<const T*>(a.dy) + (int64_t)prow[i] * a.ld_dy : nullptr;
-        fetch<T, ALIGNED>(row, c, a.out, buf + q0 * 16, lane);
-      }
+        for (int i = 0; i < kHalf; ++i) {
 #pragma unroll
-      for (int i = 0; i < kQLoads; ++i) {
-        const int q0 = (i * kWaves + wave) * 64, q = q0 + lane;
-        const int c = n0 + ((q % kQRow) ^ across_swap<T>(q / kQRow)) * kV;
-        const T* row = qrow[i] >= 0 ? static_cast<const T*>(a.x) + (int64_t)qrow[i] * a.ld_x : nullptr;
-        fetch<T, ALIGNED>(row, c, a.k, buf + kPBytes + q0 * 16, lane);
-      }
-    };
-    const int stages = (int)((r1 - r0 + kK - 1) / kK);
-    look(0);
-    issue(smem);
-    look(1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-      char* buf = smem + (st & 1) * (kPBytes + kQBytes);
-      if (st + 1 < stages) {
-        issue(smem + ((st + 1) & 1) * (kPBytes + kQBytes));
-        look(st + 2);
-      }
+          for (int j = 0; j < FN; ++j)
+            acc[half * kHalf + i][j] = Mma<T>::mul(qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
+          if (count > 0) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        u32x4 pf[FM], qf[FN];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) pf[i] = read_across<T, BM>(buf, pc + i * 16, step, lane);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) qf[j] = read_across<T, BN>(buf + kPBytes, qc + j * 16, step, lane);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::mul(qf[j], pf[i], acc[i][j]);
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+            for (int l = 0; l < kLoads; ++l)
+              if (l < count && l * kHalf / count == i) issue(l);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      MULTIPLY_STAGES(stages, load, look, true)
+      __syncthreads();   // the buffers are free for the next run's loads
     }
-  }
-  const bool whole = o1 - o0 <= a.chunk;
-  const int64_t slot = whole ? e : 2 * (o0 / a.chunk) + t;
-  void* to = whole ? a.dw : static_cast<void*>(a.part);
-  const bool f32 = !whole || a.y_f32;
+    const bool whole = pl.stage == 0 && run == pl.stages;
+    if (whole) {
+      const int c = n0 + qc + (lane >> 4) * 16;
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int o = m0 + pc + i * 16 + (lane & 15);
-    if (o >= a.out) continue;
+      for (int i = 0; i < FM; ++i) {
+        const int o = m0 + pc + i * 16 + (lane & 15);
+        if (o < a.out) store16<T>(a.dw, (pl.e * a.out + o) * a.k + c, a.k - c, a.y_f32, a.y_vec, acc[i]);
+      }
+    } else {
+      // 16 bytes a lane, lanes side by side; the join undoes the order
+      f32x4* part = reinterpret_cast<f32x4*>(a.part) +
+                    (size_t)(2 * w + (pl.stage == 0 ? 1 : 0)) * (BM * BN / 4) + threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int c = n0 + qc + j * 16 + (lane >> 4) * 4;
-      store4<T>(to, (slot * a.out + o) * a.k + c, a.k - c, f32, a.y_vec, acc[i][j]);
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) part[(i * FN + j) * kThreads] = acc[i][j];
     }
   }
 }
 
-// Adds the chunks of the groups of more than one.  Such a group has more than `chunk` rows and holds
-// exactly one position j * chunk in [o_e, o_e + chunk): workgroup row j looks for it.
-template <typename T>
-__global__ __launch_bounds__(256) void k_grouped_dw_join(DwArgs a) {
+// Adds the pieces of the tile that workgroup y's run ends inside, if it also begins there (the
+// workgroups that lie wholly inside a tile leave it to the one where the tile begins).  A workgroup
+// here takes 1 / gridDim.x of the tile, 64 f32x4 a wave at a time.  Few pieces: each wave adds all of
+// them, in the order of the line.  Many (a long group under few tiles): the four waves share the
+// pieces of the same 64, every fourth each, and their sums are added in the waves' order.  Either way
+// the order depends on the sizes alone.
+constexpr int kJoinWaves = 4;
+constexpr int kJoinFew = 8;
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
+  constexpr int kThreads = WM * WN * 64, kK = Mma<T>::kK, FN = 4;
+  __shared__ f32x4 sums[kJoinWaves][64];
   const int lane = threadIdx.x & 63;
-  const int64_t pos = (int64_t)blockIdx.y * a.chunk;
-  if (pos >= a.g.n) return;
-  // the group that holds position pos: the last e with at(e) <= pos (empty groups pushed aside)
-  int64_t lo = 0, hi = a.g.groups + 1;
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) >> 6;
-    const int64_t e = lo + lane * step;
-    int c = __popcll(__ballot(e < hi && a.g.at(e) <= pos));
-    c = c > 1 ? c - 1 : 0;
-    lo += c * step;
-    hi = lo + step < hi ? lo + step : hi;
-  }
-  if (lo >= a.g.groups) return;
-  const int64_t o0 = a.g.at(lo), rows = a.g.at(lo + 1) - o0;
-  if (rows <= a.chunk || (o0 + a.chunk - 1) / a.chunk != (int64_t)blockIdx.y) return;
-  const int64_t chunks = (rows + a.chunk - 1) / a.chunk;
-  const int64_t size = (int64_t)a.out * a.k;
-  const float* part = a.part + 2 * (o0 / a.chunk) * size;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t w = blockIdx.y;
+  const int64_t line = dw_line(a, kK);
+  const int64_t u0 = line * w / a.wgs, u1 = line * (w + 1) / a.wgs;
+  if (u1 >= line || u0 >= u1) return;
+  const DwPlace pl = dw_place(a, u1, kK, lane);
+  const int64_t begin = u1 - pl.stage, end = begin + pl.stages;
+  if (pl.stage == 0 || begin < u0) return;
+  // the last workgroup with a unit of the tile: it holds unit end - 1
+  const int64_t last = (end * a.wgs - 1) / line;
+  constexpr int kTile = BM * BN / 4;
+  const f32x4* part = reinterpret_cast<const f32x4*>(a.part);
+  // piece v (workgroup w + v) of the tile; an empty run holds none
+  auto piece = [&](int64_t v, int at) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    const int left = size - i < 4 ? (int)(size - i) : 4;
-    for (int64_t t = 0; t < chunks; ++t) {
-      if (a.y_vec) {
-        s += *reinterpret_cast<const f32x4*>(part + t * size + i);
+    if (v == w) s = part[(size_t)(2 * v + 1) * kTile + at];
+    else if (line * v / a.wgs != line * (v + 1) / a.wgs) s = part[(size_t)(2 * v) * kTile + at];
+    return s;
+  };
+  auto put = [&](int at, f32x4 s) {
+    // the lane of k_grouped_dw that wrote this f32x4, and which of its products
+    const int t = at % kThreads, ij = at / kThreads;
+    const int tl = t & 63, tw = t >> 6;
+    const int o = pl.tile / a.k_tiles * BM + tw % WM * (BM / WM) + ij / FN * 16 + (tl & 15);
+    const int c = pl.tile % a.k_tiles * BN + tw / WM * (BN / WN) + (tl >> 4) * 16 + ij % FN * 4;
+    if (o >= a.out) return;
+    const int64_t to = (pl.e * a.out + o) * a.k + c;
+    const int left = a.k - c;
+    if (a.y_f32 || sizeof(T) == 4) {
+      float* d = static_cast<float*>(a.dw) + to;
+      if (a.y_vec && left >= 4) {
+        *reinterpret_cast<f32x4*>(d) = s;
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (q < left) s[q] += part[t * size + i + q];
+          if (q < left) d[q] = s[q];
+      }
+    } else if constexpr (sizeof(T) == 2) {
+      T* d = static_cast<T*>(a.dw) + to;
+      T h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) Elem<T>::store(&h[q], s[q]);
+      if (a.y_vec && left >= 4) {
+        *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<u32x2*>(h);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < left) d[q] = h[q];
       }
     }
-    store4<T>(a.dw, lo * size + i, left, a.y_f32, a.y_vec, s);
+  };
+  const int span = kTile / (int)gridDim.x;
+  const int at0 = (int)blockIdx.x * span;
+  if (last - w < kJoinFew) {
+    for (int at = at0 + (int)threadIdx.x; at < at0 + span; at += kJoinWaves * 64) {
+      f32x4 s = piece(w, at);
+      for (int64_t v = w + 1; v <= last; ++v) s += piece(v, at);
+      put(at, s);
+    }
+    return;
+  }
+  for (int at = at0 + lane; at < at0 + span; at += 64) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    int64_t v = w + wave;
+    for (; v + 3 * kJoinWaves <= last; v += 4 * kJoinWaves) {
+      f32x4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = piece(v + i * kJoinWaves, at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += q[i];
+    }
+    for (; v <= last; v += kJoinWaves) s += piece(v, at);
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int q = 1; q < kJoinWaves; ++q) s += sums[q][lane];
+      put(at, s);
+    }
+    __syncthreads();
   }
 }
 
 template <int BM, int BN>
-constexpr int rows_lds() { return 2 * (BM + BN) * kStageBytes + BM * 4; }
+constexpr int rows_lds() { return 2 * (BM + BN) * kStageBytes + (BM > 128 ? BM : 128) * 4; }
 
 template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 hipError_t rows_launch(RowsArgs a, hipStream_t s) {
@@ -755,56 +996,106 @@ hipError_t rows_launch(RowsArgs a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// The tile sizes: workgroups of 256 x 256 (8 waves of 128 x 64, one workgroup a CU), 128 x 128 (4 waves
+// of 64 x 64, two a CU) and 64 x 64 (4 waves of 16 x 64, four a CU).
+constexpr int kTileSize[3] = {256, 128, 64};
+constexpr int kPerCu[3] = {1, 2, 4};
+// Rate of a full CU relative to 256 x 256 tiles (a smaller tile reads more of LDS and L2 a product;
+// float32 products are eight to sixteen times slower and do not notice)
+constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {1.0, 1.0, 0.9};
+
+// The tile with the least time for `tiles(size)` tiles: rounds of the card times a round's work.
+template <typename F>
+int pick_tile(int type, F tiles) {
+  const double* rate = type == IC_F32 ? kRate32 : kRate16;
+  int best = 2;
+  double least = 1e300;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t slots = (int64_t)kCUs * kPerCu[i];
+    const int64_t rounds = (tiles(kTileSize[i]) + slots - 1) / slots;
+    const double t = (double)rounds * kPerCu[i] * kTileSize[i] * kTileSize[i] / rate[i];
+    if (t < least) {
+      least = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
 template <typename T, bool QALONG>
-hipError_t rows_typed(const RowsArgs& a, bool aligned, hipStream_t s) {
-  if (!aligned) return rows_launch<T, 64, 64, 2, 2, QALONG, false>(a, s);
-  return rows_launch<T, 128, 128, 2, 2, QALONG, true>(a, s);
+hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) {
+  if (!aligned) return rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
+  const int tile = pick_tile(type, [&](int size) {
+    return (a.g.n / size + a.g.groups) * ((a.cols + size - 1) / size);
+  });
+  if (tile == 0) return rows_launch<T, 256, 256, 2, 4, QALONG, true>(a, s);
+  if (tile == 1) return rows_launch<T, 128, 128, 2, 2, QALONG, true>(a, s);
+  return rows_launch<T, 64, 64, 4, 1, QALONG, true>(a, s);
 }
 
-// Rows of a chunk: 2048 workgroups where the groups are long, at least 512 rows, and partial
-// results of at most 256 MB.
-int64_t dw_chunk(int64_t n, int out, int k) {
-  const int64_t tiles = (int64_t)((out + 127) / 128) * ((k + 127) / 128);
-  int64_t chunk = (n * tiles + 2047) / 2048;
-  const int64_t bytes = 2 * n * (int64_t)out * k * 4;
-  const int64_t by_memory = (bytes + ((int64_t)1 << 28) - 1) >> 28;
-  if (chunk < by_memory) chunk = by_memory;
-  if (chunk < 512) chunk = 512;
-  return (chunk + 63) / 64 * 64;
-}
-
+// Whether 16-byte granules can be loaded, and a granule's distance from the first row fits 32 bits.
 bool grouped_aligned(const GroupedCall& c, bool dw) {
   const int v = c.type == IC_F32 ? 4 : 8;
   const int b = c.type == IC_F32 ? 4 : 2;
   auto fits = [&](const void* p, int64_t ld) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * b) % 16 == 0;
   };
+  if (!dw && c.n * (c.ld_x * b / 16) > 0xffffffffll) return false;
   if (dw) return fits(c.x, c.ld_x) && fits(c.w, c.ld_w) && c.k % v == 0 && c.out % v == 0;
   return fits(c.x, c.ld_x) && fits(c.w, c.k) && c.k % v == 0 && c.out % v == 0;
 }
 
+// How dw runs: the tile with the least time for its part of the line, and how many workgroups.
+struct DwPlan {
+  int tile;
+  int wgs;
+};
+DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned) {
+  const int kk = kStageBytes / (type == IC_F32 ? 4 : 2);
+  const double* rate = type == IC_F32 ? kRate32 : kRate16;
+  DwPlan best = {2, 1};
+  double least = 1e300;
+  for (int i = aligned ? 0 : 2; i < 3; ++i) {
+    const int size = kTileSize[i];
+    const double tiles = (double)((out + size - 1) / size) * ((k + size - 1) / size);
+    const double line = ((double)(n / kk) + groups) * tiles;
+    // at least six units a workgroup (a piece costs its partial result and the start of a pipeline:
+    // the time of about six units as well)
+    double wgs = line / 6;
+    const double slots = (double)kCUs * kPerCu[i];
+    wgs = wgs < 1 ? 1 : wgs > slots ? slots : wgs;
+    const double t = (line / wgs + 6) * kPerCu[i] * size * size / rate[i];
+    if (t < least) {
+      least = t;
+      best = DwPlan{i, (int)wgs};
+    }
+  }
+  return best;
+}
+size_t dw_scratch_of(const DwPlan& p) {
+  return (size_t)2 * p.wgs * kTileSize[p.tile] * kTileSize[p.tile] * 4;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
 hipError_t dw_launch(DwArgs a, hipStream_t s) {
-  a.out_tiles = (a.out + BM - 1) / BM;
   a.k_tiles = (a.k + BN - 1) / BN;
-  const int64_t grid = (a.g.n / a.chunk + a.g.groups + 1) * a.out_tiles * a.k_tiles;
-  if (grid * (WM * WN * 64) > 0xffffffffll) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_grouped_dw<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)grid), dim3(WM * WN * 64),
+  const int64_t tiles = (int64_t)((a.out + BM - 1) / BM) * a.k_tiles;
+  if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+  a.tiles = (int)tiles;
+  hipLaunchKernelGGL((k_grouped_dw<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)a.wgs), dim3(WM * WN * 64),
                      (rows_lds<BM, BN>()), s, a);
-  if (a.g.n > a.chunk) {
-    int64_t x = ((int64_t)a.out * a.k + 1023) / 1024;
-    if (x > 4096) x = 4096;
-    const int64_t y = (a.g.n + a.chunk - 1) / a.chunk;
-    if (y > 65535) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_grouped_dw_join<T>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, s, a);
-  }
+  if (a.wgs > 1)
+    hipLaunchKernelGGL((k_grouped_dw_join<T, BM, BN, WM, WN>), dim3(BM * BN / 4096, (unsigned)(a.wgs - 1)),
+                       dim3(kJoinWaves * 64), 0, s, a);
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t dw_typed(DwArgs a, bool aligned, hipStream_t s) {
-  if (!aligned) return dw_launch<T, 64, 64, 2, 2, false>(a, s);
-  return dw_launch<T, 128, 128, 2, 2, true>(a, s);
+hipError_t dw_typed(const DwArgs& a, int tile, bool aligned, hipStream_t s) {
+  if (!aligned) return dw_launch<T, 64, 64, 4, 1, false>(a, s);
+  if (tile == 0) return dw_launch<T, 256, 256, 2, 4, true>(a, s);
+  if (tile == 1) return dw_launch<T, 128, 128, 2, 2, true>(a, s);
+  return dw_launch<T, 64, 64, 4, 1, true>(a, s);
 }
 
 template <typename Kernel>
@@ -817,6 +1108,9 @@ hipError_t allow_typed() {
   hipError_t e = allow(k_grouped_rows<T, 128, 128, 2, 2, true, true>, rows_lds<128, 128>());
   if (e == hipSuccess) e = allow(k_grouped_rows<T, 128, 128, 2, 2, false, true>, rows_lds<128, 128>());
   if (e == hipSuccess) e = allow(k_grouped_dw<T, 128, 128, 2, 2, true>, rows_lds<128, 128>());
+  if (e == hipSuccess) e = allow(k_grouped_rows<T, 256, 256, 2, 4, true, true>, rows_lds<256, 256>());
+  if (e == hipSuccess) e = allow(k_grouped_rows<T, 256, 256, 2, 4, false, true>, rows_lds<256, 256>());
+  if (e == hipSuccess) e = allow(k_grouped_dw<T, 256, 256, 2, 4, true>, rows_lds<256, 256>());
   return e;
 }
 
@@ -880,16 +1174,17 @@ hipError_t launch_grouped_rows(const GroupedCall& c, bool dx, hipStream_t s) {
   a.cols = dx ? c.k : c.out;
   a.y_f32 = c.y_f32 || c.type == IC_F32;
   const int yb = a.y_f32 ? 4 : 2;
-  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) % (4 * yb)) == 0 && c.ld_y % 4 == 0;
+  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && (c.ld_y * yb) % 16 == 0;
   const bool al = grouped_aligned(c, false);
-  if (c.type == IC_F32) return dx ? rows_typed<float, false>(a, al, s) : rows_typed<float, true>(a, al, s);
-  if (c.type == IC_BF16) return dx ? rows_typed<bf16_t, false>(a, al, s) : rows_typed<bf16_t, true>(a, al, s);
-  return dx ? rows_typed<f16_t, false>(a, al, s) : rows_typed<f16_t, true>(a, al, s);
+  if (c.type == IC_F32) return dx ? rows_typed<float, false>(a, c.type, al, s) : rows_typed<float, true>(a, c.type, al, s);
+  if (c.type == IC_BF16) return dx ? rows_typed<bf16_t, false>(a, c.type, al, s) : rows_typed<bf16_t, true>(a, c.type, al, s);
+  return dx ? rows_typed<f16_t, false>(a, c.type, al, s) : rows_typed<f16_t, true>(a, c.type, al, s);
 }
 
-size_t grouped_dw_scratch(int64_t n, int out, int k) {
-  const int64_t chunk = dw_chunk(n, out, k);
-  return n <= chunk ? 0 : (size_t)(2 * (n / chunk)) * out * k * 4;
+size_t grouped_dw_scratch(int64_t n, int64_t groups, int k, int out, int type) {
+  const size_t a = dw_scratch_of(dw_plan(n, groups, k, out, type, true));
+  const size_t b = dw_scratch_of(dw_plan(n, groups, k, out, type, false));
+  return a > b ? a : b;
 }
 
 hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s) {
@@ -903,14 +1198,16 @@ hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s)
   a.order = c.order;
   a.ld_dy = c.ld_w;
   a.ld_x = c.ld_x;
-  a.chunk = dw_chunk(c.n, c.out, c.k);
+  const DwPlan plan = dw_plan(c.n, c.groups, c.k, c.out, c.type, al);
+  a.wgs = plan.wgs;
   a.out = c.out;
   a.k = c.k;
   a.y_f32 = c.y_f32 || c.type == IC_F32;
-  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && c.k % 4 == 0;
-  if (c.type == IC_F32) return dw_typed<float>(a, al, s);
-  if (c.type == IC_BF16) return dw_typed<bf16_t>(a, al, s);
-  return dw_typed<f16_t>(a, al, s);
+  const int yb = a.y_f32 ? 4 : 2;
+  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && ((int64_t)c.k * yb) % 16 == 0;
+  if (c.type == IC_F32) return dw_typed<float>(a, plan.tile, al, s);
+  if (c.type == IC_BF16) return dw_typed<bf16_t>(a, plan.tile, al, s);
+  return dw_typed<f16_t>(a, plan.tile, al, s);
 }
 
 }  // namespace ic

@@ -273,7 +273,7 @@ struct GroupedCall {
   int y_f32;              // the result is float32 whatever the type
 };
 hipError_t launch_grouped_rows(const GroupedCall& c, bool dx, hipStream_t s);
-size_t grouped_dw_scratch(int64_t n, int out, int k);
+size_t grouped_dw_scratch(int64_t n, int64_t groups, int k, int out, int type);
 hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s);
 
 }  // namespace ic

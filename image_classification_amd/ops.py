@@ -1067,7 +1067,7 @@ def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
     if not dw.is_contiguous():
         raise ValueError("out must be contiguous")
     lib = _lib.load()
-    nbytes = lib.ic_grouped_matmul_dw_scratch(n, k, o)
+    nbytes = lib.ic_grouped_matmul_dw_scratch(n, groups, k, o, t)
     scratch = _scratch(nbytes, x.device)
     rc = lib.ic_grouped_matmul_dw(_lib.handle(dev), _ptr(dy), ld_dy, _ptr(x), ld_x, _ptr(dw),
                                   _ptr(offsets), _ptr(order), n, groups, k, o, t, yt, _ptr(scratch),

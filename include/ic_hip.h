@@ -354,7 +354,7 @@ int ic_grouped_matmul_dx(void* handle, const void* dy, int64_t ld_dy, const void
                          int64_t n_groups, int k, int out, int dtype, int y_dtype, void* stream);
 /* dW_g = sum over the rows i of group g of dy_i x_i^T (zeros for a group without rows): the gradient
  * with respect to w.  dw [n_groups][out][k].  The order of every sum is fixed. */
-int64_t ic_grouped_matmul_dw_scratch(int64_t n, int k, int out);
+int64_t ic_grouped_matmul_dw_scratch(int64_t n, int64_t n_groups, int k, int out, int dtype);
 int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
                          void* dw, const int64_t* offsets, const int32_t* order, int64_t n,
                          int64_t n_groups, int k, int out, int dtype, int y_dtype, void* scratch,

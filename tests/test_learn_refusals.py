@@ -77,10 +77,12 @@ def test_scratch_sizes():
     lib = _lib.load()
     assert lib.ic_group_rows_scratch(4096, 1000) == 0
     assert lib.ic_group_rows_scratch(1_000_000, 10_000) >= 12_000_000   # pairs and sorted codes
-    assert lib.ic_grouped_matmul_dw_scratch(500, 128, 64) == 0
-    # chunks of at least 512 rows, at most two partial results a chunk, 256 MB in all
-    for n, k, out in ((1_000_000, 128, 64), (65536, 2048, 2048), (3_000_000, 2048, 16), (4097, 8, 8)):
-        assert 0 <= lib.ic_grouped_matmul_dw_scratch(n, k, out) <= max(1 << 28, 2 * (n // 512) * k * out * 4)
+    # two partial tiles a workgroup: at most 256 x 2 x 256 x 256 floats, little for little work
+    for t in (0, 1, 2):
+        assert 0 < lib.ic_grouped_matmul_dw_scratch(0, 1, 8, 8, t) <= 2 * 64 * 64 * 4
+        for n, e, k, out in ((1_000_000, 10_000, 128, 64), (65536, 16, 2048, 2048), (3_000_000, 1, 2048, 16),
+                             (4097, 3, 8, 8)):
+            assert 0 < lib.ic_grouped_matmul_dw_scratch(n, e, k, out, t) <= 2 * 256 * 256 * 256 * 4
     assert lib.ic_label_logprobs_scratch(100_000, 1000, 1, 5) == 0
     assert lib.ic_label_logprobs_scratch(4, 65536, 0, 5) > 0
     assert lib.ic_label_logprobs_scratch(4, 65536, 9, 5) == 0
@@ -104,13 +106,63 @@ def test_every_tile_of_ragged_groups_has_a_number():
             tiles = -(-(ends[e] - off[e]) // bm)
             nxt = first[e + 1] if e < groups else total
             assert first[e] + tiles <= nxt
-        # partial results of groups of more than one chunk
-        used = set()
-        for e in range(groups):
-            rows = off[e + 1] - off[e]
-            if rows > bm:
-                slots = range(2 * (off[e] // bm), 2 * (off[e] // bm) + -(-rows // bm))
-                assert not used & set(slots) and max(slots) < 2 * (n // bm)
-                used |= set(slots)
-                j = -(-off[e] // bm)
-                assert off[e] <= j * bm < off[e] + bm and j * bm < off[e + 1] and j <= (n - 1) // bm
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_the_line_of_a_weight_gradient_is_covered_once(seed):
+    # the units of every tile of every group: each stage in exactly one workgroup's run, pieces of a
+    # cut tile in at most one begin and one end place of a workgroup, every tile joined exactly once
+    import numpy as np
+    rng = np.random.default_rng(seed)
+    kk = int(rng.choice([32, 64]))
+    groups, tiles, wgs = int(rng.integers(1, 9)), int(rng.integers(1, 5)), int(rng.integers(1, 40))
+    sizes = rng.choice([0, 1, kk, kk + 1, int(rng.integers(0, 2000))], groups)
+    off = np.concatenate([[0], np.cumsum(sizes)])
+    first = [int(off[e]) // kk + e for e in range(groups + 1)]
+    line = first[groups] * tiles
+
+    def place(u):
+        e = max(e for e in range(groups + 1) if first[e] <= u // tiles)
+        stages = int(off[e + 1]) // kk + 1 - int(off[e]) // kk
+        inside = u - first[e] * tiles
+        assert e < groups and 0 <= inside // stages < tiles
+        return e, inside // stages, inside % stages, stages
+
+    seen, pieces, whole, joined = {}, {}, set(), set()
+    for w in range(wgs):
+        u, u1 = line * w // wgs, line * (w + 1) // wgs
+        while u < u1:
+            e, t, st, stages = place(u)
+            run = min(stages - st, u1 - u)
+            assert stages * kk >= sizes[e]
+            for i in range(st, st + run):
+                assert (e, t, i) not in seen
+                seen[e, t, i] = w
+            if st == 0 and run == stages:
+                whole.add((e, t))
+            else:
+                key = (w, 1 if st == 0 else 0)
+                assert key not in pieces
+                pieces[key] = (e, t)
+            u += run
+    assert len(seen) == line
+    for w in range(wgs - 1):
+        u0, u1 = line * w // wgs, line * (w + 1) // wgs
+        if u1 >= line or u0 >= u1:
+            continue
+        e, t, st, stages = place(u1)
+        begin, end = u1 - st, u1 - st + stages
+        if st == 0 or begin < u0:
+            continue
+        mine = []
+        for v in range(w, wgs):
+            if v > w and line * v // wgs >= end:
+                break
+            if v > w and line * v // wgs == line * (v + 1) // wgs:
+                continue
+            mine.append((v, 1 if v == w else 0))
+        assert [pieces.pop(key) for key in mine] == [(e, t)] * len(mine)
+        assert (e, t) not in joined
+        joined.add((e, t))
+    assert not pieces and not (whole & joined)
+    assert whole | joined == {(e, t) for e in range(groups) for t in range(tiles)}
