@@ -36,57 +36,138 @@ namespace {
 static __device__ __align__(16) const unsigned kZeroGranule[4] = {0u, 0u, 0u, 0u};
 
 // ---- group_rows ----------------------------------------------------------------------------------
-constexpr int kSmallRows = 4096;
+// A least-significant-digit radix sort of (group, row), digits of up to 9 bits, groups + 1 key values
+// (the last one for rows of no group).  Equal digits keep their order: a wave takes 64 consecutive
+// rows at a time and ranks them among the lanes of equal digit with one ballot per digit bit; the
+// waves' counts are added in wave order.
+constexpr int kMaxDigitBits = 9;
 
-// Few rows: one workgroup sorts (group << 12 | row) in LDS.
+// The rank of this lane's digit among the 64 rows of the wave, on top of what cnt (this wave's counters)
+// already holds; the counters go up.  Lanes that are not `in` hold no row.
+template <typename Count>
+__device__ __forceinline__ unsigned rank_in_wave(Count* cnt, unsigned d, bool in, int digit_bits,
+                                                 unsigned long long below) {
+  unsigned long long same = __ballot(in);
+  for (int b = 0; b < digit_bits; ++b) {
+    const unsigned long long ones = __ballot((d >> b) & 1u);
+    same &= ((d >> b) & 1u) ? ones : ~ones;
+  }
+  // (only this wave touches its counters: lanes of equal digit read before the first one adds)
+  const unsigned old = cnt[d];
+  __builtin_amdgcn_wave_barrier();
+  if (in && (same & below) == 0) cnt[d] = (Count)(old + __popcll(same));
+  __builtin_amdgcn_wave_barrier();
+  return old + __popcll(same & below);
+}
+
+// Few rows: one workgroup, everything in LDS (bitonic sorting took 18.6 us for 1000 rows: 66 steps of a
+// barrier each).
+constexpr int kSmallRows = 4096;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restrict__ codes, int n,
-                                                         int64_t groups, int32_t* __restrict__ order,
+                                                         int64_t groups, int passes, int digit_bits,
+                                                         int32_t* __restrict__ order,
                                                          int64_t* __restrict__ offsets) {
-  __shared__ unsigned buf[kSmallRows];
-  int P = 2 * THREADS;
-  while (P < n) P <<= 1;
-  for (int p = threadIdx.x; p < P; p += THREADS) {
-    unsigned key = 0xffffffffu;
-    if (p < n) {
-      const int32_t c = codes[p];
-      const unsigned g = c >= 0 && c < groups ? (unsigned)c : 0xfffffu;
-      key = (g << 12) | (unsigned)p;
+  constexpr int kWaves = THREADS / 64, kMost = THREADS == 1024 ? kSmallRows / THREADS : 1;
+  constexpr int kRows = THREADS * kMost;
+  __shared__ unsigned short cnt[kWaves][1 << kMaxDigitBits];   // (at most 4096 rows)
+  __shared__ unsigned keys[kRows];
+  __shared__ unsigned short rows[kRows];
+  __shared__ unsigned wave_sum[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int digits = 1 << digit_bits;
+  const int rounds = (n + THREADS - 1) / THREADS;   // of 64 rows a wave
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const int base = wave * 64 * rounds;
+  unsigned key[kMost], row[kMost], rank[kMost];
+#pragma unroll
+  for (int r = 0; r < kMost; ++r) {
+    const int i = base + r * 64 + lane;
+    key[r] = 0;
+    row[r] = (unsigned)i;
+    if (r < rounds && i < n) {
+      const int32_t c = codes[i];
+      key[r] = c >= 0 && c < groups ? (unsigned)c : (unsigned)groups;
     }
-    buf[p] = key;
   }
-  for (int size = 2; size <= P; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    for (int d = lane; d < digits; d += 64) cnt[wave][d] = 0;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < kMost; ++r) {
+      if (r >= rounds) break;
+      const bool in = base + r * 64 + lane < n;
+      const unsigned d = (key[r] >> shift) & (digits - 1);
+      rank[r] = rank_in_wave(cnt[wave], d, in, digit_bits, below);
+    }
+    __syncthreads();
+    // exclusive prefix over (digit, wave): thread d < digits sums its digit's waves
+    unsigned total = 0;
+    for (int d0 = 0; d0 < digits; d0 += THREADS) {
+      const int d = d0 + (int)threadIdx.x;
+      unsigned sum = 0;
+      if (d < digits)
+        for (int w = 0; w < kWaves; ++w) sum += cnt[w][d];
+      unsigned inc = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const unsigned up = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 63) wave_sum[wave] = inc;
       __syncthreads();
-      for (int t = threadIdx.x; t < P / 2; t += THREADS) {
-        const int pos = 2 * t - (t & (stride - 1));
-        const unsigned a = buf[pos], b = buf[pos + stride];
-        if ((a > b) == ((pos & size) == 0)) {
-          buf[pos] = b;
-          buf[pos + stride] = a;
+      unsigned run = total + inc - sum;
+      for (int w = 0; w < kWaves; ++w) {
+        const unsigned q = wave_sum[w];
+        if (w < wave) run += q;
+        total += q;
+      }
+      if (d < digits)
+        for (int w = 0; w < kWaves; ++w) {
+          const unsigned c = cnt[w][d];
+          cnt[w][d] = (unsigned short)run;
+          run += c;
         }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < kMost; ++r) {
+      if (r >= rounds) break;
+      if (base + r * 64 + lane < n) {
+        const int at = cnt[wave][(key[r] >> shift) & (digits - 1)] + (int)rank[r];
+        keys[at] = key[r];
+        rows[at] = (unsigned short)row[r];
       }
     }
+    __syncthreads();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int r = 0; r < kMost; ++r) {
+        const int i = base + r * 64 + lane;
+        if (r < rounds && i < n) {
+          key[r] = keys[i];
+          row[r] = rows[i];
+        }
+      }
+      __syncthreads();
+    }
   }
-  __syncthreads();
-  for (int p = threadIdx.x; p < n; p += THREADS) order[p] = (int32_t)(buf[p] & 4095u);
-  // (rows of no group carry the key 0xfffff, which is behind every group)
-  for (int64_t e = threadIdx.x; e <= groups; e += THREADS) {
-    const unsigned want = (e == groups ? 0xfffffu : (unsigned)e) << 12;
+  for (int p = threadIdx.x; p < n; p += THREADS) order[p] = (int32_t)rows[p];
+  for (int64_t e = threadIdx.x; e <= groups; e += THREADS) {   // the first position of a group >= e
     int lo = 0, hi = n;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (buf[mid] < want) lo = mid + 1; else hi = mid;
+      if (keys[mid] < (unsigned)e) lo = mid + 1; else hi = mid;
     }
     offsets[e] = lo;
   }
 }
 
-// Many rows: a least-significant-digit radix sort of (group, row) pairs, digits of up to 9 bits.
+// Many rows: a pass over a digit is three launches (counts per block of rows, prefixes, scatter).
 constexpr int kSortRows = 4096;     // rows of a workgroup
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kMaxDigitBits = 9;
 
 struct SortPlan {
   int bits;        // of the key: groups + 1 values, the last for rows of no group
@@ -209,17 +290,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const bool in = i < n;
     key[r] = in ? key_of(codes, pairs, i, groups) : 0u;
     const unsigned d = (key[r] >> shift) & (digits - 1);
-    unsigned long long same = __ballot(in);
-    for (int b = 0; b < digit_bits; ++b) {
-      const unsigned long long ones = __ballot((d >> b) & 1u);
-      same &= ((d >> b) & 1u) ? ones : ~ones;
-    }
-    // (only this wave touches its counters: lanes of equal digit read before the first one adds)
-    const unsigned old = cnt[wave][d];
-    rank[r] = old + __popcll(same & below);
-    __builtin_amdgcn_wave_barrier();
-    if (in && (same & below) == 0) cnt[wave][d] = old + __popcll(same);
-    __builtin_amdgcn_wave_barrier();
+    rank[r] = rank_in_wave(cnt[wave], d, in, digit_bits, below);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kSortThreads) {
@@ -340,31 +411,30 @@ __device__ __forceinline__ void lds_load4(const void* src, char* lds_wave_base) 
 }
 __device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Products of one granule of each operand (16 x 16 results).  float32 granules hold 4 elements, one
+// product of depth 4 each (kParts): lane group g of element j stands for k = 4 g + j in both operands,
+// and the order of k inside a step does not matter.  The products of one accumulator are kept apart by
+// those of the others.
 template <typename T> struct Mma;
 template <> struct Mma<float> {
-  static constexpr int kK = kStageBytes / 4;
-  // a granule of each operand: 4 products deep in k (the lane's granule, one element a product; the
-  // order of k inside a step is the same for both operands and does not matter)
-  static __device__ __forceinline__ f32x4 mul(u32x4 q, u32x4 p, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[j]), __uint_as_float(p[j]), c, 0, 0, 0);
-    return c;
+  static constexpr int kK = kStageBytes / 4, kParts = 4;
+  static __device__ __forceinline__ f32x4 mul(int part, u32x4 q, u32x4 p, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[part]), __uint_as_float(p[part]), c, 0, 0, 0);
   }
 };
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <> struct Mma<bf16_t> {
-  static constexpr int kK = kStageBytes / 2;
-  static __device__ __forceinline__ f32x4 mul(u32x4 q, u32x4 p, f32x4 c) {
+  static constexpr int kK = kStageBytes / 2, kParts = 1;
+  static __device__ __forceinline__ f32x4 mul(int, u32x4 q, u32x4 p, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q),
                                                    __builtin_bit_cast(bf16x8, p), c, 0, 0, 0);
   }
 };
 template <> struct Mma<f16_t> {
-  static constexpr int kK = kStageBytes / 2;
-  static __device__ __forceinline__ f32x4 mul(u32x4 q, u32x4 p, f32x4 c) {
+  static constexpr int kK = kStageBytes / 2, kParts = 1;
+  static __device__ __forceinline__ f32x4 mul(int, u32x4 q, u32x4 p, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, q),
                                                   __builtin_bit_cast(f16x8, p), c, 0, 0, 0);
   }
@@ -700,8 +770,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
       for (int i = 0; i < kHalf; ++i) {
         if (busy)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[half * kHalf + i][j] = Mma<T>::mul(qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
+        for (int part = 0; part < Mma<T>::kParts; ++part)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[half * kHalf + i][j] = Mma<T>::mul(part, qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
         if (count > 0) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -722,6 +794,93 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
     const int row = rows[pr + i * 16 + (lane & 15)];
     if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y + c, a.cols - c, a.y_f32, a.y_vec, acc[i]);
   }
+}
+
+// Few rows a group (single rows to serve): the matrices are the traffic, so a workgroup takes 16 rows
+// of a group and few columns and keeps as many loads in flight as its registers hold; nothing is
+// shared, so nothing goes through LDS on the way.  BYDEPTH: the four waves share the depth of the same
+// 32 columns and add their sums in LDS, in wave order; otherwise (short rows) each wave takes 16 columns
+// of its own.  A lane's granules of a chunk are neighbours (32 bytes), four lanes read 128 bytes.
+template <typename T, bool BYDEPTH>
+__global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
+  constexpr int kV = Elem<T>::kVec;
+  constexpr int kChunk = 8 * kV;                 // of the depth: 2 granules in each quarter wave
+  constexpr int CF = BYDEPTH ? 2 : 1;            // fragments of 16 columns a wave
+  constexpr int kCols = BYDEPTH ? 32 : 64;       // of a workgroup
+  constexpr int kAhead = BYDEPTH ? 4 : 2;        // chunks whose loads are in flight together
+  __shared__ f32x4 sums[BYDEPTH ? 4 : 1][CF][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t tile = (int64_t)blockIdx.x / a.col_tiles;
+  const int c0 = (int)(blockIdx.x % a.col_tiles) * kCols + (BYDEPTH ? 0 : wave * 16);
+  const int64_t e = find_group(a.g, tile, 16, lane);
+  const int64_t o0 = uniform(a.g.at(e)), o1 = uniform(a.g.at(e + 1));
+  const int64_t t = tile - (o0 / 16 + e);
+  const int64_t r0 = o0 + t * 16;
+  if (t < 0 || r0 >= o1) return;
+  int64_t row = -1;
+  if (r0 + (lane & 15) < o1) {
+    row = a.order ? (int64_t)a.order[r0 + (lane & 15)] : r0 + (lane & 15);
+    if (row < 0 || row >= a.g.n) row = -1;
+  }
+  f32x4 acc[CF];
+#pragma unroll
+  for (int j = 0; j < CF; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (e < a.g.groups) {
+    const int kq = (lane >> 4) * 2 * kV;
+    const T* p = static_cast<const T*>(a.p) + (row < 0 ? 0 : row) * a.ld_p + kq;
+    const T* q[CF];
+#pragma unroll
+    for (int j = 0; j < CF; ++j) {
+      int c = c0 + j * 16 + (lane & 15);
+      if (c >= a.cols) c = a.cols - 1;           // (its products are not stored)
+      q[j] = static_cast<const T*>(a.q) + e * a.q_stride + (int64_t)c * a.ld_q + kq;
+    }
+    const int chunks = (a.depth + kChunk - 1) / kChunk;
+    const int first = BYDEPTH ? (int)((int64_t)chunks * wave / 4) : 0;
+    const int last = BYDEPTH ? (int)((int64_t)chunks * (wave + 1) / 4) : chunks;
+    for (int c = first; c < last; c += kAhead) {
+      u32x4 pv[kAhead][2], qv[kAhead][CF][2];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = (c + i) * kChunk + h * kV;
+          const bool in = c + i < last && k + kq < a.depth;
+          pv[i][h] = in ? *reinterpret_cast<const u32x4*>(p + k) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int j = 0; j < CF; ++j)
+            qv[i][j][h] = in ? *reinterpret_cast<const u32x4*>(q[j] + k) : u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int part = 0; part < Mma<T>::kParts; ++part)
+#pragma unroll
+            for (int j = 0; j < CF; ++j) acc[j] = Mma<T>::mul(part, qv[i][j][h], pv[i][h], acc[j]);
+    }
+  }
+  if (BYDEPTH) {
+#pragma unroll
+    for (int j = 0; j < CF; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= CF) return;
+    // wave j finishes fragment j
+    acc[0] = sums[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) acc[0] += sums[w][wave][lane];
+  }
+  const int c = c0 + (BYDEPTH ? wave * 16 : 0) + (lane >> 4) * 4;
+  if (row < 0) return;
+  const int64_t at = row * a.ld_y + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < a.cols) {
+      if (a.y_f32 || sizeof(T) == 4) static_cast<float*>(a.y)[at + i] = acc[0][i];
+      else Elem<T>::store(static_cast<T*>(a.y) + at + i, acc[0][i]);
+    }
 }
 
 // ---- dw ---------------------------------------------------------------------------------------------
@@ -852,8 +1011,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
 #pragma unroll
         for (int i = 0; i < kHalf; ++i) {
 #pragma unroll
-          for (int j = 0; j < FN; ++j)
-            acc[half * kHalf + i][j] = Mma<T>::mul(qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
+          for (int part = 0; part < Mma<T>::kParts; ++part)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+              acc[half * kHalf + i][j] = Mma<T>::mul(part, qf[q][j], pf[p][i], acc[half * kHalf + i][j]);
           if (count > 0) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1002,7 +1163,7 @@ constexpr int kTileSize[3] = {256, 128, 64};
 constexpr int kPerCu[3] = {1, 2, 4};
 // Rate of a full CU relative to 256 x 256 tiles (a smaller tile reads more of LDS and L2 a product;
 // float32 products are eight to sixteen times slower and do not notice)
-constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {1.0, 1.0, 0.9};
+constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.95};
 
 // The tile with the least time for `tiles(size)` tiles: rounds of the card times a round's work.
 template <typename F>
@@ -1022,9 +1183,22 @@ int pick_tile(int type, F tiles) {
   return best;
 }
 
+// Up to 8 rows a group on average (or hardly any rows at all), forward.
+template <typename T>
+hipError_t few_launch(RowsArgs a, hipStream_t s) {
+  const bool by_depth = a.depth >= 512;
+  a.col_tiles = by_depth ? (a.cols + 31) / 32 : (a.cols + 63) / 64;
+  const int64_t grid = (a.g.n / 16 + a.g.groups + 1) * a.col_tiles;
+  if (grid * 256 > 0xffffffffll) return hipErrorInvalidValue;
+  if (by_depth) hipLaunchKernelGGL((k_grouped_few<T, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_grouped_few<T, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 template <typename T, bool QALONG>
 hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) {
   if (!aligned) return rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
+  if (QALONG && (a.g.n <= 8 * a.g.groups || a.g.n <= 32)) return few_launch<T>(a, s);
   const int tile = pick_tile(type, [&](int size) {
     return (a.g.n / size + a.g.groups) * ((a.cols + size - 1) / size);
   });
@@ -1124,20 +1298,21 @@ hipError_t grouped_init() {
 }
 
 size_t group_rows_scratch(int64_t n, int64_t groups) {
-  if (n <= kSmallRows && groups <= 0xfffff) return 0;
-  return sort_plan(n, groups).bytes;
+  return n <= kSmallRows ? 0 : sort_plan(n, groups).bytes;
 }
 
 hipError_t launch_group_rows(const int32_t* codes, int64_t n, int64_t groups, int32_t* order,
                              int64_t* offsets, void* scratch, hipStream_t s) {
-  if (n <= kSmallRows && groups <= 0xfffff) {
-    if (n <= 512)
-      hipLaunchKernelGGL(k_group_small<256>, dim3(1), dim3(256), 0, s, codes, (int)n, groups, order, offsets);
+  const SortPlan p = sort_plan(n, groups);
+  if (n <= kSmallRows) {
+    if (n <= 256)
+      hipLaunchKernelGGL(k_group_small<256>, dim3(1), dim3(256), 0, s, codes, (int)n, groups, p.passes,
+                         p.digit_bits, order, offsets);
     else
-      hipLaunchKernelGGL(k_group_small<1024>, dim3(1), dim3(1024), 0, s, codes, (int)n, groups, order, offsets);
+      hipLaunchKernelGGL(k_group_small<1024>, dim3(1), dim3(1024), 0, s, codes, (int)n, groups, p.passes,
+                         p.digit_bits, order, offsets);
     return hipGetLastError();
   }
-  const SortPlan p = sort_plan(n, groups);
   char* ws = static_cast<char*>(scratch);
   unsigned* tab = reinterpret_cast<unsigned*>(ws + p.o_tab);
   unsigned* total = reinterpret_cast<unsigned*>(ws + p.o_total);

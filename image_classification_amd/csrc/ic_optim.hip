@@ -144,48 +144,73 @@ __global__ __launch_bounds__(256) void k_adamw32(AdamTable tab, AdamArgs a) {
 
 // -- 8-bit codes -----------------------------------------------------------------------------------
 // An unsigned float code of MANT mantissa bits stands for the integer
-//     (e ? 2^MANT + f : f) << max(e - 1, 0),   e = c >> MANT, f = c & (2^MANT - 1).
+//     (e ? 2^MANT + f : f) << max(e - 1, 0),   e = c >> MANT, f = c & (2^MANT - 1),
+// which is the float32 with the code's bits at the top of its exponent and mantissa fields, times
+// 2^(126 + MANT): float32's own subnormals stand for the code's.
 template <int MANT>
-__device__ __forceinline__ unsigned code_value(unsigned c) {
-  const unsigned e = c >> MANT, f = c & ((1u << MANT) - 1u);
-  return (e ? (f | (1u << MANT)) : f) << (e ? e - 1u : 0u);
+__device__ __forceinline__ float code_float(unsigned c) {
+  return __uint_as_float(c << (23 - MANT));
 }
-// The code nearest to q >= 0 (in the same units), a middle to the even one, at most `top`.
-// float64 bits: the exponent and the 20 mantissa bits of the upper word, the rest folded into a
-// sticky bit, so that "exactly the middle" is told from "a little above it".
+// that factor, as a power of two for float64
+constexpr double kMUnit = 0x1p129, kRUnit = 0x1p130;
+
+// The code nearest to q >= 0 (in units of the smallest code above zero), a middle to the even one, at
+// most `top`.  float64 bits: the exponent and the 20 mantissa bits of the upper word, the rest folded
+// into a sticky bit, so that "exactly the middle" is told from "a little above it".  Below 2^MANT, where
+// the grid is 1, q + 2^MANT has the same grid and 2^MANT codes more.
 template <int MANT>
 __device__ __forceinline__ unsigned nearest_code(double q, unsigned top) {
-  // below 2^(MANT+1) the grid is 1: adding 2^52 rounds to an integer, to nearest even
-  constexpr double kOne52 = 4503599627370496.0;
-  if (q < (double)(2 << MANT)) return (unsigned)(int)((q + kOne52) - kOne52);
-  const unsigned long long bits = __double_as_longlong(q);
+  const bool small = q < (double)(1 << MANT);
+  const unsigned long long bits = __double_as_longlong(q + (small ? (double)(1 << MANT) : 0.0));
   unsigned hi = (unsigned)(bits >> 32);
   hi |= (unsigned)((unsigned)bits != 0u);            // sticky
   constexpr int kDrop = 20 - MANT;
   const unsigned r = hi + ((1u << (kDrop - 1)) - 1u) + ((hi >> kDrop) & 1u);
   // r >> kDrop = biased exponent and MANT bits; exponent MANT is code exponent 1
-  const unsigned c = (r >> kDrop) - ((1023u + MANT - 1u) << MANT);
+  const unsigned c = (r >> kDrop) - (((1023u + MANT - 1u) << MANT) + (small ? 1u << MANT : 0u));
   return c < top ? c : top;
 }
 
-__device__ __forceinline__ double m_value(unsigned c, double scale) {   // scale / 512 as argument
-  const unsigned mag = c & 127u;
-  const double v = (double)code_value<3>(mag) * scale;
-  const double s = (c & 128u) ? -v : v;
-  return mag == 127u ? __builtin_nan("") : s;
+// sqrt of a normal float64 > 0 to within its last bit or two: the hardware's estimate of 1 / sqrt and
+// two steps of Newton's method (the library's also scales the exponent and handles every special value)
+__device__ __forceinline__ double root_of(double v) {
+  const double y = __builtin_amdgcn_rsq(v);
+  double g = v * y, h = 0.5 * y;
+  const double r = fma(-g, h, 0.5);
+  g = fma(g, r, g);
+  h = fma(h, r, h);
+  return fma(fma(-g, g, v), h, g);
 }
-__device__ __forceinline__ double r_value(unsigned c, double scale) {
-  return c == 255u ? __builtin_nan("") : (double)code_value<4>(c) * scale;
-}
+// v = 0 becomes kTiny, whose root is far below every scale; any v above zero has a larger root
+constexpr double kTiny = 1e-290, kSeen = 1.1e-145;
 
-// largest over the 32 lanes that hold one block of 256 elements (values >= 0, compared as bits)
+// Largest over the 32 lanes that hold one block of 256 elements; values >= 0.
+template <int CTRL>
+__device__ __forceinline__ double dpp_max(double v) {
+  const unsigned long long b = __double_as_longlong(v);
+  const unsigned long long o = ((unsigned long long)dpp_u32<CTRL>(0u, (unsigned)(b >> 32)) << 32) |
+                               dpp_u32<CTRL>(0u, (unsigned)b);
+  return fmax(v, __longlong_as_double(o));
+}
 __device__ __forceinline__ double half_wave_max(double v) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double w = __shfl_xor(v, o, 64);
-    v = w > v ? w : v;
-  }
-  return v;
+  v = dpp_max<0x111>(v);
+  v = dpp_max<0x112>(v);
+  v = dpp_max<0x114>(v);
+  v = dpp_max<0x118>(v);
+  v = dpp_max<0x142>(v);   // lane 31 now holds the first 32 lanes' value, lane 63 the others'
+  const unsigned long long b = __double_as_longlong(v);
+  const int lo = (int)(unsigned)b, hi = (int)(b >> 32);
+  const bool first = (threadIdx.x & 32) == 0;
+  const unsigned l = (unsigned)(first ? __builtin_amdgcn_readlane(lo, 31) : __builtin_amdgcn_readlane(lo, 63));
+  const unsigned h = (unsigned)(first ? __builtin_amdgcn_readlane(hi, 31) : __builtin_amdgcn_readlane(hi, 63));
+  return __longlong_as_double(((unsigned long long)h << 32) | l);
+}
+// |v|, or next to nothing where v is not finite
+__device__ __forceinline__ double finite_size(double v) {
+  const unsigned long long b = __double_as_longlong(v) & 0x7fffffffffffffffull;
+  const unsigned hi = (unsigned)(b >> 32);
+  const unsigned keep = hi < 0x7ff00000u ? hi : 0u;
+  return __longlong_as_double(((unsigned long long)keep << 32) | (unsigned)b);
 }
 
 __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
@@ -204,7 +229,7 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
   const int64_t block = (t.state0 + i) / kStateBlock;
   const u32x2 mc = *reinterpret_cast<const u32x2*>(mp);
   const u32x2 vc = *reinterpret_cast<const u32x2*>(vp);
-  const double sm = (double)a.scale_m[block] * (1.0 / 512.0), sv = (double)a.scale_v[block];
+  const double sm = (double)a.scale_m[block] * (kMUnit / 512.0), sv = (double)a.scale_v[block] * kRUnit;
   float p[8], g[8];
   get_typed(t.g, t.g_type, i, t.n, t.g_vec, g);
   get_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
@@ -213,32 +238,37 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const double gq = (double)(g[q] * a.grad_scale);
-    const double m0 = m_value((mc[q >> 2] >> (8 * (q & 3))) & 255u, sm);
-    const double r0 = r_value((vc[q >> 2] >> (8 * (q & 3))) & 255u, sv);
-    const double v = fma(a.b2, r0 * r0, a.omb2 * gq * gq);
-    m[q] = i + q < t.n ? fma(a.b1, m0, a.omb1 * gq) : 0.0;
-    r[q] = i + q < t.n ? sqrt(v) : 0.0;
-    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 / ((float)(r[q] * root) + eps);
-    const double am = fabs(m[q]);
-    if (am > top_m && am < __builtin_inf()) top_m = am;
-    if (r[q] > top_r && r[q] < __builtin_inf()) top_r = r[q];
+    const unsigned cm = (mc[q >> 2] >> (8 * (q & 3))) & 255u, cv = (vc[q >> 2] >> (8 * (q & 3))) & 255u;
+    float fm = __uint_as_float(__float_as_uint(code_float<3>(cm & 127u)) | ((cm & 128u) << 24));
+    fm = (cm & 127u) == 127u ? __builtin_nanf("") : fm;
+    const float fr = cv == 255u ? __builtin_nanf("") : code_float<4>(cv);
+    const double r0 = (double)fr * sv;
+    m[q] = fma(a.b1, (double)fm * sm, a.omb1 * gq);
+    const double v = fma(a.b2, r0 * r0, a.omb2 * (gq * gq));
+    r[q] = root_of(v > kTiny ? v : v + kTiny);   // (NaN stays)
+    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 * __builtin_amdgcn_rcpf((float)(r[q] * root) + eps);
+    if (i + q >= t.n) {
+      m[q] = 0.0;
+      r[q] = 0.0;
+    }
+    top_m = fmax(top_m, finite_size(m[q]));
+    top_r = fmax(top_r, finite_size(r[q]));
   }
   put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
-  const float new_sm = (float)(half_wave_max(top_m) / 448.0);
-  const float new_sv = (float)(half_wave_max(top_r) / 491520.0);
+  const float new_sm = (float)(half_wave_max(top_m) * (1.0 / 448.0));
+  const float new_sv = (float)(half_wave_max(top_r) * (1.0 / 491520.0));
   const double im = new_sm > 0.0f ? 512.0 / (double)new_sm : 0.0;
   const double iv = new_sv > 0.0f ? 1.0 / (double)new_sv : 0.0;
   u32x2 mo = {0u, 0u}, vo = {0u, 0u};
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const double am = fabs(m[q]);
-    unsigned cm = am < __builtin_inf() ? nearest_code<3>(am * im, 126u) : 127u;
+    unsigned cm = nearest_code<3>(am * im, 126u);
+    cm = am < __builtin_inf() ? cm : 127u;
     cm |= m[q] < 0.0 ? 128u : 0u;
-    unsigned cv = 255u;
-    if (r[q] < __builtin_inf()) {
-      cv = nearest_code<4>(r[q] * iv, 254u);
-      if (cv == 0u && r[q] * iv > 0.0) cv = 1u;
-    }
+    unsigned cv = nearest_code<4>(r[q] * iv, 254u);
+    cv = cv == 0u && r[q] > kSeen && new_sv > 0.0f ? 1u : cv;
+    cv = r[q] < __builtin_inf() ? cv : 255u;
     mo[q >> 2] |= cm << (8 * (q & 3));
     vo[q >> 2] |= cv << (8 * (q & 3));
   }
@@ -263,9 +293,9 @@ __global__ __launch_bounds__(256) void k_adamw_values(const unsigned char* mc, c
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const unsigned c = (cm >> (8 * q)) & 255u, d = (cv >> (8 * q)) & 255u;
-    const float x = (float)code_value<3>(c & 127u) * (1.0f / 512.0f) * sm;
+    const float x = (float)((double)code_float<3>(c & 127u) * (kMUnit / 512.0)) * sm;
     om[q] = (c & 127u) == 127u ? __builtin_nanf("") : (c & 128u) ? -x : x;
-    const float y = (float)code_value<4>(d) * sv;
+    const float y = (float)((double)code_float<4>(d) * kRUnit) * sv;
     ov[q] = d == 255u ? __builtin_nanf("") : y * y;
   }
   *reinterpret_cast<f32x4*>(m + i) = om;

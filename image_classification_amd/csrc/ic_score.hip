@@ -160,20 +160,20 @@ struct RowView {
   __device__ __forceinline__ int granules() const {
     return (v + head + Elem<T>::kVec - 1) / Elem<T>::kVec;
   }
-  // x[i] = element g * kVec + i - head of the row, -inf outside it
-  __device__ __forceinline__ void get(int g, float* x) const {
+  // elements g * kVec - head .. of the row, -inf outside it
+  __device__ __forceinline__ u32x4 get_raw(int g) const {
     constexpr int kV = Elem<T>::kVec;
     const int j0 = g * kV - head;
-    if (j0 >= 0 && j0 + kV <= v) {
-      Elem<T>::unpack(*reinterpret_cast<const u32x4*>(base + (size_t)g * 16), x);
-    } else {
+    if (j0 >= 0 && j0 + kV <= v) return *reinterpret_cast<const u32x4*>(base + (size_t)g * 16);
+    float x[kV];
 #pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        const int j = j0 + i;
-        x[i] = (j >= 0 && j < v) ? Elem<T>::load(row + j) : -__builtin_inff();
-      }
+    for (int i = 0; i < kV; ++i) {
+      const int j = j0 + i;
+      x[i] = (j >= 0 && j < v) ? Elem<T>::load(row + j) : -__builtin_inff();
     }
+    return Elem<T>::pack(x);
   }
+  __device__ __forceinline__ void get(int g, float* x) const { Elem<T>::unpack(get_raw(g), x); }
 };
 
 struct ScoreArgs {
@@ -225,6 +225,31 @@ __device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const
   }
 }
 
+// 16-bit scores of a row of at most kPackedMost columns rank as one 32-bit word: the monotone 16 bits
+// of the score above, 65535 - index below.  All words differ, so ranking is minima and maxima of words,
+// ties included, and an element behind the row (-inf, a larger index) never comes before one of the
+// row.  NaN does not rank this way: rows that hold one take the general path.
+constexpr int kPackedMost = 65520;
+template <typename T>
+__device__ __forceinline__ unsigned rank16x2(unsigned w) {   // two scores, -0 as +0
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const s16x2 v = __builtin_bit_cast(s16x2, w);
+  const s16x2 sign = v >> (short)15;
+  const s16x2 mag = v & (short)0x7fff;
+  const s16x2 k = ((mag ^ sign) - sign) ^ (short)0x8000;
+  return __builtin_bit_cast(unsigned, k);
+}
+template <typename T> __device__ __forceinline__ float value16(unsigned key16);
+template <> __device__ __forceinline__ float value16<bf16_t>(unsigned k) {
+  const unsigned b = (k & 0x8000u) ? k ^ 0x8000u : 0x8000u | (0x8000u - k);
+  return __uint_as_float(b << 16);
+}
+template <> __device__ __forceinline__ float value16<f16_t>(unsigned k) {
+  const unsigned b = (k & 0x8000u) ? k ^ 0x8000u : 0x8000u | (0x8000u - k);
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)b);
+}
+template <> __device__ __forceinline__ float value16<float>(unsigned) { return 0.0f; }
+
 // Rows of up to 64 * NC granules: one wave a row, the row stays in registers between the maximum,
 // the sums and the ranking.
 template <typename T, int NC, bool TOP>
@@ -236,55 +261,109 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
   const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
   const RowView<T> rv(xr, a.v);
   const float c = a.inv_t * kLog2e;
-  float x[NC][kV];
+  u32x4 raw[NC];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) rv.get(i * 64 + lane, x[i]);
+  for (int i = 0; i < NC; ++i) raw[i] = rv.get_raw(i * 64 + lane);
   float m = kLowest;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
+  for (int i = 0; i < NC; ++i) {
+    float x[kV];
+    Elem<T>::unpack(raw[i], x);
 #pragma unroll
-    for (int j = 0; j < kV; ++j) m = fmaxf(m, x[i][j]);
+    for (int j = 0; j < kV; ++j) m = fmaxf(m, x[j]);
+  }
   Stats st;
   st.m = wave_max_f32(m);
   st.s = 0.0f;
   st.u = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
+  for (int i = 0; i < NC; ++i) {
+    float x[kV];
+    Elem<T>::unpack(raw[i], x);
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
-      const float d = x[i][j] - st.m;
+      const float d = x[j] - st.m;
       const float e = __builtin_amdgcn_exp2f(d * c);
       st.s += e;
       st.u = fmaf(e, fmaxf(d, kFar), st.u);
     }
+  }
   st.s = wave_sum_f32(st.s);
   st.u = wave_sum_f32(st.u);
   unsigned rk = 0;
   int ri = -1;
   if (TOP) {
-    auto index_at = [&](int i, int j) { return (i * 64 + lane) * kV + j - rv.head; };
-    auto inside = [&](int idx) { return idx >= 0 && idx < a.v; };
-    Best2 b = {0u, 0u, -1, -1};
+    if (sizeof(T) == 2 && a.v <= kPackedMost && st.s == st.s) {
+      // word (i, w, h): element 2 w + h of granule i.  `floor_`: only words below it count.
+      auto best2 = [&](unsigned floor_, unsigned* k1, unsigned* k2) {
+        unsigned b1 = 0, b2 = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+        for (int i = 0; i < NC; ++i) {
+          const int low = 65535 - ((i * 64 + lane) * kV - rv.head);
 #pragma unroll
-      for (int j = 0; j < kV; ++j) {
-        const int idx = index_at(i, j);
-        keep(b, inside(idx) ? rank_of(x[i][j]) : 0u, idx);
-      }
-    take_best(b, a.top, lane, &rk, &ri, [&](int, unsigned k0, int i0, unsigned* nk, int* ni) {
-      Best2 q = {0u, 0u, -1, -1};
+          for (int w = 0; w < 4; ++w) {
+            const unsigned pair = rank16x2<T>(raw[i][w]);
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int j = 0; j < kV; ++j) {
-          const int idx = index_at(i, j);
-          const unsigned k = inside(idx) ? rank_of(x[i][j]) : 0u;
-          if (after(k, idx, k0, i0)) keep(q, k, idx);
+            for (int h = 0; h < 2; ++h) {
+              const unsigned at = (unsigned)(low - 2 * w - h);
+              unsigned k = h ? (pair & 0xffff0000u) | (at & 0xffffu) : (pair << 16) | (at & 0xffffu);
+              // (elements before the row lie in granule 0)
+              if (i == 0) k = at > 65535u ? 0u : k;
+              k = k < floor_ ? k : 0u;
+              const unsigned lesser = b1 < k ? b1 : k;
+              b1 = b1 > k ? b1 : k;
+              b2 = b2 > lesser ? b2 : lesser;
+            }
+          }
         }
-      *nk = q.k1;
-      *ni = q.i1;
-    });
+        *k1 = b1;
+        *k2 = b2;
+      };
+      unsigned k1, k2;
+      best2(0xffffffffu, &k1, &k2);
+      unsigned mine = 0;
+      for (int r = 0; r < a.top; ++r) {
+        const unsigned kb = wave_max_u32(k1);
+        mine = lane == r ? kb : mine;
+        const bool won = k1 == kb;
+        // a lane that gives away its second looks for its next two
+        const bool spent = won && k2 == 0u;
+        k1 = won ? k2 : k1;
+        k2 = won ? 0u : k2;
+        if (r + 1 < a.top && __ballot(spent)) {
+          unsigned n1, n2;
+          best2(kb, &n1, &n2);
+          k1 = spent ? n1 : k1;
+          k2 = spent ? n2 : k2;
+        }
+      }
+      ri = 65535 - (int)(mine & 0xffffu);
+      rk = rank_of(value16<T>(mine >> 16));
+    } else {
+      auto index_at = [&](int i, int j) { return (i * 64 + lane) * kV + j - rv.head; };
+      auto inside = [&](int idx) { return idx >= 0 && idx < a.v; };
+      auto best2 = [&](unsigned k0, int i0, bool all) {
+        Best2 q = {0u, 0u, -1, -1};
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          float x[kV];
+          Elem<T>::unpack(raw[i], x);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const int idx = index_at(i, j);
+            const unsigned k = inside(idx) ? rank_of(x[j]) : 0u;
+            if (all || after(k, idx, k0, i0)) keep(q, k, idx);
+          }
+        }
+        return q;
+      };
+      take_best(best2(0u, 0, true), a.top, lane, &rk, &ri,
+                [&](int, unsigned k0, int i0, unsigned* nk, int* ni) {
+                  const Best2 q = best2(k0, i0, false);
+                  *nk = q.k1;
+                  *ni = q.i1;
+                });
+    }
   }
   write_row<T>(a, row, xr, st, lane, rk, ri);
 }
