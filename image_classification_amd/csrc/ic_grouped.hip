@@ -364,20 +364,47 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)(((uint64_t)high << 32) | low);
 }
 
-// The last e in [0, groups] whose first tile, at(e) / bm + e, is <= tile.  Every lane of the wave
-// takes part and gets the answer.
-__device__ __forceinline__ int64_t find_group(const Groups& g, int64_t tile, int64_t bm, int lane) {
-  int64_t lo = 0, hi = g.groups + 1;
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) >> 6;
-    const int64_t e = lo + lane * step;
-    const bool yes = e < hi && g.at(e) / bm + e <= tile;
-    int c = __popcll(__ballot(yes));
-    c = c > 1 ? c - 1 : 0;
-    lo += c * step;
+// The last group e in [0, groups] whose first tile, at(e) / bm + e, is <= tile, and where its rows begin
+// and end.  The 64 lanes of a wave look at 64 groups at a time, so that 63 groups take one round of
+// loads and 10 000 take three; the last round's loads already hold the group's begin and end.
+// (Four groups a lane are a round fewer and were slower: 40 groups apart, each lane's load is a cache
+// line of its own.)
+struct Found {
+  int64_t e, o0, o1;
+};
+__device__ __forceinline__ Found find_group(const Groups& g, int64_t tile64, int64_t bm64, int lane) {
+  // (rows, groups and tiles all fit 32 bits)
+  const unsigned tile = (unsigned)tile64, bm = (unsigned)bm64, groups = (unsigned)g.groups;
+  unsigned lo = 0, hi = groups + 1;
+  for (;;) {
+    const unsigned step = (hi - lo + 62u) / 63u;
+    const unsigned e = lo + (unsigned)lane * step;
+    const unsigned at = (unsigned)g.at(e < groups + 1 ? e : groups + 1);
+    const int count = __popcll(__ballot(e < hi && at / bm + e <= tile));
+    const int last = __builtin_amdgcn_readfirstlane(count > 0 ? count - 1 : 0);
+    if (step == 1)
+      return Found{(int64_t)(lo + (unsigned)last), (int64_t)(unsigned)__builtin_amdgcn_readlane((int)at, last),
+                   (int64_t)(unsigned)__builtin_amdgcn_readlane((int)at, last + 1)};
+    lo += (unsigned)last * step;
     hi = lo + step < hi ? lo + step : hi;
   }
-  return uniform(lo);
+}
+// The same for a whole workgroup: its first wave looks (the others' loads of the same lines were a
+// quarter of all loads where tiles are small), `box` [3] in LDS hands the answer on.
+__device__ __forceinline__ Found find_group_once(const Groups& g, int64_t tile, int64_t bm, int wave, int lane,
+                                                 unsigned* box) {
+  if (wave == 0) {
+    const Found f = find_group(g, tile, bm, lane);
+    if (lane == 0) {
+      box[0] = (unsigned)f.e;
+      box[1] = (unsigned)f.o0;
+      box[2] = (unsigned)f.o1;
+    }
+  }
+  __syncthreads();
+  return Found{(int64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)box[0]),
+               (int64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)box[1]),
+               (int64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)box[2])};
 }
 
 // Workgroup numbers are dealt to the 8 XCDs in turn; this gives each XCD a run of neighbours, whose
@@ -410,6 +437,9 @@ __device__ __forceinline__ void lds_load4(const void* src, char* lds_wave_base) 
                : "memory", "m0");
 }
 __device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// all but this wave's last COUNT loads
+template <int COUNT>
+__device__ __forceinline__ void all_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
 
 // Products of one granule of each operand (16 x 16 results).  float32 granules hold 4 elements, one
 // product of depth 4 each (kParts): lane group g of element j stands for k = 4 g + j in both operands,
@@ -441,26 +471,39 @@ template <> struct Mma<f16_t> {
 };
 
 // Which columns the lanes of a fragment stand for.  A product of fragment j of the Q side leaves a lane
-// with results 4 (lane >> 4) .. + 3 of its 16; taking column
-//     spread(i, j) = 16 (i >> 2) + 4 j + (i & 3)
-// as result i of fragment j (j = 0 .. 3) makes that 16 neighbouring columns a lane over the four
-// fragments, and 64 neighbouring columns a row: whole cache lines are stored.
-//
-// Tile "along": [rows][128 bytes], granule s of row r holds granule s ^ swap(r) of the stage.  P is
-// read 16 neighbouring rows at a time, Q in the rows spread(0 .. 15, j); 8 lanes of a read reach 8
-// different places of the 256 bytes of the banks in either.
+// with results 4 g .. 4 g + 3 of its 16, g = lane >> 4.  float32: result i of fragment j is column
+// 16 j + i, so that the four lanes of a row store 64 neighbouring bytes an instruction.  16-bit types:
+// column 8 (i >> 2) + 4 (j & 1) + (i & 3) + 32 (j >> 1), so that fragments 2 h and 2 h + 1 leave a lane with 8
+// neighbouring columns and the four lanes store 64 neighbouring bytes as well.  (With 16 neighbouring
+// columns a lane, whole lines of a row in four instructions of 16 bytes at a stride of 64, the stores
+// of 1M x 64 float32 took 78 us of their own.)
+template <typename T>
+__device__ __forceinline__ constexpr int spread_row(int i) {   // of result i in fragment 0
+  return sizeof(T) == 4 ? i : (i >> 2) * 8 + (i & 3);
+}
+template <typename T>
+__device__ __forceinline__ constexpr int spread_step(int j) {  // from fragment 0 to fragment j
+  return sizeof(T) == 4 ? j * 16 : (j & 1) * 4 + (j >> 1) * 32;
+}
+
+// Tile "along": [rows][128 bytes], granule s of row r holds granule s ^ swap(r) of the stage; 8 lanes
+// of a read reach 8 different places of the 256 bytes of the banks.
 __device__ __forceinline__ int along_swap_p(int r) { return r & 7; }
-__device__ __forceinline__ int along_swap_q(int r) { return ((r >> 3) & 6) | ((r >> 1) & 1); }
-// A lane's place of fragment 0, step 0 (bytes behind the operand's tile).  Fragment i of P lies 16
-// rows further, fragment j of Q 4 rows; step 1 exchanges the halves of a row (the swaps and the quarter
+template <typename T>
+__device__ __forceinline__ int along_swap_q(int r) {
+  return sizeof(T) == 4 ? r & 7 : ((r >> 2) & 6) | ((r >> 1) & 1);
+}
+// A lane's place of fragment 0, step 0 (bytes behind the operand's tile).  Fragment i of P lies 16 i
+// rows further, fragment j of Q spread_step(j) rows; step 1 exchanges the halves of a row (the swaps and the quarter
 // wave's granule share no bit with it).
 __device__ __forceinline__ int along_place_p(int r0, int lane) {
   const int r = r0 + (lane & 15);
   return r * kStageBytes + ((lane >> 4) ^ along_swap_p(r)) * 16;
 }
+template <typename T>
 __device__ __forceinline__ int along_place_q(int r0, int lane) {
-  const int r = r0 + ((lane & 12) << 2) + (lane & 3);
-  return r * kStageBytes + ((lane >> 4) ^ along_swap_q(r)) * 16;
+  const int r = r0 + spread_row<T>(lane & 15);
+  return r * kStageBytes + ((lane >> 4) ^ along_swap_q<T>(r)) * 16;
 }
 
 // Tile "across": [kK rows of the contraction][COLS], granules exchanged by the contraction row k.  In
@@ -474,20 +517,20 @@ __device__ __forceinline__ int across_swap_p(int k) {
 }
 template <typename T, int COLS>
 __device__ __forceinline__ int across_swap_q(int k) {
-  if (sizeof(T) == 4) return (k >> 2) & 3;
-  return COLS >= 128 ? (k & 1) | ((k & 2) << 2) : k & 1;
+  if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+  return COLS >= 128 ? (k & 3) << 2 : (k & 1) << 2;
 }
 // A lane's place of fragment 0, step 0: the column whose 8 bytes (16-bit types) or 4 bytes (float32) it
 // points at, in its row of the contraction.  The fragments' columns and the swaps only set bits that
 // are clear in the wave's first column, so fragment i of P lies at place ^ 16 i columns and fragment j
-// of Q at place ^ 4 j columns; a step is kK / 2 rows.
+// of Q at place ^ spread_step(j) columns; a step is kK / 2 rows.
 template <typename T, int COLS, bool Q>
 __device__ __forceinline__ int across_place(int c0, int lane) {
   constexpr int kRow = COLS * (int)sizeof(T), kV = 16 / (int)sizeof(T);
   const int k = sizeof(T) == 2 ? (lane >> 4) * 8 + ((lane & 15) >> 2) : (lane >> 4) * 4;
   int c;
-  if (sizeof(T) == 2) c = (lane & 3) * (Q ? 16 : 4);
-  else c = Q ? ((lane & 12) << 2) + (lane & 3) : lane & 15;
+  if (sizeof(T) == 2) c = (lane & 3) * (Q ? 8 : 4);
+  else c = lane & 15;
   c += c0;
   const int swap = Q ? across_swap_q<T, COLS>(k) : across_swap_p<T, COLS>(k);
   return k * kRow + ((c / kV) ^ swap) * 16 + c % kV * (int)sizeof(T);
@@ -524,12 +567,13 @@ __device__ __forceinline__ void read_fragments(const char* tile, int place, int 
     const char* p = tile + (place ^ (step * 64));
 #pragma unroll
     for (int i = 0; i < COUNT; ++i)
-      out[i] = *reinterpret_cast<const u32x4*>(p + (first + i) * (Q ? 4 : 16) * kStageBytes);
+      out[i] = *reinterpret_cast<const u32x4*>(p + (Q ? spread_step<T>(first + i) : (first + i) * 16) * kStageBytes);
   } else {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i)
       out[i] = read_across<T, COLS>(tile + step * (Mma<T>::kK / 2 * COLS * (int)sizeof(T)) +
-                                    (place ^ ((first + i) * (Q ? 4 : 16) * (int)sizeof(T))));
+                                    (place ^ ((Q ? spread_step<T>(first + i) : (first + i) * 16) *
+                                              (int)sizeof(T))));
   }
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -583,11 +627,13 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       __syncthreads();                                                               \
     }                                                                                \
     _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0, smem);             \
-    all_landed();                                                                    \
-    __syncthreads();                                                                 \
     if (STAGES > 1) {                                                                \
       _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1, smem + kStage);  \
+      all_but<kLoads>();                                                             \
+    } else {                                                                         \
+      all_landed();                                                                  \
     }                                                                                \
+    __syncthreads();                                                                 \
     if (PREPARES) NEXT(2);                                                           \
     read_q(smem, 0, 0);                                                              \
     read_p(smem, 0, 0, 0);                                                           \
@@ -638,35 +684,39 @@ struct RowsArgs {
   int y_f32, y_vec;    // y_vec: four columns can be stored at once
 };
 
-// Sixteen neighbouring results of one row, v[j] the j-th four of them; `left` columns are left.
-// vec: 16 bytes can be stored at once.
+// A lane's sixteen results of one row, v[j] those of fragment j, in the 64 columns from c on; the row
+// begins at `at` and has `cols` columns.  vec: 16 bytes can be stored at once.
 template <typename T>
-__device__ __forceinline__ void store16(void* y, int64_t at, int left, bool f32, bool vec, const f32x4* v) {
-  if (left <= 0) return;
-  if (f32 || sizeof(T) == 4) {
+__device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, int lane, bool f32, bool vec,
+                                        const f32x4* v) {
+  if (sizeof(T) == 4 || f32) {
     float* d = static_cast<float*>(y) + at;
-    if (vec && left >= 16) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(d + 4 * j) = v[j];
-    } else {
+    for (int j = 0; j < 4; ++j) {
+      const int cj = c + spread_row<T>((lane >> 4) * 4) + spread_step<T>(j);
+      if (vec && cj + 4 <= cols) {
+        *reinterpret_cast<f32x4*>(d + cj) = v[j];
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) d[i] = v[i >> 2][i & 3];
+        for (int i = 0; i < 4; ++i)
+          if (cj + i < cols) d[cj + i] = v[j][i];
+      }
     }
   } else if constexpr (sizeof(T) == 2) {
     T* d = static_cast<T*>(y) + at;
-    if (vec && left >= 16) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float f[8];
+    for (int h = 0; h < 2; ++h) {
+      const int cj = c + spread_row<T>((lane >> 4) * 4) + spread_step<T>(2 * h);
+      float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = v[2 * h + (i >> 2)][i & 3];
-        *reinterpret_cast<u32x4*>(d + 8 * h) = Elem<T>::pack(f);
+      for (int i = 0; i < 8; ++i) f[i] = v[2 * h + (i >> 2)][i & 3];
+      if (vec && cj + 8 <= cols) {
+        *reinterpret_cast<u32x4*>(d + cj) = Elem<T>::pack(f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (cj + i < cols) Elem<T>::store(d + cj + i, f[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) Elem<T>::store(d + i, v[i >> 2][i & 3]);
     }
   }
 }
@@ -676,7 +726,7 @@ template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  static_assert(FN == 4, "a lane's sixteen columns");
+  static_assert(FN == 4, "64 columns a wave");
   constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
   constexpr int kPBytes = BM * kStageBytes, kQBytes = BN * kStageBytes;
   constexpr int kPLoads = BM * 8 / kThreads, kQLoads = BN * 8 / kThreads;
@@ -684,27 +734,24 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   static_assert(kPLoads * kThreads == BM * 8 && kQLoads * kThreads == BN * 8, "tile");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int* rows = reinterpret_cast<int*>(smem + 2 * (kPBytes + kQBytes));
+  __shared__ unsigned box[3];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = xcd_run(blockIdx.x, gridDim.x);
   const int64_t tile = id / a.col_tiles;
   const int c0 = (int)(id % a.col_tiles) * BN;
-  const int64_t e = find_group(a.g, tile, BM, lane);
-  const int64_t o0 = uniform(a.g.at(e)), o1 = uniform(a.g.at(e + 1));
+  const Found f = find_group_once(a.g, tile, BM, wave, lane, box);
+  const int64_t e = f.e, o0 = f.o0, o1 = f.o1;
   const int64_t t = tile - (o0 / BM + e);
   const int64_t r0 = o0 + t * BM;
   if (t < 0 || r0 >= o1) return;   // (t < 0: only if the offsets do not ascend)
   const int m = o1 - r0 < BM ? (int)(o1 - r0) : BM;
-  // the rows' numbers; -1 behind the group's end and for an entry of `order` that is no row
-  for (int i = threadIdx.x; i < BM; i += kThreads) {
-    int64_t r = -1;
-    if (i < m) {
-      r = a.order ? (int64_t)a.order[r0 + i] : r0 + i;
-      if (r < 0 || r >= a.g.n) r = -1;
-    }
-    rows[i] = (int)r;
-  }
-  __syncthreads();
+  // the number of a row of the tile; -1 behind the group's end and for an entry of `order` that is no row
+  auto row_at = [&](int i) {
+    if (i >= m) return (int64_t)-1;
+    const int64_t r = a.order ? (int64_t)a.order[r0 + i] : r0 + i;
+    return r >= 0 && r < a.g.n ? r : (int64_t)-1;
+  };
   const int wm = wave % WM, wn = wave / WM;
   const int pr = wm * (BM / WM), qc = wn * (BN / WN);
   f32x4 acc[FM][FN];
@@ -712,6 +759,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // (for the end; read behind the barriers of the stages)
+  for (int i = threadIdx.x; i < BM; i += kThreads) rows[i] = (int)row_at(i);
 
   if (e < a.g.groups) {
     const T* qb = static_cast<const T*>(a.q) + e * a.q_stride;
@@ -723,8 +772,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
     Off prow[kPLoads];
 #pragma unroll
     for (int i = 0; i < kPLoads; ++i) {
-      const int row = rows[((i * kWaves + wave) * 64 + lane) >> 3];
-      prow[i] = (Off)((int64_t)(row < 0 ? 0 : row) * (a.ld_p / kUnit));
+      const int64_t row = row_at(((i * kWaves + wave) * 64 + lane) >> 3);
+      prow[i] = (Off)((row < 0 ? 0 : row) * (a.ld_p / kUnit));
     }
     // granule i of this lane lies a fixed number of matrix rows behind granule 0
     const int lin = wave * 64 + lane;
@@ -745,7 +794,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
       if (QALONG) {
         const bool in = c0 + qfirst + i * kQStep < a.cols;
         fetch<T, ALIGNED>(in ? qrow + (int64_t)(i * kQStep) * a.ld_q : nullptr,
-                          k0 + ((lin & 7) ^ along_swap_q(qfirst + i * kQStep)) * kV, a.depth, to, lane);
+                          k0 + ((lin & 7) ^ along_swap_q<T>(qfirst + i * kQStep)) * kV, a.depth, to, lane);
       } else {
         const int k = qfirst + i * kQStep;
         const int c = c0 + ((lin % kQRow) ^ across_swap_q<T, BN>(k)) * kV;
@@ -757,7 +806,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
     constexpr int kHalves = FM >= 4 ? 2 : 1, kHalf = FM / kHalves;
     u32x4 pf[2][kHalf], qf[2][FN];
     const int pplace = along_place_p(pr, lane);
-    const int qplace = kPBytes + (QALONG ? along_place_q(qc, lane) : across_place<T, BN, true>(qc, lane));
+    const int qplace = kPBytes + (QALONG ? along_place_q<T>(qc, lane) : across_place<T, BN, true>(qc, lane));
     auto read_p = [&](const char* buf, int step, int half, int to) {
       if (busy) read_fragments<T, BM, true, false, kHalf>(buf, pplace, step, half * kHalf, pf[to]);
     };
@@ -786,14 +835,98 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
     };
     auto next = [](int) {};
     MULTIPLY_STAGES(stages, load, next, false)
+  } else {
+    __syncthreads();
   }
-  // lane: row pr + 16 i + (lane & 15), 16 columns from qc + 16 (lane >> 4)
-  const int c = c0 + qc + (lane >> 4) * 16;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int row = rows[pr + i * 16 + (lane & 15)];
-    if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y + c, a.cols - c, a.y_f32, a.y_vec, acc[i]);
+    if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y, c0 + qc, a.cols, lane, a.y_f32, a.y_vec, acc[i]);
   }
+}
+
+// Short rows (a contraction of at most NS stages, 512 bytes: the 128 float32 of a local descriptor), tiles
+// of 64 x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
+// goes to LDS, shared by the four waves; each wave's 16 rows go straight to the registers that the
+// products take them from.  One barrier, one memory latency behind the search for the group.
+// (1M rows x 128 float32, 10 000 groups of 64 x 128: staged like the longer ones 355 us.)
+// Five workgroups share a CU: 32 KB of LDS and 96 registers each.
+template <typename T, int NS, bool QALONG>
+__global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
+  constexpr int BN = 64, kWaves = 4, FN = 4;
+  constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
+  constexpr int kQRow = BN * (int)sizeof(T) / 16;
+  constexpr int kStage = BN * kStageBytes;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t tile = id / a.col_tiles;
+  const int c0 = (int)(id % a.col_tiles) * BN;
+  // (what still loads goes before what multiplies: 3 %)
+  __builtin_amdgcn_s_setprio(3);
+  const Found f = find_group_once(a.g, tile, 64, wave, lane, reinterpret_cast<unsigned*>(smem));
+  __syncthreads();   // (the box is read: its place may be filled)
+  const int64_t t = tile - (f.o0 / 64 + f.e);
+  const int64_t r0 = f.o0 + t * 64;
+  if (t < 0 || r0 >= f.o1) return;
+  // the last tile of a group leaves waves without rows: not the same ones in every tile
+  const int quarter = (wave + (int)tile) & 3;
+  const int64_t pos = r0 + quarter * 16 + (lane & 15);
+  int64_t row = -1;
+  if (pos < f.o1) {
+    row = a.order ? (int64_t)a.order[pos] : pos;
+    if (row < 0 || row >= a.g.n) row = -1;
+  }
+  f32x4 acc[FN];
+#pragma unroll
+  for (int j = 0; j < FN; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (f.e < a.g.groups) {
+    const bool busy = r0 + quarter * 16 < f.o1;
+    const T* p = static_cast<const T*>(a.p) + (row < 0 ? 0 : row) * a.ld_p + (lane >> 4) * kV;
+    u32x4 pf[2 * NS];
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        const int k = i * 4 * kV;
+        pf[i] = k + (lane >> 4) * kV < a.depth ? *reinterpret_cast<const u32x4*>(p + k) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    const T* qb = static_cast<const T*>(a.q) + f.e * a.q_stride;
+    const int lin = wave * 64 + lane;
+#pragma unroll
+    for (int st = 0; st < NS; ++st)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = i * 256 + lin;
+        char* to = smem + st * kStage + (i * kWaves + wave) * 1024;
+        if (QALONG) {
+          const int r = q >> 3;
+          fetch<T, true>(c0 + r < a.cols ? qb + (int64_t)(c0 + r) * a.ld_q : nullptr,
+                         st * kK + ((q & 7) ^ along_swap_q<T>(r)) * kV, a.depth, to, lane);
+        } else {
+          const int k = q / kQRow;
+          fetch<T, true>(st * kK + k < a.depth ? qb + (int64_t)(st * kK + k) * a.ld_q : nullptr,
+                         c0 + ((q % kQRow) ^ across_swap_q<T, BN>(k)) * kV, a.cols, to, lane);
+        }
+      }
+    const int qplace = QALONG ? along_place_q<T>(0, lane) : across_place<T, BN, true>(0, lane);
+    all_landed();
+    __syncthreads();
+    __builtin_amdgcn_s_setprio(0);
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        u32x4 qf[FN];
+        read_fragments<T, BN, QALONG, true, FN>(smem + i / 2 * kStage, qplace, i % 2, 0, qf);
+#pragma unroll
+        for (int part = 0; part < Mma<T>::kParts; ++part)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[j] = Mma<T>::mul(part, qf[j], pf[i], acc[j]);
+      }
+    }
+  }
+  if (row >= 0) store16<T>(a.y, row * a.ld_y, c0, a.cols, lane, a.y_f32, a.y_vec, acc);
 }
 
 // Few rows a group (single rows to serve): the matrices are the traffic, so a workgroup takes 16 rows
@@ -813,8 +946,9 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tile = (int64_t)blockIdx.x / a.col_tiles;
   const int c0 = (int)(blockIdx.x % a.col_tiles) * kCols + (BYDEPTH ? 0 : wave * 16);
-  const int64_t e = find_group(a.g, tile, 16, lane);
-  const int64_t o0 = uniform(a.g.at(e)), o1 = uniform(a.g.at(e + 1));
+  __shared__ unsigned box[3];
+  const Found f = find_group_once(a.g, tile, 16, wave, lane, box);
+  const int64_t e = f.e, o0 = f.o0, o1 = f.o1;
   const int64_t t = tile - (o0 / 16 + e);
   const int64_t r0 = o0 + t * 16;
   if (t < 0 || r0 >= o1) return;
@@ -918,10 +1052,10 @@ __device__ __forceinline__ int64_t dw_line(const DwArgs& a, int64_t kk) {
 }
 __device__ __forceinline__ DwPlace dw_place(const DwArgs& a, int64_t u, int64_t kk, int lane) {
   DwPlace p;
-  p.e = find_group(a.g, u / a.tiles, kk, lane);
-  if (p.e >= a.g.groups) p.e = a.g.groups - 1;   // (only if the offsets do not ascend)
-  p.o0 = uniform(a.g.at(p.e));
-  p.o1 = uniform(a.g.at(p.e + 1));
+  const Found f = find_group(a.g, u / a.tiles, kk, lane);
+  p.e = f.e < a.g.groups ? f.e : a.g.groups - 1;   // (it always is if the offsets ascend)
+  p.o0 = f.o0;
+  p.o1 = f.o1;
   if (p.o1 < p.o0) p.o1 = p.o0;
   p.stages = p.o1 / kk + 1 - p.o0 / kk;
   int64_t in = u - (p.o0 / kk + p.e) * a.tiles;
@@ -936,7 +1070,7 @@ template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  static_assert(FN == 4, "a lane's sixteen columns");
+  static_assert(FN == 4, "64 columns a wave");
   static_assert(BM == BN, "both operands' granules lie in the same rows");
   constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
   constexpr int kPBytes = BM * kStageBytes, kQBytes = BN * kStageBytes;
@@ -1030,11 +1164,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
     }
     const bool whole = pl.stage == 0 && run == pl.stages;
     if (whole) {
-      const int c = n0 + qc + (lane >> 4) * 16;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int o = m0 + pc + i * 16 + (lane & 15);
-        if (o < a.out) store16<T>(a.dw, (pl.e * a.out + o) * a.k + c, a.k - c, a.y_f32, a.y_vec, acc[i]);
+        if (o < a.out) store16<T>(a.dw, (pl.e * a.out + o) * a.k, n0 + qc, a.k, lane, a.y_f32, a.y_vec, acc[i]);
       }
     } else {
       // 16 bytes a lane, lanes side by side; the join undoes the order
@@ -1085,7 +1218,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
     const int t = at % kThreads, ij = at / kThreads;
     const int tl = t & 63, tw = t >> 6;
     const int o = pl.tile / a.k_tiles * BM + tw % WM * (BM / WM) + ij / FN * 16 + (tl & 15);
-    const int c = pl.tile % a.k_tiles * BN + tw / WM * (BN / WN) + (tl >> 4) * 16 + ij % FN * 4;
+    const int c = pl.tile % a.k_tiles * BN + tw / WM * (BN / WN) + spread_row<T>((tl >> 4) * 4) +
+                  spread_step<T>(ij % FN);
     if (o >= a.out) return;
     const int64_t to = (pl.e * a.out + o) * a.k + c;
     const int left = a.k - c;
@@ -1183,6 +1317,15 @@ int pick_tile(int type, F tiles) {
   return best;
 }
 
+template <typename T, int NS, bool QALONG>
+hipError_t short_launch(RowsArgs a, hipStream_t s) {
+  a.col_tiles = (a.cols + 63) / 64;
+  const int64_t grid = (a.g.n / 64 + a.g.groups + 1) * a.col_tiles;
+  if (grid * 256 > 0xffffffffll) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_grouped_short<T, NS, QALONG>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 // Up to 8 rows a group on average (or hardly any rows at all), forward.
 template <typename T>
 hipError_t few_launch(RowsArgs a, hipStream_t s) {
@@ -1199,6 +1342,13 @@ template <typename T, bool QALONG>
 hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) {
   if (!aligned) return rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
   if (QALONG && (a.g.n <= 8 * a.g.groups || a.g.n <= 32)) return few_launch<T>(a, s);
+  // rows of at most 512 bytes whose tiles would be 64 x 64 anyway (fewer columns, or short groups)
+  const int64_t row_bytes = (int64_t)a.depth * (int)sizeof(T);
+  if (row_bytes <= 512 && (a.cols <= 64 || a.g.n < 128 * a.g.groups)) {
+    if (row_bytes <= 128) return short_launch<T, 1, QALONG>(a, s);
+    if (row_bytes <= 256) return short_launch<T, 2, QALONG>(a, s);
+    return short_launch<T, 4, QALONG>(a, s);
+  }
   const int tile = pick_tile(type, [&](int size) {
     return (a.g.n / size + a.g.groups) * ((a.cols + size - 1) / size);
   });
