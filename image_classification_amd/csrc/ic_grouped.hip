@@ -429,6 +429,14 @@ __device__ __forceinline__ void lds_load16(const void* src, char* lds_wave_base)
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(to))
                : "memory", "m0");
 }
+// The same from a scalar base and 32-bit offsets: no vector instruction besides the load itself.
+__device__ __forceinline__ void lds_load16_at(const void* base, unsigned offset, char* lds_wave_base) {
+  const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds_wave_base;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to))
+               : "memory", "m0");
+}
 __device__ __forceinline__ void lds_load4(const void* src, char* lds_wave_base) {
   const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds_wave_base;
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
@@ -614,9 +622,9 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
 // The freed buffer is refilled with stage st + 2 one load per four products, during the last part of
 // st and the first of st + 1: issued in one go behind the barrier, the 8 waves' loads would hold up
 // the products behind them in every wave.
-// LOAD(i, stage, buffer) issues load i of kLoads; with PREPARES, NEXT(stage) fetches what the loads of
+// LOAD(i, stage, buffer) issues load i of kLoads (LOADS_EACH instructions); with PREPARES, NEXT(stage) fetches what the loads of
 // that stage need, and lands a barrier before them.
-#define MULTIPLY_STAGES(STAGES, LOAD, NEXT, PREPARES)                                          \
+#define MULTIPLY_STAGES(STAGES, LOAD, NEXT, PREPARES, LOADS_EACH)                                          \
   {                                                                                  \
     constexpr int kStage = kPBytes + kQBytes, kFirst = kLoads / 2;                   \
     auto none = [](int) {};                                                          \
@@ -629,7 +637,7 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
     _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0, smem);             \
     if (STAGES > 1) {                                                                \
       _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1, smem + kStage);  \
-      all_but<kLoads>();                                                             \
+      all_but<kLoads * LOADS_EACH>();                                                \
     } else {                                                                         \
       all_landed();                                                                  \
     }                                                                                \
@@ -764,41 +772,54 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 
   if (e < a.g.groups) {
     const T* qb = static_cast<const T*>(a.q) + e * a.q_stride;
-    // this lane's granules: the row and the first element inside the stage
-    // (its row's distance from the first row in units of kUnit elements, 32 bits; behind the
-    // group's end row 0 stands in: such rows are multiplied and not stored)
-    constexpr int kUnit = ALIGNED ? kV : 1;
-    typedef typename std::conditional<ALIGNED, unsigned, int64_t>::type Off;
-    Off prow[kPLoads];
+    // P: the rows of this lane's granules (behind the group's end row 0 stands in: such rows are
+    // multiplied and not stored)
+    const int lin = wave * 64 + lane;
+    const int along = ((lin & 7) ^ along_swap_p(lin >> 3)) * kV;   // (a step of i keeps the low bits)
+    const T* prow[kPLoads];
 #pragma unroll
     for (int i = 0; i < kPLoads; ++i) {
       const int64_t row = row_at(((i * kWaves + wave) * 64 + lane) >> 3);
-      prow[i] = (Off)((row < 0 ? 0 : row) * (a.ld_p / kUnit));
+      prow[i] = static_cast<const T*>(a.p) + (row < 0 ? 0 : row) * a.ld_p;
     }
-    // granule i of this lane lies a fixed number of matrix rows behind granule 0
-    const int lin = wave * 64 + lane;
+    // Q: granule i of this lane lies kQStep rows of the matrix behind granule 0.  Where the tile lies
+    // inside the matrix, a load is a scalar base and one of (at most) two offsets that a lane keeps.
     constexpr int kQStep = QALONG ? kThreads / 8 : kThreads / kQRow;
     const int qfirst = QALONG ? lin >> 3 : lin / kQRow;
-    const T* qrow = qb + (int64_t)(QALONG ? c0 + qfirst : qfirst) * a.ld_q;
-    const int along = ((lin & 7) ^ along_swap_p(lin >> 3)) * kV;   // (a step of i keeps the low bits)
+    auto qgranule = [&](int i) {
+      return QALONG ? (lin & 7) ^ along_swap_q<T>(qfirst + i * kQStep)
+                    : (lin % kQRow) ^ across_swap_q<T, BN>(qfirst + i * kQStep);
+    };
+    const unsigned qoff0 = (unsigned)(qfirst * a.ld_q + qgranule(0) * kV) * (unsigned)sizeof(T);
+    const unsigned qoff1 = (unsigned)(qfirst * a.ld_q + qgranule(1) * kV) * (unsigned)sizeof(T);
+    const bool inside = ALIGNED && c0 + BN <= a.cols;
+    const int full = a.depth / kK;     // stages that lie inside the depth
     constexpr int kLoads = kPLoads + kQLoads;
     auto load = [&](int i, int st, char* buf) {
       const int64_t k0 = (int64_t)st * kK;
       if (i < kPLoads) {
-        fetch<T, ALIGNED>(static_cast<const T*>(a.p) + (int64_t)prow[i] * kUnit, k0 + along, a.depth,
-                          buf + (i * kWaves + wave) * 1024, lane);
+        char* to = buf + (i * kWaves + wave) * 1024;
+        if (ALIGNED && st < full) lds_load16(prow[i] + along + k0, to);
+        else fetch<T, ALIGNED>(prow[i], k0 + along, a.depth, to, lane);
         return;
       }
       i -= kPLoads;
       char* to = buf + kPBytes + (i * kWaves + wave) * 1024;
       if (QALONG) {
-        const bool in = c0 + qfirst + i * kQStep < a.cols;
-        fetch<T, ALIGNED>(in ? qrow + (int64_t)(i * kQStep) * a.ld_q : nullptr,
-                          k0 + ((lin & 7) ^ along_swap_q<T>(qfirst + i * kQStep)) * kV, a.depth, to, lane);
+        if (inside && st < full) {
+          lds_load16_at(qb + (int64_t)(c0 + i * kQStep) * a.ld_q + k0, i % 2 ? qoff1 : qoff0, to);
+        } else {
+          const int c = c0 + qfirst + i * kQStep;
+          fetch<T, ALIGNED>(c < a.cols ? qb + (int64_t)c * a.ld_q : nullptr, k0 + qgranule(i) * kV, a.depth, to,
+                            lane);
+        }
       } else {
-        const int k = qfirst + i * kQStep;
-        const int c = c0 + ((lin % kQRow) ^ across_swap_q<T, BN>(k)) * kV;
-        fetch<T, ALIGNED>(k0 + k < a.depth ? qrow + (k0 + i * kQStep) * a.ld_q : nullptr, c, a.cols, to, lane);
+        if (inside && st < full) {
+          lds_load16_at(qb + (k0 + i * kQStep) * a.ld_q + c0, i % 2 ? qoff1 : qoff0, to);
+        } else {
+          const int64_t k = k0 + qfirst + i * kQStep;
+          fetch<T, ALIGNED>(k < a.depth ? qb + k * a.ld_q : nullptr, c0 + qgranule(i) * kV, a.cols, to, lane);
+        }
       }
     };
     const int stages = (int)(((int64_t)a.depth + kK - 1) / kK);
@@ -834,7 +855,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     };
     auto next = [](int) {};
-    MULTIPLY_STAGES(stages, load, next, false)
+    MULTIPLY_STAGES(stages, load, next, false, 1)
   } else {
     __syncthreads();
   }
@@ -1106,31 +1127,51 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       // The rows of a stage: `order` goes to LDS, one wave's load a stage, two stages ahead of the
       // loads that need it (without an order the positions are the rows).
       const int64_t stages = (r1 - r0 + kK - 1) / kK;
+      // this lane's first granule of either operand, and its row stride, in bytes
+      constexpr bool kFixed = ALIGNED && kThreads / kPRow % 16 == 0;
+      const int lin = wave * 64 + lane;
+      const int cd0 = m0 + ((lin % kPRow) ^ across_swap_p<T, BM>(lin / kPRow)) * kV;
+      const int cx0 = n0 + ((lin % kPRow) ^ across_swap_q<T, BN>(lin / kPRow)) * kV;
+      const char* zero = reinterpret_cast<const char*>(kZeroGranule);
+      const char* dy0 = cd0 < a.out ? reinterpret_cast<const char*>(static_cast<const T*>(a.dy) + cd0) : zero;
+      const char* x0 = cx0 < a.k ? reinterpret_cast<const char*>(static_cast<const T*>(a.x) + cx0) : zero;
+      const unsigned dy_ld = cd0 < a.out ? (unsigned)(a.ld_dy * (int64_t)sizeof(T)) : 0u;
+      const unsigned x_ld = cx0 < a.k ? (unsigned)(a.ld_x * (int64_t)sizeof(T)) : 0u;
       auto look = [&](int64_t st) {
         if (!a.order || wave != 0 || st >= stages) return;
         int64_t pos = r0 + st * kK + (lane < kK ? lane : kK - 1);
         if (pos >= a.g.n) pos = a.g.n - 1;
         lds_load4(a.order + pos, reinterpret_cast<char*>(ids + (st & 1) * 64));
       };
-      constexpr int kLoads = 2 * kPLoads;   // dy's and x's granules of a row in turn
+      // load i: dy's and x's granules of one row
+      constexpr int kLoads = kPLoads;
       auto load = [&](int i, int64_t st, char* buf) {
-        const int q0 = (i / 2 * kWaves + wave) * 64;
+        const int q0 = (i * kWaves + wave) * 64;
+        const int64_t first = r0 + st * kK;
+        if (kFixed && first + kK <= r1) {
+          // (the columns are the same for every i, and behind the matrix a lane's pointer is that of
+          // the zeros, its row stride 0)
+          int k = lin / kPRow + i * (kThreads / kPRow);
+          unsigned r = (unsigned)first + (unsigned)k;
+          if (a.order) r = (unsigned)ids[(st & 1) * 64 + k];
+          const bool in = r < (unsigned)a.g.n;
+          const char* d = dy0 + (uint64_t)r * dy_ld;
+          const char* x = x0 + (uint64_t)r * x_ld;
+          lds_load16(in ? d : reinterpret_cast<const char*>(kZeroGranule), buf + q0 * 16);
+          lds_load16(in ? x : reinterpret_cast<const char*>(kZeroGranule), buf + kPBytes + q0 * 16);
+          return;
+        }
         int q = q0 + lane;
         asm volatile("" : "+v"(q));   // (worked out at each load: there are no registers to keep it in)
         const int k = q / kPRow, s = q % kPRow;
-        const int64_t first = r0 + st * kK;
         int r = (int)first + k;
         if (a.order) r = ids[(st & 1) * 64 + k];
         const bool in = k < r1 - first && (unsigned)r < (unsigned)a.g.n;
-        if (i % 2 == 0) {
-          const int c = m0 + (s ^ across_swap_p<T, BM>(k)) * kV;
-          const T* row = static_cast<const T*>(a.dy) + (int64_t)r * a.ld_dy;
-          fetch<T, ALIGNED>(in ? row : nullptr, c, a.out, buf + q0 * 16, lane);
-        } else {
-          const int c = n0 + (s ^ across_swap_q<T, BN>(k)) * kV;
-          const T* row = static_cast<const T*>(a.x) + (int64_t)r * a.ld_x;
-          fetch<T, ALIGNED>(in ? row : nullptr, c, a.k, buf + kPBytes + q0 * 16, lane);
-        }
+        const int cd = m0 + (s ^ across_swap_p<T, BM>(k)) * kV, cx = n0 + (s ^ across_swap_q<T, BN>(k)) * kV;
+        const T* rd = static_cast<const T*>(a.dy) + (int64_t)r * a.ld_dy;
+        const T* rx = static_cast<const T*>(a.x) + (int64_t)r * a.ld_x;
+        fetch<T, ALIGNED>(in ? rd : nullptr, cd, a.out, buf + q0 * 16, lane);
+        fetch<T, ALIGNED>(in ? rx : nullptr, cx, a.k, buf + kPBytes + q0 * 16, lane);
       };
       constexpr int kHalves = FM >= 4 ? 2 : 1, kHalf = FM / kHalves;
       u32x4 pf[2][kHalf], qf[2][FN];
@@ -1159,7 +1200,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      MULTIPLY_STAGES(stages, load, look, true)
+      MULTIPLY_STAGES(stages, load, look, true, 2)
       __syncthreads();   // the buffers are free for the next run's loads
     }
     const bool whole = pl.stage == 0 && run == pl.stages;
@@ -1297,7 +1338,7 @@ constexpr int kTileSize[3] = {256, 128, 64};
 constexpr int kPerCu[3] = {1, 2, 4};
 // Rate of a full CU relative to 256 x 256 tiles (a smaller tile reads more of LDS and L2 a product;
 // float32 products are eight to sixteen times slower and do not notice)
-constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.95};
+constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.85};
 
 // The tile with the least time for `tiles(size)` tiles: rounds of the card times a round's work.
 template <typename F>
@@ -1357,14 +1398,13 @@ hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) 
   return rows_launch<T, 64, 64, 4, 1, QALONG, true>(a, s);
 }
 
-// Whether 16-byte granules can be loaded, and a granule's distance from the first row fits 32 bits.
+// Whether 16-byte granules can be loaded, and a row's stride in bytes fits 32 bits.
 bool grouped_aligned(const GroupedCall& c, bool dw) {
   const int v = c.type == IC_F32 ? 4 : 8;
   const int b = c.type == IC_F32 ? 4 : 2;
   auto fits = [&](const void* p, int64_t ld) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * b) % 16 == 0;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * b) % 16 == 0 && ld * b <= 0xffffffffll;
   };
-  if (!dw && c.n * (c.ld_x * b / 16) > 0xffffffffll) return false;
   if (dw) return fits(c.x, c.ld_x) && fits(c.w, c.ld_w) && c.k % v == 0 && c.out % v == 0;
   return fits(c.x, c.ld_x) && fits(c.w, c.k) && c.k % v == 0 && c.out % v == 0;
 }
