@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   const int pplace = across_place<T, BM, false>(pc, lane);
   const int qplace = kPBytes + across_place<T, BN, true>(qc, lane);
   int* ids = reinterpret_cast<int*>(smem + 2 * (kPBytes + kQBytes));   // [2][kK] rows of a stage
-  while (u < u1) {
+  for (int64_t done = 0; u < u1;) {
     const DwPlace pl = dw_place(a, u, kK, lane);
     const int64_t run = pl.stages - pl.stage < u1 - u ? pl.stages - pl.stage : u1 - u;
     u += run;
@@ -1137,9 +1137,19 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       const char* x0 = cx0 < a.k ? reinterpret_cast<const char*>(static_cast<const T*>(a.x) + cx0) : zero;
       const unsigned dy_ld = cd0 < a.out ? (unsigned)(a.ld_dy * (int64_t)sizeof(T)) : 0u;
       const unsigned x_ld = cx0 < a.k ? (unsigned)(a.ld_x * (int64_t)sizeof(T)) : 0u;
+      // The workgroups of an XCD work on tiles of the same rows, each beginning its run somewhere in the
+      // line.  Taking a tile's stages not from its first but from the one that a clock common to
+      // all (units since the start, `done`) points at keeps them at the same rows at the same time,
+      // and the rows in the L2 (65 536 rows, 16 groups of 2048 x 2048 bf16: 1.93 -> 1.46 GB fetched,
+      // 823 -> 737 us).
+      const int64_t turn = (done + stages - pl.stage % stages) % stages;
+      auto place_of = [&](int64_t st) {
+        const int64_t t = st + turn;
+        return t < stages ? t : t - stages;
+      };
       auto look = [&](int64_t st) {
         if (!a.order || wave != 0 || st >= stages) return;
-        int64_t pos = r0 + st * kK + (lane < kK ? lane : kK - 1);
+        int64_t pos = r0 + place_of(st) * kK + (lane < kK ? lane : kK - 1);
         if (pos >= a.g.n) pos = a.g.n - 1;
         lds_load4(a.order + pos, reinterpret_cast<char*>(ids + (st & 1) * 64));
       };
@@ -1147,7 +1157,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       constexpr int kLoads = kPLoads;
       auto load = [&](int i, int64_t st, char* buf) {
         const int q0 = (i * kWaves + wave) * 64;
-        const int64_t first = r0 + st * kK;
+        const int64_t first = r0 + place_of(st) * kK;
         if (kFixed && first + kK <= r1) {
           // (the columns are the same for every i, and behind the matrix a lane's pointer is that of
           // the zeros, its row stride 0)
@@ -1203,6 +1213,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       MULTIPLY_STAGES(stages, load, look, true, 2)
       __syncthreads();   // the buffers are free for the next run's loads
     }
+    done += run;
     const bool whole = pl.stage == 0 && run == pl.stages;
     if (whole) {
 #pragma unroll

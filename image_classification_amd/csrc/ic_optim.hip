@@ -213,6 +213,58 @@ __device__ __forceinline__ double finite_size(double v) {
   return __longlong_as_double(((unsigned long long)keep << 32) | (unsigned)b);
 }
 
+// A block of 256 elements is held by 32 lanes, eight elements each, from the codes to the new codes.
+// CAREFUL: some value of the wave is not finite (a gradient, or a code that marks one); it keeps such
+// values out of the scales and writes the marking codes.  The usual path has no test for them.
+template <bool CAREFUL>
+__device__ __forceinline__ void adamw8_lane(const AdamTensor& t, const AdamArgs& a, int64_t i, u32x2 mc, u32x2 vc,
+                                            const float* g, float* p, double sm, double sv, float lr1, float lrwd,
+                                            float eps, double root, u32x2* mo, u32x2* vo, float* out_sm,
+                                            float* out_sv) {
+  double m[8], r[8];
+  double top_m = 0.0, top_r = 0.0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const double gq = (double)g[q];
+    const unsigned cm = (mc[q >> 2] >> (8 * (q & 3))) & 255u, cv = (vc[q >> 2] >> (8 * (q & 3))) & 255u;
+    float fm = __uint_as_float(__float_as_uint(code_float<3>(cm & 127u)) | ((cm & 128u) << 24));
+    float fr = code_float<4>(cv);
+    if (CAREFUL) {
+      fm = (cm & 127u) == 127u ? __builtin_nanf("") : fm;
+      fr = cv == 255u ? __builtin_nanf("") : fr;
+    }
+    const double r0 = (double)fr * sv;
+    m[q] = fma(a.b1, (double)fm * sm, a.omb1 * gq);
+    const double v = fma(a.b2, r0 * r0, a.omb2 * (gq * gq));
+    r[q] = root_of(CAREFUL ? (v > kTiny ? v : v + kTiny) : fmax(v, kTiny));   // (careful: NaN stays)
+    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 * __builtin_amdgcn_rcpf((float)(r[q] * root) + eps);
+    top_m = fmax(top_m, CAREFUL ? finite_size(m[q]) : fabs(m[q]));
+    top_r = fmax(top_r, CAREFUL ? finite_size(r[q]) : r[q]);
+  }
+  const float new_sm = (float)(half_wave_max(top_m) * (1.0 / 448.0));
+  const float new_sv = (float)(half_wave_max(top_r) * (1.0 / 491520.0));
+  const double im = new_sm > 0.0f ? 512.0 / (double)new_sm : 0.0;
+  const double iv = new_sv > 0.0f ? 1.0 / (double)new_sv : 0.0;
+  // (a block without a value above zero keeps all its codes at zero)
+  const double seen = new_sv > 0.0f ? kSeen : __builtin_inf();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    unsigned cm = nearest_code<3>(fabs(m[q]) * im, 126u);
+    unsigned cv = nearest_code<4>(r[q] * iv, 254u);
+    const unsigned least = r[q] > seen ? 1u : 0u;
+    cv = cv > least ? cv : least;
+    if (CAREFUL) {
+      cm = fabs(m[q]) < __builtin_inf() ? cm : 127u;
+      cv = r[q] < __builtin_inf() ? cv : 255u;
+    }
+    cm |= m[q] < 0.0 ? 128u : 0u;
+    (*mo)[q >> 2] |= cm << (8 * (q & 3));
+    (*vo)[q >> 2] |= cv << (8 * (q & 3));
+  }
+  *out_sm = new_sm;
+  *out_sv = new_sv;
+}
+
 __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
   const int chunk = blockIdx.x;
   const AdamTensor& t = tab.t[find_tensor(tab, chunk)];
@@ -227,51 +279,41 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
   unsigned char* mp = static_cast<unsigned char*>(a.m) + t.state0 + i;
   unsigned char* vp = static_cast<unsigned char*>(a.v) + t.state0 + i;
   const int64_t block = (t.state0 + i) / kStateBlock;
-  const u32x2 mc = *reinterpret_cast<const u32x2*>(mp);
-  const u32x2 vc = *reinterpret_cast<const u32x2*>(vp);
+  u32x2 mc = *reinterpret_cast<const u32x2*>(mp);
+  u32x2 vc = *reinterpret_cast<const u32x2*>(vp);
   const double sm = (double)a.scale_m[block] * (kMUnit / 512.0), sv = (double)a.scale_v[block] * kRUnit;
   float p[8], g[8];
   get_typed(t.g, t.g_type, i, t.n, t.g_vec, g);
   get_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
-  double m[8], r[8];
-  double top_m = 0.0, top_r = 0.0;
+  if (i + 8 > t.n) {   // behind the tensor's end the states are 0, and so are p and g (get8)
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (i + q >= t.n) {
+        mc[q >> 2] &= ~(255u << (8 * (q & 3)));
+        vc[q >> 2] &= ~(255u << (8 * (q & 3)));
+      }
+  }
+  // anything that is not finite: x * 0 is NaN then; a byte of m with all of its lower seven bits set, or
+  // of v with all eight
+  float odd = 0.0f;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
-    const double gq = (double)(g[q] * a.grad_scale);
-    const unsigned cm = (mc[q >> 2] >> (8 * (q & 3))) & 255u, cv = (vc[q >> 2] >> (8 * (q & 3))) & 255u;
-    float fm = __uint_as_float(__float_as_uint(code_float<3>(cm & 127u)) | ((cm & 128u) << 24));
-    fm = (cm & 127u) == 127u ? __builtin_nanf("") : fm;
-    const float fr = cv == 255u ? __builtin_nanf("") : code_float<4>(cv);
-    const double r0 = (double)fr * sv;
-    m[q] = fma(a.b1, (double)fm * sm, a.omb1 * gq);
-    const double v = fma(a.b2, r0 * r0, a.omb2 * (gq * gq));
-    r[q] = root_of(v > kTiny ? v : v + kTiny);   // (NaN stays)
-    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 * __builtin_amdgcn_rcpf((float)(r[q] * root) + eps);
-    if (i + q >= t.n) {
-      m[q] = 0.0;
-      r[q] = 0.0;
-    }
-    top_m = fmax(top_m, finite_size(m[q]));
-    top_r = fmax(top_r, finite_size(r[q]));
+    g[q] *= a.grad_scale;
+    odd = fmaf(g[q], 0.0f, odd);
   }
-  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
-  const float new_sm = (float)(half_wave_max(top_m) * (1.0 / 448.0));
-  const float new_sv = (float)(half_wave_max(top_r) * (1.0 / 491520.0));
-  const double im = new_sm > 0.0f ? 512.0 / (double)new_sm : 0.0;
-  const double iv = new_sv > 0.0f ? 1.0 / (double)new_sv : 0.0;
+  unsigned marks = 0;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    marks |= ((mc[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    marks |= ((vc[w] & 0x7f7f7f7fu) + 0x01010101u) & vc[w] & 0x80808080u;
+  }
   u32x2 mo = {0u, 0u}, vo = {0u, 0u};
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const double am = fabs(m[q]);
-    unsigned cm = nearest_code<3>(am * im, 126u);
-    cm = am < __builtin_inf() ? cm : 127u;
-    cm |= m[q] < 0.0 ? 128u : 0u;
-    unsigned cv = nearest_code<4>(r[q] * iv, 254u);
-    cv = cv == 0u && r[q] > kSeen && new_sv > 0.0f ? 1u : cv;
-    cv = r[q] < __builtin_inf() ? cv : 255u;
-    mo[q >> 2] |= cm << (8 * (q & 3));
-    vo[q >> 2] |= cv << (8 * (q & 3));
-  }
+  float new_sm, new_sv;
+  if (__ballot(marks != 0u || odd != odd))
+    adamw8_lane<true>(t, a, i, mc, vc, g, p, sm, sv, lr1, lrwd, eps, root, &mo, &vo, &new_sm, &new_sv);
+  else
+    adamw8_lane<false>(t, a, i, mc, vc, g, p, sm, sv, lr1, lrwd, eps, root, &mo, &vo, &new_sm, &new_sv);
+  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
   *reinterpret_cast<u32x2*>(mp) = mo;
   *reinterpret_cast<u32x2*>(vp) = vo;
   if ((threadIdx.x & 31) == 0) {
