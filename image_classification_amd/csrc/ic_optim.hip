@@ -20,6 +20,8 @@
 // The update uses the new m and v before they are rounded.
 //
 // What bounds it: memory.  See the figures at each kernel.
+#include <cmath>
+
 #include "ic_wave.h"
 
 namespace ic {
@@ -37,6 +39,7 @@ struct AdamArgs {
   float* scale_m;
   float* scale_v;
   double lr, b1, b2, omb1, omb2, eps, wd, c1, c2;   // omb = 1 - b; c = 1 - b^t
+  double lr1, root2;         // lr / c1, sqrt(1 / c2): the usual step has no division in the kernel
   const float* lr_dev;       // not NULL: the learning rate is read here
   const int64_t* step_dev;   // not NULL: t is read here
   float grad_scale;
@@ -100,15 +103,19 @@ __device__ __forceinline__ void put_typed(void* p, int type, int64_t i, int64_t 
   else put8(static_cast<f16_t*>(p), i, n, vec, x);
 }
 
-__device__ __forceinline__ void corrections(const AdamArgs& a, double* lr, double* c1, double* c2) {
-  *lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-  if (a.step_dev) {
-    const int64_t t = *a.step_dev;
-    *c1 = 1.0 - power(a.b1, t);
-    *c2 = 1.0 - power(a.b2, t);
-  } else {
-    *c1 = a.c1;
-    *c2 = a.c2;
+__device__ __forceinline__ void corrections(const AdamArgs& a, double* lr, double* lr1, double* root2) {
+  *lr = a.lr;
+  *lr1 = a.lr1;
+  *root2 = a.root2;
+  if (a.lr_dev || a.step_dev) {
+    if (a.lr_dev) *lr = (double)*a.lr_dev;
+    double c1 = a.c1;
+    if (a.step_dev) {
+      const int64_t t = *a.step_dev;
+      c1 = 1.0 - power(a.b1, t);
+      *root2 = sqrt(1.0 / (1.0 - power(a.b2, t)));
+    }
+    *lr1 = *lr / c1;
   }
 }
 
@@ -117,11 +124,11 @@ __global__ __launch_bounds__(256) void k_adamw32(AdamTable tab, AdamArgs a) {
   const AdamTensor& t = tab.t[find_tensor(tab, chunk)];
   const int64_t i = (int64_t)(chunk - t.chunk0) * kChunk + (int64_t)threadIdx.x * 8;
   if (i >= t.n) return;
-  double lr, c1, c2;
-  corrections(a, &lr, &c1, &c2);
+  double lr, lr1d, root2;
+  corrections(a, &lr, &lr1d, &root2);
   const float b1 = (float)a.b1, b2 = (float)a.b2, omb1 = (float)a.omb1, omb2 = (float)a.omb2;
-  const float eps = (float)a.eps, lrwd = (float)(lr * a.wd), lr1 = (float)(lr / c1);
-  const float ic2 = (float)(1.0 / c2);
+  const float eps = (float)a.eps, lrwd = (float)(lr * a.wd), lr1 = (float)lr1d;
+  const float root = (float)root2;
   float p[8], g[8], m[8], v[8];
   float* mp = static_cast<float*>(a.m) + t.state0;
   float* vp = static_cast<float*>(a.v) + t.state0;
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(256) void k_adamw32(AdamTable tab, AdamArgs a) {
     const float gq = g[q] * a.grad_scale;
     m[q] = fmaf(b1, m[q], omb1 * gq);
     v[q] = fmaf(b2, v[q], omb2 * gq * gq);
-    const float den = __builtin_sqrtf(v[q] * ic2) + eps;
+    const float den = fmaf(__builtin_sqrtf(v[q]), root, eps);
     p[q] = fmaf(-lrwd, p[q], p[q]) - m[q] * lr1 / den;
   }
   put8(mp, i, t.n, true, m);
@@ -181,6 +188,12 @@ __device__ __forceinline__ double root_of(double v) {
   h = fma(h, r, h);
   return fma(fma(-g, g, v), h, g);
 }
+// 1 / x of a normal float64 to within its last bit or two, the same way
+__device__ __forceinline__ double inverse_of(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  y = fma(fma(-x, y, 1.0), y, y);
+  return fma(fma(-x, y, 1.0), y, y);
+}
 // v = 0 becomes kTiny, whose root is far below every scale; any v above zero has a larger root
 constexpr double kTiny = 1e-290, kSeen = 1.1e-145;
 
@@ -213,14 +226,26 @@ __device__ __forceinline__ double finite_size(double v) {
   return __longlong_as_double(((unsigned long long)keep << 32) | (unsigned)b);
 }
 
+// What a lane needs besides its elements: the block's old scales as the codes' units, the step.
+struct Lane8 {
+  double sm, sv;      // times a code's float32 (code_float) = the value
+  double b1, b2, omb1, omb2, root;
+  float lr1, lrwd, eps;
+};
+
+__device__ __forceinline__ float stepped(float p, float m, double r, const Lane8& s) {
+  return fmaf(-s.lrwd, p, p) - m * s.lr1 * __builtin_amdgcn_rcpf((float)(r * s.root) + s.eps);
+}
+
 // A block of 256 elements is held by 32 lanes, eight elements each, from the codes to the new codes.
-// CAREFUL: some value of the wave is not finite (a gradient, or a code that marks one); it keeps such
-// values out of the scales and writes the marking codes.  The usual path has no test for them.
-template <bool CAREFUL>
-__device__ __forceinline__ void adamw8_lane(const AdamTensor& t, const AdamArgs& a, int64_t i, u32x2 mc, u32x2 vc,
-                                            const float* g, float* p, double sm, double sv, float lr1, float lrwd,
-                                            float eps, double root, u32x2* mo, u32x2* vo, float* out_sm,
-                                            float* out_sv) {
+//
+// adamw8_careful decides every code in float64 and handles what is not finite.
+// adamw8_quick is for finite values.  Its codes come from the float64 quotients rounded to float32
+// once: m's by the hardware's conversion to this format (e4m3), v's from the float32 bits.  That is the
+// same code except where the float32 is exactly a middle between two codes (one in 2^19 or so), in
+// which case it returns true and the wave takes the careful way instead.
+__device__ __forceinline__ void adamw8_careful(const Lane8& s, u32x2 mc, u32x2 vc, const float* g, const float* p,
+                                               float* p_out, u32x2* mo, u32x2* vo, float* out_sm, float* out_sv) {
   double m[8], r[8];
   double top_m = 0.0, top_r = 0.0;
 #pragma unroll
@@ -229,34 +254,31 @@ __device__ __forceinline__ void adamw8_lane(const AdamTensor& t, const AdamArgs&
     const unsigned cm = (mc[q >> 2] >> (8 * (q & 3))) & 255u, cv = (vc[q >> 2] >> (8 * (q & 3))) & 255u;
     float fm = __uint_as_float(__float_as_uint(code_float<3>(cm & 127u)) | ((cm & 128u) << 24));
     float fr = code_float<4>(cv);
-    if (CAREFUL) {
-      fm = (cm & 127u) == 127u ? __builtin_nanf("") : fm;
-      fr = cv == 255u ? __builtin_nanf("") : fr;
-    }
-    const double r0 = (double)fr * sv;
-    m[q] = fma(a.b1, (double)fm * sm, a.omb1 * gq);
-    const double v = fma(a.b2, r0 * r0, a.omb2 * (gq * gq));
-    r[q] = root_of(CAREFUL ? (v > kTiny ? v : v + kTiny) : fmax(v, kTiny));   // (careful: NaN stays)
-    p[q] = fmaf(-lrwd, p[q], p[q]) - (float)m[q] * lr1 * __builtin_amdgcn_rcpf((float)(r[q] * root) + eps);
-    top_m = fmax(top_m, CAREFUL ? finite_size(m[q]) : fabs(m[q]));
-    top_r = fmax(top_r, CAREFUL ? finite_size(r[q]) : r[q]);
+    fm = (cm & 127u) == 127u ? __builtin_nanf("") : fm;
+    fr = cv == 255u ? __builtin_nanf("") : fr;
+    const double r0 = (double)fr * s.sv;
+    m[q] = fma(s.b1, (double)fm * s.sm, s.omb1 * gq);
+    const double v = fma(s.b2, r0 * r0, s.omb2 * (gq * gq));
+    r[q] = root_of(v > kTiny ? v : v + kTiny);   // (NaN stays)
+    p_out[q] = stepped(p[q], (float)m[q], r[q], s);
+    top_m = fmax(top_m, finite_size(m[q]));
+    top_r = fmax(top_r, finite_size(r[q]));
   }
   const float new_sm = (float)(half_wave_max(top_m) * (1.0 / 448.0));
   const float new_sv = (float)(half_wave_max(top_r) * (1.0 / 491520.0));
-  const double im = new_sm > 0.0f ? 512.0 / (double)new_sm : 0.0;
-  const double iv = new_sv > 0.0f ? 1.0 / (double)new_sv : 0.0;
-  // (a block without a value above zero keeps all its codes at zero)
+  const double im = new_sm > 0.0f ? 512.0 * inverse_of((double)new_sm) : 0.0;
+  const double iv = new_sv > 0.0f ? inverse_of((double)new_sv) : 0.0;
   const double seen = new_sv > 0.0f ? kSeen : __builtin_inf();
+  *mo = u32x2{0u, 0u};
+  *vo = u32x2{0u, 0u};
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     unsigned cm = nearest_code<3>(fabs(m[q]) * im, 126u);
     unsigned cv = nearest_code<4>(r[q] * iv, 254u);
     const unsigned least = r[q] > seen ? 1u : 0u;
     cv = cv > least ? cv : least;
-    if (CAREFUL) {
-      cm = fabs(m[q]) < __builtin_inf() ? cm : 127u;
-      cv = r[q] < __builtin_inf() ? cv : 255u;
-    }
+    cm = fabs(m[q]) < __builtin_inf() ? cm : 127u;
+    cv = r[q] < __builtin_inf() ? cv : 255u;
     cm |= m[q] < 0.0 ? 128u : 0u;
     (*mo)[q >> 2] |= cm << (8 * (q & 3));
     (*vo)[q >> 2] |= cv << (8 * (q & 3));
@@ -265,17 +287,75 @@ __device__ __forceinline__ void adamw8_lane(const AdamTensor& t, const AdamArgs&
   *out_sv = new_sv;
 }
 
+__device__ __forceinline__ bool adamw8_quick(const Lane8& s, u32x2 mc, u32x2 vc, const float* g, const float* p,
+                                             float* p_out, u32x2* mo, u32x2* vo, float* out_sm, float* out_sv) {
+  double m[8], r[8];
+  double top_m = 0.0, top_r = 0.0;
+  // (the hardware decodes m in units of the scale; code_float's unit is 2^-129 of it)
+  const double b1sm = s.b1 * s.sm * 0x1p-120, b2sv2 = s.b2 * (s.sv * s.sv);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const double gq = (double)g[q];
+    const int w = (int)mc[q >> 2];
+    const float fm = (q & 3) == 0 ? __builtin_amdgcn_cvt_f32_fp8(w, 0)
+                     : (q & 3) == 1 ? __builtin_amdgcn_cvt_f32_fp8(w, 1)
+                     : (q & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8(w, 2)
+                                    : __builtin_amdgcn_cvt_f32_fp8(w, 3);
+    const double fr = (double)code_float<4>((vc[q >> 2] >> (8 * (q & 3))) & 255u);
+    m[q] = fma((double)fm, b1sm, s.omb1 * gq);
+    const double v = fma(fr * fr, b2sv2, s.omb2 * (gq * gq));
+    r[q] = root_of(fmax(v, kTiny));
+    p_out[q] = stepped(p[q], (float)m[q], r[q], s);
+    top_m = fmax(top_m, fabs(m[q]));
+    top_r = fmax(top_r, r[q]);
+  }
+  const float new_sm = (float)(half_wave_max(top_m) * (1.0 / 448.0));
+  const float new_sv = (float)(half_wave_max(top_r) * (1.0 / 491520.0));
+  const double im = new_sm > 0.0f ? inverse_of((double)new_sm) : 0.0;
+  const double iv = new_sv > 0.0f ? inverse_of((double)new_sv) : 0.0;
+  const double seen = new_sv > 0.0f ? kSeen : __builtin_inf();
+  bool doubt = false;
+  float qm[8];
+  *vo = u32x2{0u, 0u};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    qm[q] = (float)(m[q] * im);
+    // below 2^-6 e4m3's grid is that of [2^-6, 2^-5)
+    const float am = fabsf(qm[q]);
+    const float t = am + (am < 0x1p-6f ? 0x1p-6f : 0.0f);
+    doubt |= (__float_as_uint(t) & 0xfffffu) == 0x80000u;
+    // v: below 16 the grid is that of [16, 32)
+    float qv = (float)(r[q] * iv);
+    qv = r[q] > seen ? fmaxf(qv, 1.0f) : 0.0f;
+    const bool small = qv < 16.0f;
+    const unsigned bits = __float_as_uint(qv + (small ? 16.0f : 0.0f));
+    doubt |= (bits & 0x7ffffu) == 0x40000u;
+    // exponent 4 is code exponent 1
+    const unsigned base = small ? (131u << 23) : (130u << 23);
+    const unsigned cv = (bits + 0x3ffffu + ((bits >> 19) & 1u) - base) >> 19;
+    (*vo)[q >> 2] |= cv << (8 * (q & 3));
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(qm[4 * w], qm[4 * w + 1], 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(qm[4 * w + 2], qm[4 * w + 3], c, true);
+    (*mo)[w] = (unsigned)c;
+  }
+  *out_sm = new_sm;
+  *out_sv = new_sv;
+  return doubt;
+}
+
 __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
   const int chunk = blockIdx.x;
   const AdamTensor& t = tab.t[find_tensor(tab, chunk)];
   const int64_t i = (int64_t)(chunk - t.chunk0) * kChunk + (int64_t)threadIdx.x * 8;
   const int64_t padded = (t.n + kStateBlock - 1) / kStateBlock * kStateBlock;
   if (i >= padded) return;   // whole blocks: their 32 lanes stay together
-  double lr, c1, c2;
-  corrections(a, &lr, &c1, &c2);
+  double lr, lr1d, root;
+  corrections(a, &lr, &lr1d, &root);
   // (the step itself is float32: only what becomes a code has to be decided in float64)
-  const float lr1 = (float)(lr / c1), lrwd = (float)(lr * a.wd), eps = (float)a.eps;
-  const double root = sqrt(1.0 / c2);
+  const float lr1 = (float)lr1d, lrwd = (float)(lr * a.wd), eps = (float)a.eps;
   unsigned char* mp = static_cast<unsigned char*>(a.m) + t.state0 + i;
   unsigned char* vp = static_cast<unsigned char*>(a.v) + t.state0 + i;
   const int64_t block = (t.state0 + i) / kStateBlock;
@@ -307,13 +387,13 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
     marks |= ((mc[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
     marks |= ((vc[w] & 0x7f7f7f7fu) + 0x01010101u) & vc[w] & 0x80808080u;
   }
-  u32x2 mo = {0u, 0u}, vo = {0u, 0u};
-  float new_sm, new_sv;
-  if (__ballot(marks != 0u || odd != odd))
-    adamw8_lane<true>(t, a, i, mc, vc, g, p, sm, sv, lr1, lrwd, eps, root, &mo, &vo, &new_sm, &new_sv);
-  else
-    adamw8_lane<false>(t, a, i, mc, vc, g, p, sm, sv, lr1, lrwd, eps, root, &mo, &vo, &new_sm, &new_sv);
-  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p);
+  const Lane8 l{sm, sv, a.b1, a.b2, a.omb1, a.omb2, root, lr1, lrwd, eps};
+  u32x2 mo, vo;
+  float p_out[8], new_sm, new_sv;
+  bool again = marks != 0u || odd != odd;
+  if (!__ballot(again)) again = adamw8_quick(l, mc, vc, g, p, p_out, &mo, &vo, &new_sm, &new_sv);
+  if (__ballot(again)) adamw8_careful(l, mc, vc, g, p, p_out, &mo, &vo, &new_sm, &new_sv);
+  put_typed(t.p, t.p_type, i, t.n, t.p_vec, p_out);
   *reinterpret_cast<u32x2*>(mp) = mo;
   *reinterpret_cast<u32x2*>(vp) = vo;
   if ((threadIdx.x & 31) == 0) {
@@ -374,6 +454,8 @@ hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int bits, void
   }
   a.c1 = 1.0 - p1;
   a.c2 = 1.0 - p2;
+  a.lr1 = lr / a.c1;
+  a.root2 = std::sqrt(1.0 / a.c2);
   a.lr_dev = lr_dev;
   a.step_dev = step_dev;
   a.grad_scale = grad_scale;
