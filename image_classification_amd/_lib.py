@@ -104,6 +104,8 @@ def library_path():
 def load():
     """Load libic_hip.so and declare every prototype.  Raises if the library was not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lib_lock:
         if _lib is None:
             path = library_path()

@@ -4,6 +4,7 @@ torch is used for device memory and streams only; all arithmetic happens in libi
 numpy-in / numpy-out mirrors of the reference's call sites (vq.py, features.py, classifiers.py,
 robust_matching.py, scene_functions.py) are thin layers over these functions.
 """
+import array
 import collections
 import ctypes
 import os
@@ -912,6 +913,20 @@ def ransac_homography(pts, offsets, n_iter, th, samples=None, seed=0, min_inlier
 # -- what is learned on top of the codes -------------------------------------------------------------
 # Launches only: memory a call needs for itself is allocated here, from torch's allocator on the
 # current stream, so these calls may be captured into a graph and used on any stream.
+# (A small call is bound by what Python does around it: addresses go to ctypes as plain integers, and
+# the stream is asked for once, without a Stream object.)
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(dev):
+    return _raw_stream(dev) if _raw_stream is not None \
+        else torch.cuda.current_stream(dev).cuda_stream
+
+
 _TYPE_NUMBER = {torch.float32: _lib.IC_F32, torch.bfloat16: _lib.IC_BF16, torch.float16: _lib.IC_F16}
 MAX_TOP = 32                 # alternatives label_logprobs returns per row
 MAX_GROUPS = 1 << 26
@@ -966,8 +981,8 @@ def group_rows(codes, n_groups):
     lib = _lib.load()
     nbytes = lib.ic_group_rows_scratch(n, n_groups)
     scratch = _scratch(nbytes, codes.device)
-    rc = lib.ic_group_rows(_lib.handle(dev), _ptr(codes), n, n_groups, _ptr(order), _ptr(offsets),
-                           _ptr(scratch), nbytes, _stream_ptr(dev))
+    rc = lib.ic_group_rows(_lib.handle(dev), _addr(codes), n, n_groups, _addr(order), _addr(offsets),
+                           _addr(scratch), nbytes, _stream_of(dev))
     _lib.check(rc, "ic_group_rows")
     return order, offsets
 
@@ -1021,8 +1036,8 @@ def _grouped_rows(fn_name, x, w, offsets, order, out, out_dtype, dx):
     y, yt = _result(out, out_dtype, (n, cols), x, "the result")
     ld_y = _check_rows(y, "out")
     lib = _lib.load()
-    rc = getattr(lib, fn_name)(_lib.handle(dev), _ptr(x), ld_x, _ptr(w), _ptr(y), ld_y, _ptr(offsets),
-                               _ptr(order), n, groups, k, o, t, yt, _stream_ptr(dev))
+    rc = getattr(lib, fn_name)(_lib.handle(dev), _addr(x), ld_x, _addr(w), _addr(y), ld_y, _addr(offsets),
+                               _addr(order), n, groups, k, o, t, yt, _stream_of(dev))
     _lib.check(rc, fn_name)
     return y
 
@@ -1069,9 +1084,9 @@ def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
     lib = _lib.load()
     nbytes = lib.ic_grouped_matmul_dw_scratch(n, groups, k, o, t)
     scratch = _scratch(nbytes, x.device)
-    rc = lib.ic_grouped_matmul_dw(_lib.handle(dev), _ptr(dy), ld_dy, _ptr(x), ld_x, _ptr(dw),
-                                  _ptr(offsets), _ptr(order), n, groups, k, o, t, yt, _ptr(scratch),
-                                  nbytes, _stream_ptr(dev))
+    rc = lib.ic_grouped_matmul_dw(_lib.handle(dev), _addr(dy), ld_dy, _addr(x), ld_x, _addr(dw),
+                                  _addr(offsets), _addr(order), n, groups, k, o, t, yt, _addr(scratch),
+                                  nbytes, _stream_of(dev))
     _lib.check(rc, "ic_grouped_matmul_dw")
     return dw
 
@@ -1125,9 +1140,9 @@ def label_logprobs(logits, labels=None, top=0, temperature=1.0):
     lib = _lib.load()
     nbytes = lib.ic_label_logprobs_scratch(n, v, t, top)
     scratch = _scratch(nbytes, device)
-    rc = lib.ic_label_logprobs(_lib.handle(dev), _ptr(logits), ld, n, v, t, _ptr(labels), l64, inv, top,
-                               _ptr(logp), _ptr(stats[0]), _ptr(stats[1]), _ptr(top_logp),
-                               _ptr(top_idx), _ptr(scratch), nbytes, _stream_ptr(dev))
+    rc = lib.ic_label_logprobs(_lib.handle(dev), _addr(logits), ld, n, v, t, _addr(labels), l64, inv, top,
+                               _addr(logp), _addr(stats[0]), _addr(stats[1]), _addr(top_logp),
+                               _addr(top_idx), _addr(scratch), nbytes, _stream_of(dev))
     _lib.check(rc, "ic_label_logprobs")
     return logp, stats[0], stats[1], top_logp, top_idx
 
@@ -1165,15 +1180,14 @@ def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=Non
         raise ValueError("out must be a %s %s tensor on %s" % (logits.dtype, (n, v), device))
     ld_out = _check_rows(out, "out")
     rc = _lib.load().ic_label_logprobs_grad(
-        _lib.handle(dev), _ptr(logits), ld, n, v, t, _ptr(labels), l64, inv, _ptr(lse), _ptr(entropy),
-        _ptr(d_logp), _ptr(d_entropy), _ptr(out), ld_out, _stream_ptr(dev))
+        _lib.handle(dev), _addr(logits), ld, n, v, t, _addr(labels), l64, inv, _addr(lse), _addr(entropy),
+        _addr(d_logp), _addr(d_entropy), _addr(out), ld_out, _stream_of(dev))
     _lib.check(rc, "ic_label_logprobs_grad")
     return out
 
 
-# one row of the table adamw_step hands over: struct ic_adamw_tensor
-_ADAMW_TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("n", "<i8"), ("state_offset", "<i8"),
-                          ("param_dtype", "<i4"), ("grad_dtype", "<i4")])
+# param_dtype and grad_dtype of struct ic_adamw_tensor (int32 each) as one little-endian word
+_ADAMW_TYPES = {(p, g): pt | gt << 32 for p, pt in _TYPE_NUMBER.items() for g, gt in _TYPE_NUMBER.items()}
 ADAMW_BLOCK = _lib.IC_ADAMW_BLOCK
 
 
@@ -1228,21 +1242,20 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
             or exp_avg_sq.shape != exp_avg.shape or not exp_avg.is_contiguous() \
             or not exp_avg_sq.is_contiguous():
         raise ValueError("exp_avg and exp_avg_sq must be flat, contiguous and alike")
-    table = np.empty(count, dtype=_ADAMW_TENSOR)
-    rows = []
+    table = []      # struct ic_adamw_tensor, the two type numbers as one integer
     at = 0
-    types = _TYPE_NUMBER
     for p, g in zip(params, grads):
         n = p.numel()
-        if g.numel() != n or p.device != device or g.device != device:
+        if g.numel() != n or p.get_device() != dev or g.get_device() != dev:
             raise ValueError("a gradient must match its parameter, on the states' device")
         if not (p.is_contiguous() and g.is_contiguous()):
             raise ValueError("parameters and gradients must be contiguous")
         try:
-            rows.append((p.data_ptr(), g.data_ptr(), n, at, types[p.dtype], types[g.dtype]))
+            kinds = _ADAMW_TYPES[p.dtype, g.dtype]
         except KeyError:
             raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
-        at += (n + ADAMW_BLOCK - 1) // ADAMW_BLOCK * ADAMW_BLOCK
+        table += (p.data_ptr(), g.data_ptr(), n, at, kinds)
+        at += -(-n // ADAMW_BLOCK) * ADAMW_BLOCK
     size = exp_avg.shape[0]
     if at != size:
         raise ValueError("the states have %d elements, these tensors need %d" % (size, at))
@@ -1251,7 +1264,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
         raise ValueError("uint8 states need contiguous float32 scales [2, %d]" % (size // ADAMW_BLOCK))
     if count == 0:
         return
-    table[:] = rows
+    table = array.array("q", table)
     lr_t = step_t = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
@@ -1267,9 +1280,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not eps >= 0:
         raise ValueError("betas must be in [0, 1) and eps must not be negative")
     rc = _lib.load().ic_adamw_step(
-        _lib.handle(dev), table.ctypes.data, count, bits, _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(scales),
-        size, float(lr), _ptr(lr_t), b1, b2, float(eps), float(weight_decay), int(step), _ptr(step_t),
-        float(grad_scale), _stream_ptr(dev))
+        _lib.handle(dev), table.buffer_info()[0], count, bits, _addr(exp_avg), _addr(exp_avg_sq), _addr(scales),
+        size, float(lr), _addr(lr_t), b1, b2, float(eps), float(weight_decay), int(step), _addr(step_t),
+        float(grad_scale), _stream_of(dev))
     _lib.check(rc, "ic_adamw_step")
 
 
@@ -1290,8 +1303,8 @@ def adamw_state_values(exp_avg, exp_avg_sq, scales=None):
     _check_same_device(exp_avg.device, (exp_avg_sq, "exp_avg_sq"), (scales, "scales"))
     m = torch.empty(size, dtype=torch.float32, device=exp_avg.device)
     v = torch.empty(size, dtype=torch.float32, device=exp_avg.device)
-    rc = _lib.load().ic_adamw_state_values(_lib.handle(dev), _ptr(exp_avg), _ptr(exp_avg_sq),
-                                           _ptr(scales), size, _ptr(m), _ptr(v), _stream_ptr(dev))
+    rc = _lib.load().ic_adamw_state_values(_lib.handle(dev), _addr(exp_avg), _addr(exp_avg_sq),
+                                           _addr(scales), size, _addr(m), _addr(v), _stream_of(dev))
     _lib.check(rc, "ic_adamw_state_values")
     return m, v
 
