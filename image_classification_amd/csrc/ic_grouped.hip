@@ -62,7 +62,7 @@ __device__ __forceinline__ unsigned rank_in_wave(Count* cnt, unsigned d, bool in
 
 // Few rows: one workgroup, everything in LDS (bitonic sorting took 18.6 us for 1000 rows: 66 steps of a
 // barrier each).
-constexpr int kSmallRows = 4096;
+constexpr int kSmallRows = 8192, kSmallBits = 8;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restrict__ codes, int n,
                                                          int64_t groups, int passes, int digit_bits,
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restri
                                                          int64_t* __restrict__ offsets) {
   constexpr int kWaves = THREADS / 64, kMost = THREADS == 1024 ? kSmallRows / THREADS : 1;
   constexpr int kRows = THREADS * kMost;
-  __shared__ unsigned short cnt[kWaves][1 << kMaxDigitBits];   // (at most 4096 rows)
+  __shared__ unsigned short cnt[kWaves][1 << kSmallBits];   // (at most 8192 rows)
   __shared__ unsigned keys[kRows];
   __shared__ unsigned short rows[kRows];
   __shared__ unsigned wave_sum[kWaves];
@@ -586,30 +586,33 @@ __device__ __forceinline__ void read_fragments(const char* tile, int place, int 
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// One granule of an operand: elements [c, c + kVec) of a row of `cols` elements (NULL row: zeros).
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, char* lds_wave_base, int lane) {
+// One granule of an operand: elements [c, c + kVec) of a row of `cols` elements (NULL row: zeros), to
+// LDS.  ALIGNED: granules begin at 16 bytes and do not cross the row's end.
+template <typename T>
+__device__ __forceinline__ u32x4 granule_of(const T* row, int64_t c, int64_t cols) {
   constexpr int kV = Elem<T>::kVec;
-  if constexpr (ALIGNED) {
-    const void* src = row && c < cols ? static_cast<const void*>(row + c)
-                                      : static_cast<const void*>(kZeroGranule);
-    lds_load16(src, lds_wave_base);
-  } else {
-    u32x4 w = {0u, 0u, 0u, 0u};
-    if (row) {
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (row && c + kV <= cols) {
+    __builtin_memcpy(&w, row + c, 16);   // (a 16-byte load: memory may be read at any address)
+  } else if (row) {
 #pragma unroll
-      for (int i = 0; i < kV; ++i)
-        if (c + i < cols) {
-          if constexpr (sizeof(T) == 2) {
-            const unsigned b = reinterpret_cast<const unsigned short*>(row)[c + i];
-            w[i >> 1] |= b << (16 * (i & 1));
-          } else {
-            w[i] = reinterpret_cast<const unsigned*>(row)[c + i];
-          }
+    for (int i = 0; i < kV; ++i)
+      if (c + i < cols) {
+        if constexpr (sizeof(T) == 2) {
+          const unsigned b = reinterpret_cast<const unsigned short*>(row)[c + i];
+          w[i >> 1] |= b << (16 * (i & 1));
+        } else {
+          w[i] = reinterpret_cast<const unsigned*>(row)[c + i];
         }
-    }
-    *reinterpret_cast<u32x4*>(lds_wave_base + lane * 16) = w;
+      }
   }
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, char* lds_wave_base) {
+  const void* src = row && c < cols ? static_cast<const void*>(row + c)
+                                    : static_cast<const void*>(kZeroGranule);
+  lds_load16(src, lds_wave_base);
 }
 
 // The stages of a tile.  Each is multiplied in two steps, and a step in kHalves parts of the wave's
@@ -620,13 +623,15 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
 //     ... | read the last part | multiply the one before | stage st + 1 has landed, barrier |
 //     read the first part of st + 1 | multiply the last part of st
 // The freed buffer is refilled with stage st + 2 one load per four products, during the last part of
-// st and the first of st + 1: issued in one go behind the barrier, the 8 waves' loads would hold up
-// the products behind them in every wave.
-// LOAD(i, stage, buffer) issues load i of kLoads (LOADS_EACH instructions); with PREPARES, NEXT(stage) fetches what the loads of
+// st and (of four parts) the first of st + 1: issued in one go behind the barrier, the 8 waves' loads
+// would hold up the products behind them in every wave.
+// LOAD(i, stage, buffer) issues load i of kLoads (LOADS_EACH instructions), straight to the buffer if
+// ALIGNED, else to registers that PLACE(i, buffer) writes there a stage later; with PREPARES, NEXT(stage) fetches what the loads of
 // that stage need, and lands a barrier before them.
-#define MULTIPLY_STAGES(STAGES, LOAD, NEXT, PREPARES, LOADS_EACH)                                          \
+#define MULTIPLY_STAGES(STAGES, LOAD, PLACE, NEXT, PREPARES, LOADS_EACH)                                          \
   {                                                                                  \
-    constexpr int kStage = kPBytes + kQBytes, kFirst = kLoads / 2;                   \
+    constexpr int kStage = kPBytes + kQBytes;                                        \
+    constexpr int kFirst = kHalves == 2 && ALIGNED ? kLoads / 2 : kLoads;            \
     auto none = [](int) {};                                                          \
     if (PREPARES) {                                                                  \
       NEXT(0);                                                                       \
@@ -635,8 +640,14 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       __syncthreads();                                                               \
     }                                                                                \
     _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0, smem);             \
+    if (!ALIGNED) {                                                                  \
+      _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, smem);             \
+    }                                                                                \
     if (STAGES > 1) {                                                                \
       _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1, smem + kStage);  \
+      if (!ALIGNED) {                                                                \
+        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, smem + kStage);  \
+      }                                                                              \
       all_but<kLoads * LOADS_EACH>();                                                \
     } else {                                                                         \
       all_landed();                                                                  \
@@ -658,6 +669,9 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       mul(0, 0, 0, kLoads - kFirst, [&](int i) {                                     \
         if (more) LOAD(kFirst + i, st + 1, other);                                   \
       });                                                                            \
+      if (!ALIGNED && more) {                                                        \
+        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, other);          \
+      }                                                                              \
       if (PREPARES && st > 0) NEXT(st + 2);                                          \
       if (kHalves == 2) {                                                            \
         read_q(buf, 1, 1);                                                           \
@@ -795,31 +809,44 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
     const bool inside = ALIGNED && c0 + BN <= a.cols;
     const int full = a.depth / kK;     // stages that lie inside the depth
     constexpr int kLoads = kPLoads + kQLoads;
+    u32x4 held[ALIGNED ? 1 : kLoads];
     auto load = [&](int i, int st, char* buf) {
       const int64_t k0 = (int64_t)st * kK;
       if (i < kPLoads) {
         char* to = buf + (i * kWaves + wave) * 1024;
-        if (ALIGNED && st < full) lds_load16(prow[i] + along + k0, to);
-        else fetch<T, ALIGNED>(prow[i], k0 + along, a.depth, to, lane);
+        if constexpr (!ALIGNED) held[i] = granule_of<T>(prow[i], k0 + along, a.depth);
+        else if (st < full) lds_load16(prow[i] + along + k0, to);
+        else fetch<T>(prow[i], k0 + along, a.depth, to);
         return;
       }
-      i -= kPLoads;
-      char* to = buf + kPBytes + (i * kWaves + wave) * 1024;
+      const int q = i - kPLoads;
+      char* to = buf + kPBytes + (q * kWaves + wave) * 1024;
+      if (inside && st < full) {
+        const T* base = QALONG ? qb + (int64_t)(c0 + q * kQStep) * a.ld_q + k0 : qb + (k0 + q * kQStep) * a.ld_q + c0;
+        if constexpr (ALIGNED) lds_load16_at(base, q % 2 ? qoff1 : qoff0, to);
+        return;
+      }
+      const T* row;
+      int64_t from, width;
       if (QALONG) {
-        if (inside && st < full) {
-          lds_load16_at(qb + (int64_t)(c0 + i * kQStep) * a.ld_q + k0, i % 2 ? qoff1 : qoff0, to);
-        } else {
-          const int c = c0 + qfirst + i * kQStep;
-          fetch<T, ALIGNED>(c < a.cols ? qb + (int64_t)c * a.ld_q : nullptr, k0 + qgranule(i) * kV, a.depth, to,
-                            lane);
-        }
+        const int c = c0 + qfirst + q * kQStep;
+        row = c < a.cols ? qb + (int64_t)c * a.ld_q : nullptr;
+        from = k0 + qgranule(q) * kV;
+        width = a.depth;
       } else {
-        if (inside && st < full) {
-          lds_load16_at(qb + (k0 + i * kQStep) * a.ld_q + c0, i % 2 ? qoff1 : qoff0, to);
-        } else {
-          const int64_t k = k0 + qfirst + i * kQStep;
-          fetch<T, ALIGNED>(k < a.depth ? qb + k * a.ld_q : nullptr, c0 + qgranule(i) * kV, a.cols, to, lane);
-        }
+        const int64_t k = k0 + qfirst + q * kQStep;
+        row = k < a.depth ? qb + k * a.ld_q : nullptr;
+        from = c0 + qgranule(q) * kV;
+        width = a.cols;
+      }
+      if constexpr (ALIGNED) fetch<T>(row, from, width, to);
+      else held[i] = granule_of<T>(row, from, width);
+    };
+    auto place = [&](int i, char* buf) {
+      if constexpr (!ALIGNED) {
+        char* to = i < kPLoads ? buf + (i * kWaves + wave) * 1024
+                               : buf + kPBytes + ((i - kPLoads) * kWaves + wave) * 1024;
+        *reinterpret_cast<u32x4*>(to + lane * 16) = held[i];
       }
     };
     const int stages = (int)(((int64_t)a.depth + kK - 1) / kK);
@@ -855,7 +882,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     };
     auto next = [](int) {};
-    MULTIPLY_STAGES(stages, load, next, false, 1)
+    MULTIPLY_STAGES(stages, load, place, next, false, 1)
   } else {
     __syncthreads();
   }
@@ -923,12 +950,12 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
         char* to = smem + st * kStage + (i * kWaves + wave) * 1024;
         if (QALONG) {
           const int r = q >> 3;
-          fetch<T, true>(c0 + r < a.cols ? qb + (int64_t)(c0 + r) * a.ld_q : nullptr,
-                         st * kK + ((q & 7) ^ along_swap_q<T>(r)) * kV, a.depth, to, lane);
+          fetch<T>(c0 + r < a.cols ? qb + (int64_t)(c0 + r) * a.ld_q : nullptr,
+                         st * kK + ((q & 7) ^ along_swap_q<T>(r)) * kV, a.depth, to);
         } else {
           const int k = q / kQRow;
-          fetch<T, true>(st * kK + k < a.depth ? qb + (int64_t)(st * kK + k) * a.ld_q : nullptr,
-                         c0 + ((q % kQRow) ^ across_swap_q<T, BN>(k)) * kV, a.cols, to, lane);
+          fetch<T>(st * kK + k < a.depth ? qb + (int64_t)(st * kK + k) * a.ld_q : nullptr,
+                         c0 + ((q % kQRow) ^ across_swap_q<T, BN>(k)) * kV, a.cols, to);
         }
       }
     const int qplace = QALONG ? along_place_q<T>(0, lane) : across_place<T, BN, true>(0, lane);
@@ -1128,15 +1155,24 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       // loads that need it (without an order the positions are the rows).
       const int64_t stages = (r1 - r0 + kK - 1) / kK;
       // this lane's first granule of either operand, and its row stride, in bytes
-      constexpr bool kFixed = ALIGNED && kThreads / kPRow % 16 == 0;
+      constexpr bool kFixed = ALIGNED;
       const int lin = wave * 64 + lane;
-      const int cd0 = m0 + ((lin % kPRow) ^ across_swap_p<T, BM>(lin / kPRow)) * kV;
-      const int cx0 = n0 + ((lin % kPRow) ^ across_swap_q<T, BN>(lin / kPRow)) * kV;
+      // (granule i lies kStep rows behind granule 0, where the swap is the same, or one of two in turn)
+      constexpr int kStep = kThreads / kPRow, kTurns = kStep % 16 == 0 ? 1 : 2;
+      static_assert(kStep % 8 == 0, "the swaps repeat");
       const char* zero = reinterpret_cast<const char*>(kZeroGranule);
-      const char* dy0 = cd0 < a.out ? reinterpret_cast<const char*>(static_cast<const T*>(a.dy) + cd0) : zero;
-      const char* x0 = cx0 < a.k ? reinterpret_cast<const char*>(static_cast<const T*>(a.x) + cx0) : zero;
-      const unsigned dy_ld = cd0 < a.out ? (unsigned)(a.ld_dy * (int64_t)sizeof(T)) : 0u;
-      const unsigned x_ld = cx0 < a.k ? (unsigned)(a.ld_x * (int64_t)sizeof(T)) : 0u;
+      const char *dy0[kTurns], *x0[kTurns];
+      unsigned dy_ld[kTurns], x_ld[kTurns];
+#pragma unroll
+      for (int h = 0; h < kTurns; ++h) {
+        const int k = lin / kPRow + h * kStep;
+        const int cd = m0 + ((lin % kPRow) ^ across_swap_p<T, BM>(k)) * kV;
+        const int cx = n0 + ((lin % kPRow) ^ across_swap_q<T, BN>(k)) * kV;
+        dy0[h] = cd < a.out ? reinterpret_cast<const char*>(static_cast<const T*>(a.dy) + cd) : zero;
+        x0[h] = cx < a.k ? reinterpret_cast<const char*>(static_cast<const T*>(a.x) + cx) : zero;
+        dy_ld[h] = cd < a.out ? (unsigned)(a.ld_dy * (int64_t)sizeof(T)) : 0u;
+        x_ld[h] = cx < a.k ? (unsigned)(a.ld_x * (int64_t)sizeof(T)) : 0u;
+      }
       // The workgroups of an XCD work on tiles of the same rows, each beginning its run somewhere in the
       // line.  Taking a tile's stages not from its first but from the one that a clock common to
       // all (units since the start, `done`) points at keeps them at the same rows at the same time,
@@ -1155,18 +1191,18 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       };
       // load i: dy's and x's granules of one row
       constexpr int kLoads = kPLoads;
+      u32x4 held[ALIGNED ? 1 : 2 * kLoads];
       auto load = [&](int i, int64_t st, char* buf) {
         const int q0 = (i * kWaves + wave) * 64;
         const int64_t first = r0 + place_of(st) * kK;
         if (kFixed && first + kK <= r1) {
-          // (the columns are the same for every i, and behind the matrix a lane's pointer is that of
-          // the zeros, its row stride 0)
-          int k = lin / kPRow + i * (kThreads / kPRow);
+          // (behind the matrix a lane's pointer is that of the zeros, its row stride 0)
+          const int k = lin / kPRow + i * kStep, h = i % kTurns;
           unsigned r = (unsigned)first + (unsigned)k;
           if (a.order) r = (unsigned)ids[(st & 1) * 64 + k];
           const bool in = r < (unsigned)a.g.n;
-          const char* d = dy0 + (uint64_t)r * dy_ld;
-          const char* x = x0 + (uint64_t)r * x_ld;
+          const char* d = dy0[h] + (uint64_t)r * dy_ld[h];
+          const char* x = x0[h] + (uint64_t)r * x_ld[h];
           lds_load16(in ? d : reinterpret_cast<const char*>(kZeroGranule), buf + q0 * 16);
           lds_load16(in ? x : reinterpret_cast<const char*>(kZeroGranule), buf + kPBytes + q0 * 16);
           return;
@@ -1180,8 +1216,20 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         const int cd = m0 + (s ^ across_swap_p<T, BM>(k)) * kV, cx = n0 + (s ^ across_swap_q<T, BN>(k)) * kV;
         const T* rd = static_cast<const T*>(a.dy) + (int64_t)r * a.ld_dy;
         const T* rx = static_cast<const T*>(a.x) + (int64_t)r * a.ld_x;
-        fetch<T, ALIGNED>(in ? rd : nullptr, cd, a.out, buf + q0 * 16, lane);
-        fetch<T, ALIGNED>(in ? rx : nullptr, cx, a.k, buf + kPBytes + q0 * 16, lane);
+        if constexpr (ALIGNED) {
+          fetch<T>(in ? rd : nullptr, cd, a.out, buf + q0 * 16);
+          fetch<T>(in ? rx : nullptr, cx, a.k, buf + kPBytes + q0 * 16);
+        } else {
+          held[2 * i] = granule_of<T>(in ? rd : nullptr, cd, a.out);
+          held[2 * i + 1] = granule_of<T>(in ? rx : nullptr, cx, a.k);
+        }
+      };
+      auto place = [&](int i, char* buf) {
+        if constexpr (!ALIGNED) {
+          const int at = ((i * kWaves + wave) * 64 + lane) * 16;
+          *reinterpret_cast<u32x4*>(buf + at) = held[2 * i];
+          *reinterpret_cast<u32x4*>(buf + kPBytes + at) = held[2 * i + 1];
+        }
       };
       constexpr int kHalves = FM >= 4 ? 2 : 1, kHalf = FM / kHalves;
       u32x4 pf[2][kHalf], qf[2][FN];
@@ -1210,7 +1258,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      MULTIPLY_STAGES(stages, load, look, true, 2)
+      MULTIPLY_STAGES(stages, load, place, look, true, 2)
       __syncthreads();   // the buffers are free for the next run's loads
     }
     done += run;
@@ -1506,12 +1554,13 @@ hipError_t launch_group_rows(const int32_t* codes, int64_t n, int64_t groups, in
                              int64_t* offsets, void* scratch, hipStream_t s) {
   const SortPlan p = sort_plan(n, groups);
   if (n <= kSmallRows) {
+    const int passes = (p.bits + kSmallBits - 1) / kSmallBits, bits = (p.bits + passes - 1) / passes;
     if (n <= 256)
-      hipLaunchKernelGGL(k_group_small<256>, dim3(1), dim3(256), 0, s, codes, (int)n, groups, p.passes,
-                         p.digit_bits, order, offsets);
+      hipLaunchKernelGGL(k_group_small<256>, dim3(1), dim3(256), 0, s, codes, (int)n, groups, passes, bits,
+                         order, offsets);
     else
-      hipLaunchKernelGGL(k_group_small<1024>, dim3(1), dim3(1024), 0, s, codes, (int)n, groups, p.passes,
-                         p.digit_bits, order, offsets);
+      hipLaunchKernelGGL(k_group_small<1024>, dim3(1), dim3(1024), 0, s, codes, (int)n, groups, passes, bits,
+                         order, offsets);
     return hipGetLastError();
   }
   char* ws = static_cast<char*>(scratch);

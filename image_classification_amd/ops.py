@@ -1132,7 +1132,7 @@ def label_logprobs(logits, labels=None, top=0, temperature=1.0):
     device = logits.device
     l64 = _check_labels(labels, n, device)
     stats = torch.empty((3, n), dtype=torch.float32, device=device)
-    logp = stats[2] if labels is not None else None
+    at = stats.data_ptr()
     top_logp = top_idx = None
     if top:
         top_logp = torch.empty((n, top), dtype=torch.float32, device=device)
@@ -1141,10 +1141,11 @@ def label_logprobs(logits, labels=None, top=0, temperature=1.0):
     nbytes = lib.ic_label_logprobs_scratch(n, v, t, top)
     scratch = _scratch(nbytes, device)
     rc = lib.ic_label_logprobs(_lib.handle(dev), _addr(logits), ld, n, v, t, _addr(labels), l64, inv, top,
-                               _addr(logp), _addr(stats[0]), _addr(stats[1]), _addr(top_logp),
-                               _addr(top_idx), _addr(scratch), nbytes, _stream_of(dev))
+                               at + 8 * n if labels is not None else None, at, at + 4 * n,
+                               _addr(top_logp), _addr(top_idx), _addr(scratch), nbytes, _stream_of(dev))
     _lib.check(rc, "ic_label_logprobs")
-    return logp, stats[0], stats[1], top_logp, top_idx
+    entropy, lse, logp = stats.unbind(0)
+    return (logp if labels is not None else None), entropy, lse, top_logp, top_idx
 
 
 def _check_vector(t, name, n, device):
