@@ -14,12 +14,12 @@ from .clustering import chisqr, intersection, kmeans_assign, kmeans_fit
 from .features import BagOfWords, SpatialBagOfWords, Vocabulary
 from .scene_functions import (compute_spatial_features, compute_spatial_features_from_xml,
                               compute_vocab_features)
-from .classifiers import KNNScikit
+from .classifiers import KNNScikit, SoftmaxClassifier
 from .robust_matching import RobustMatcher
 from .shortlist import KnnTrainer, fit_shortlist_index
 
 __all__ = ["ImageDesc", "vq", "kmeans2", "kmeans_assign", "kmeans_fit", "BagOfWords",
            "SpatialBagOfWords", "Vocabulary", "compute_vocab_features", "compute_spatial_features",
            "compute_spatial_features_from_xml", "KNNScikit", "KnnTrainer", "fit_shortlist_index", "RobustMatcher",
-           "intersection", "chisqr"]
+           "SoftmaxClassifier", "intersection", "chisqr"]
 __version__ = "0.1.0"

@@ -150,6 +150,33 @@ class HipBackend(object):
         return ops.ransac_homography(pts, offsets, n_iter, th, samples, seed, min_inliers,
                                      accept_mean_err, cv_rules)
 
+    # -- what is learned on top of the codes ----------------------------------------------------
+    def group_rows(self, codes, n_groups):
+        return ops.group_rows(codes, n_groups)
+
+    def grouped_matmul(self, x, w, offsets, order=None):
+        return ops.grouped_matmul(x, w, offsets, order)
+
+    def grouped_matmul_dx(self, dy, w, offsets, order=None):
+        return ops.grouped_matmul_dx(dy, w, offsets, order)
+
+    def grouped_matmul_dw(self, dy, x, offsets, order=None):
+        return ops.grouped_matmul_dw(dy, x, offsets, order)
+
+    def label_logprobs(self, logits, labels=None, top=0, temperature=1.0):
+        return ops.label_logprobs(logits, labels, top, temperature)
+
+    def label_logprobs_grad(self, logits, labels, lse, entropy, d_logp=None, d_entropy=None,
+                            temperature=1.0, out=None):
+        return ops.label_logprobs_grad(logits, labels, lse, entropy, d_logp, d_entropy, temperature,
+                                       out)
+
+    def adamw_states(self, params, bits=32):
+        return ops.adamw_states(params, bits)
+
+    def adamw_step(self, params, grads, exp_avg, exp_avg_sq, lr, step, **kwargs):
+        return ops.adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, **kwargs)
+
     def make_codebook(self, c_dev):
         """Wrap a device tensor produced by centroid_finalize as a codebook."""
         return _device.ResidentCodebook(c_dev, self.device)
