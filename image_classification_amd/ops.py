@@ -960,8 +960,8 @@ def _check_same_device(dev, *named):
             raise ValueError("%s lives on %s, expected %s" % (name, t.device, dev))
 
 
-def _scratch(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _scratch(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def group_rows(codes, n_groups):
@@ -976,11 +976,11 @@ def group_rows(codes, n_groups):
     dev = _dev_index(codes)
     codes = codes.contiguous()
     n = codes.shape[0]
-    order = torch.empty(n, dtype=torch.int32, device=codes.device)
-    offsets = torch.empty(n_groups + 1, dtype=torch.int64, device=codes.device)
+    order = torch.empty_like(codes)
+    offsets = codes.new_empty(n_groups + 1, dtype=torch.int64)
     lib = _lib.load()
     nbytes = lib.ic_group_rows_scratch(n, n_groups)
-    scratch = _scratch(nbytes, codes.device)
+    scratch = _scratch(nbytes, codes)
     rc = lib.ic_group_rows(_lib.handle(dev), _addr(codes), n, n_groups, _addr(order), _addr(offsets),
                            _addr(scratch), nbytes, _stream_of(dev))
     _lib.check(rc, "ic_group_rows")
@@ -1009,7 +1009,7 @@ def _check_group_matrices(w):
 def _result(out, out_dtype, shape, like, name):
     """(tensor, its type number) for a result of `shape`: `out`, or a new one."""
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or like.dtype, device=like.device)
+        out = like.new_empty(shape, dtype=out_dtype)
     elif tuple(out.shape) != tuple(shape) or out.device != like.device or \
             (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError("out must be a %s tensor on %s" % (tuple(shape), like.device))
@@ -1083,7 +1083,7 @@ def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
         raise ValueError("out must be contiguous")
     lib = _lib.load()
     nbytes = lib.ic_grouped_matmul_dw_scratch(n, groups, k, o, t)
-    scratch = _scratch(nbytes, x.device)
+    scratch = _scratch(nbytes, x)
     rc = lib.ic_grouped_matmul_dw(_lib.handle(dev), _addr(dy), ld_dy, _addr(x), ld_x, _addr(dw),
                                   _addr(offsets), _addr(order), n, groups, k, o, t, yt, _addr(scratch),
                                   nbytes, _stream_of(dev))
@@ -1131,15 +1131,15 @@ def label_logprobs(logits, labels=None, top=0, temperature=1.0):
     dev = _dev_index(logits)
     device = logits.device
     l64 = _check_labels(labels, n, device)
-    stats = torch.empty((3, n), dtype=torch.float32, device=device)
+    stats = logits.new_empty((3, n), dtype=torch.float32)
     at = stats.data_ptr()
     top_logp = top_idx = None
     if top:
-        top_logp = torch.empty((n, top), dtype=torch.float32, device=device)
-        top_idx = torch.empty((n, top), dtype=torch.int32, device=device)
+        top_logp = logits.new_empty((n, top), dtype=torch.float32)
+        top_idx = logits.new_empty((n, top), dtype=torch.int32)
     lib = _lib.load()
     nbytes = lib.ic_label_logprobs_scratch(n, v, t, top)
-    scratch = _scratch(nbytes, device)
+    scratch = _scratch(nbytes, logits)
     rc = lib.ic_label_logprobs(_lib.handle(dev), _addr(logits), ld, n, v, t, _addr(labels), l64, inv, top,
                                at + 8 * n if labels is not None else None, at, at + 4 * n,
                                _addr(top_logp), _addr(top_idx), _addr(scratch), nbytes, _stream_of(dev))
@@ -1176,7 +1176,7 @@ def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=Non
     if lse is None or (d_entropy is not None and entropy is None):
         raise ValueError("lse is needed, and entropy where d_entropy is given")
     if out is None:
-        out = torch.empty((n, v), dtype=logits.dtype, device=device)
+        out = logits.new_empty((n, v))
     elif out.dtype != logits.dtype or tuple(out.shape) != (n, v) or out.device != device:
         raise ValueError("out must be a %s %s tensor on %s" % (logits.dtype, (n, v), device))
     ld_out = _check_rows(out, "out")
