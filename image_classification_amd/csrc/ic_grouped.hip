@@ -1359,12 +1359,12 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
   for (int at = at0 + lane; at < at0 + span; at += 64) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     int64_t v = w + wave;
-    for (; v + 3 * kJoinWaves <= last; v += 4 * kJoinWaves) {
-      f32x4 q[4];
+    for (; v + 7 * kJoinWaves <= last; v += 8 * kJoinWaves) {
+      f32x4 q[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = piece(v + i * kJoinWaves, at);
+      for (int i = 0; i < 8; ++i) q[i] = piece(v + i * kJoinWaves, at);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += q[i];
+      for (int i = 0; i < 8; ++i) s += q[i];
     }
     for (; v <= last; v += kJoinWaves) s += piece(v, at);
     sums[wave][lane] = s;
@@ -1482,9 +1482,10 @@ DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned
     const int size = kTileSize[i];
     const double tiles = (double)((out + size - 1) / size) * ((k + size - 1) / size);
     const double line = ((double)(n / kk) + groups) * tiles;
-    // at least six units a workgroup (a piece costs its partial result and the start of a pipeline:
-    // the time of about six units as well)
-    double wgs = line / 6;
+    // at least four units a workgroup (5003 rows, 37 groups of 317 x 193 fp16, join included: 32.0 us with
+    // at least six, 28.9 with four, 31.9 with two); a piece costs its partial result and the start of a
+    // pipeline, the time of about six units
+    double wgs = line / 4;
     const double slots = (double)kCUs * kPerCu[i];
     wgs = wgs < 1 ? 1 : wgs > slots ? slots : wgs;
     const double t = (line / wgs + 6) * kPerCu[i] * size * size / rate[i];
@@ -1507,9 +1508,19 @@ hipError_t dw_launch(DwArgs a, hipStream_t s) {
   a.tiles = (int)tiles;
   hipLaunchKernelGGL((k_grouped_dw<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)a.wgs), dim3(WM * WN * 64),
                      (rows_lds<BM, BN>()), s, a);
-  if (a.wgs > 1)
-    hipLaunchKernelGGL((k_grouped_dw_join<T, BM, BN, WM, WN>), dim3(BM * BN / 4096, (unsigned)(a.wgs - 1)),
-                       dim3(kJoinWaves * 64), 0, s, a);
+  if (a.wgs > 1) {
+    // Workgroups a tile: one for each 4096 of its elements, and sixteen where a tile is cut into very many
+    // pieces, which are read one behind the other (100 000 rows, 1 group of 100 x 128 float32, 256
+    // pieces a tile: 467 -> 33 us).  Most workgroups find nothing to add, and that costs more than the
+    // wider split saves where tiles are cut into few (4096 rows, 16 groups of 512 x 512 bf16, both
+    // kernels: 23.7 us with one, 27.1 with four, 45.0 with sixteen), unless there are few workgroups
+    // in all (2000 rows, 8 groups of 64 x 128 float32: 15.5 with one, 12.5 with four).
+    constexpr int kEach = BM * BN / 4096;
+    const double pieces = (double)a.wgs / ((double)a.tiles * (double)a.g.groups);
+    const int split = pieces >= 32 ? 16 : (pieces >= 1.5 || a.wgs <= 64) && kEach * a.wgs <= 1024 ? 4 : 1;
+    hipLaunchKernelGGL((k_grouped_dw_join<T, BM, BN, WM, WN>),
+                       dim3(kEach * split, (unsigned)(a.wgs - 1)), dim3(kJoinWaves * 64), 0, s, a);
+  }
   return hipGetLastError();
 }
 
