@@ -1281,12 +1281,13 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   }
 }
 
-// Adds the pieces of the tile that workgroup y's run ends inside, if it also begins there (the
-// workgroups that lie wholly inside a tile leave it to the one where the tile begins).  A workgroup
-// here takes 1 / gridDim.x of the tile, 64 f32x4 a wave at a time.  Few pieces: each wave adds all of
-// them, in the order of the line.  Many (a long group under few tiles): the four waves share the
-// pieces of the same 64, every fourth each, and their sums are added in the waves' order.  Either way
-// the order depends on the sizes alone.
+// Adds the pieces of the tiles that are cut.  Workgroup row y stands for the end of run y of the line:
+// if it lies inside a tile, the rows y of all the ends inside that tile share its elements, 64 f32x4 at a
+// time, so that a tile cut into many pieces has as many workgroups to read them (100 000 rows, 1 group
+// of 100 x 128 float32, 256 pieces a tile: 467 us with one, 22 us).  Few pieces: each wave adds all
+// of its 64, in the order of the line.  Many: the four waves share the pieces of the same 64, every
+// fourth each, and their sums are added in the waves' order.  Either way the order depends on the sizes
+// alone.
 constexpr int kJoinWaves = 4;
 constexpr int kJoinFew = 8;
 template <typename T, int BM, int BN, int WM, int WN>
@@ -1297,19 +1298,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t w = blockIdx.y;
   const int64_t line = dw_line(a, kK);
-  const int64_t u0 = line * w / a.wgs, u1 = line * (w + 1) / a.wgs;
-  if (u1 >= line || u0 >= u1) return;
+  const int64_t u1 = line * (w + 1) / a.wgs;
+  if (u1 >= line) return;
   const DwPlace pl = dw_place(a, u1, kK, lane);
   const int64_t begin = u1 - pl.stage, end = begin + pl.stages;
-  if (pl.stage == 0 || begin < u0) return;
-  // the last workgroup with a unit of the tile: it holds unit end - 1
-  const int64_t last = (end * a.wgs - 1) / line;
+  if (pl.stage == 0 || begin < 0 || end > line) return;   // (outside only if the offsets do not ascend)
+  // the workgroups that hold the tile's first and last unit; the ends of all but the last lie inside
+  const int64_t first = ((begin + 1) * a.wgs - 1) / line, last = (end * a.wgs - 1) / line;
   constexpr int kTile = BM * BN / 4;
   const f32x4* part = reinterpret_cast<const f32x4*>(a.part);
-  // piece v (workgroup w + v) of the tile; an empty run holds none
+  // workgroup v's piece of the tile; an empty run holds none
   auto piece = [&](int64_t v, int at) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (v == w) s = part[(size_t)(2 * v + 1) * kTile + at];
+    if (v == first) s = part[(size_t)(2 * v + 1) * kTile + at];
     else if (line * v / a.wgs != line * (v + 1) / a.wgs) s = part[(size_t)(2 * v) * kTile + at];
     return s;
   };
@@ -1346,19 +1347,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
       }
     }
   };
-  const int span = kTile / (int)gridDim.x;
-  const int at0 = (int)blockIdx.x * span;
-  if (last - w < kJoinFew) {
-    for (int at = at0 + (int)threadIdx.x; at < at0 + span; at += kJoinWaves * 64) {
-      f32x4 s = piece(w, at);
-      for (int64_t v = w + 1; v <= last; ++v) s += piece(v, at);
+  const int mine = (int)((w - first) * gridDim.x + blockIdx.x);      // of this tile's workgroups
+  const int all = (int)((last - first) * gridDim.x);
+  if (last - first < kJoinFew) {
+    for (int at = (mine * kJoinWaves + wave) * 64 + lane; at < kTile; at += all * kJoinWaves * 64) {
+      f32x4 s = piece(first, at);
+      for (int64_t v = first + 1; v <= last; ++v) s += piece(v, at);
       put(at, s);
     }
     return;
   }
-  for (int at = at0 + lane; at < at0 + span; at += 64) {
+  for (int at = mine * 64 + lane; at < kTile; at += all * 64) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    int64_t v = w + wave;
+    int64_t v = first + wave;
     for (; v + 7 * kJoinWaves <= last; v += 8 * kJoinWaves) {
       f32x4 q[8];
 #pragma unroll
@@ -1509,17 +1510,13 @@ hipError_t dw_launch(DwArgs a, hipStream_t s) {
   hipLaunchKernelGGL((k_grouped_dw<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)a.wgs), dim3(WM * WN * 64),
                      (rows_lds<BM, BN>()), s, a);
   if (a.wgs > 1) {
-    // Workgroups a tile: one for each 4096 of its elements, and sixteen where a tile is cut into very many
-    // pieces, which are read one behind the other (100 000 rows, 1 group of 100 x 128 float32, 256
-    // pieces a tile: 467 -> 33 us).  Most workgroups find nothing to add, and that costs more than the
-    // wider split saves where tiles are cut into few (4096 rows, 16 groups of 512 x 512 bf16, both
-    // kernels: 23.7 us with one, 27.1 with four, 45.0 with sixteen), unless there are few workgroups
-    // in all (2000 rows, 8 groups of 64 x 128 float32: 15.5 with one, 12.5 with four).
+    // a workgroup for each 4096 elements and each end of a run; four where that makes few (2000 rows,
+    // 8 groups of 64 x 128 float32, both kernels: 14.8 -> 12.5 us; with many, most find nothing to add and
+    // more of them cost time: 4096 rows, 16 groups of 512 x 512 bf16, 23.7 us with one, 27.1 with four)
     constexpr int kEach = BM * BN / 4096;
-    const double pieces = (double)a.wgs / ((double)a.tiles * (double)a.g.groups);
-    const int split = pieces >= 32 ? 16 : (pieces >= 1.5 || a.wgs <= 64) && kEach * a.wgs <= 1024 ? 4 : 1;
-    hipLaunchKernelGGL((k_grouped_dw_join<T, BM, BN, WM, WN>),
-                       dim3(kEach * split, (unsigned)(a.wgs - 1)), dim3(kJoinWaves * 64), 0, s, a);
+    const int each = kEach * a.wgs <= 256 ? 4 * kEach : kEach;
+    hipLaunchKernelGGL((k_grouped_dw_join<T, BM, BN, WM, WN>), dim3(each, (unsigned)(a.wgs - 1)),
+                       dim3(kJoinWaves * 64), 0, s, a);
   }
   return hipGetLastError();
 }
