@@ -7,6 +7,8 @@ robust_matching.py, scene_functions.py) are thin layers over these functions.
 import array
 import collections
 import ctypes
+import itertools
+import operator
 import os
 import threading
 
@@ -34,7 +36,7 @@ def check_descriptor_dim(d, who):
 def _dev_index(t):
     if not t.is_cuda:
         raise ValueError("expected a CUDA tensor (there is no CPU path)")
-    return t.device.index if t.device.index is not None else torch.cuda.current_device()
+    return t.get_device()
 
 
 def _stream_ptr(device_index):
@@ -941,17 +943,19 @@ def _type_number(t, name):
 
 def _check_rows(t, name):
     """A matrix of unit-stride rows (a slice of a wider one is fine); returns its row stride."""
-    if t.dim() != 2:
-        raise ValueError("%s must be 2-D, got shape %s" % (name, tuple(t.shape)))
-    n, d = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError("%s must be 2-D, got shape %s" % (name, tuple(shape)))
+    n, d = shape
+    ld, step = t.stride()
     if n <= 1 or d == 0:
-        if d > 1 and t.stride(1) != 1:
+        if d > 1 and step != 1:
             raise ValueError("the elements of a row of %s must be adjacent" % name)
         return max(d, 1)
-    if (d > 1 and t.stride(1) != 1) or t.stride(0) < d:
+    if (d > 1 and step != 1) or ld < d:
         raise ValueError("%s must have adjacent elements in a row and rows that do not overlap "
-                         "(strides %s)" % (name, tuple(t.stride())))
-    return t.stride(0)
+                         "(strides %s)" % (name, (ld, step)))
+    return ld
 
 
 def _check_same_device(dev, *named):
@@ -987,29 +991,30 @@ def group_rows(codes, n_groups):
     return order, offsets
 
 
-def _check_groups(offsets, order, n, n_groups, device):
-    if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.shape[0] != n_groups + 1 \
-            or not offsets.is_contiguous():
+def _check_groups(offsets, order, n, n_groups, dev):
+    if offsets.dtype != torch.int64 or offsets.shape != (n_groups + 1,) or not offsets.is_contiguous():
         raise ValueError("offsets must be contiguous int64 [n_groups + 1] = [%d]" % (n_groups + 1))
-    if order is not None and (order.dtype != torch.int32 or order.dim() != 1 or order.shape[0] != n
-                              or not order.is_contiguous()):
+    if order is not None and (order.dtype != torch.int32 or order.shape != (n,) or not order.is_contiguous()):
         raise ValueError("order must be contiguous int32 with one entry per row")
-    _check_same_device(device, (offsets, "offsets"), (order, "order"))
+    if offsets.get_device() != dev or (order is not None and order.get_device() != dev):
+        raise ValueError("offsets and order must live on cuda:%d" % dev)
 
 
 def _check_group_matrices(w):
-    if w.dim() != 3 or not w.is_contiguous():
-        raise ValueError("w must be contiguous [n_groups, out, k], got shape %s" % (tuple(w.shape),))
-    if w.shape[0] < 1 or w.shape[1] < 1 or w.shape[2] < 1:
-        raise ValueError("w must not be empty, got shape %s" % (tuple(w.shape),))
-    if w.shape[0] > MAX_GROUPS:
-        raise ValueError("at most %d groups, got %d" % (MAX_GROUPS, w.shape[0]))
+    shape = w.shape
+    if len(shape) != 3 or not w.is_contiguous():
+        raise ValueError("w must be contiguous [n_groups, out, k], got shape %s" % (tuple(shape),))
+    if 0 in shape:
+        raise ValueError("w must not be empty, got shape %s" % (tuple(shape),))
+    if shape[0] > MAX_GROUPS:
+        raise ValueError("at most %d groups, got %d" % (MAX_GROUPS, shape[0]))
+    return shape
 
 
 def _result(out, out_dtype, shape, like, name):
     """(tensor, its type number) for a result of `shape`: `out`, or a new one."""
     if out is None:
-        out = like.new_empty(shape, dtype=out_dtype)
+        out = like.new_empty(shape) if out_dtype is None else like.new_empty(shape, dtype=out_dtype)
     elif tuple(out.shape) != tuple(shape) or out.device != like.device or \
             (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError("out must be a %s tensor on %s" % (tuple(shape), like.device))
@@ -1019,22 +1024,22 @@ def _result(out, out_dtype, shape, like, name):
 
 
 def _grouped_rows(fn_name, x, w, offsets, order, out, out_dtype, dx):
-    _check_group_matrices(w)
-    groups, o, k = w.shape
+    groups, o, k = _check_group_matrices(w)
     ld_x = _check_rows(x, "dy" if dx else "x")
     width, cols = (o, k) if dx else (k, o)
-    if x.shape[1] != width:
+    n, found = x.shape
+    if found != width:
         raise ValueError("dimension mismatch: rows have %d columns, w is %s"
                          % (x.shape[1], tuple(w.shape)))
     if x.dtype != w.dtype:
         raise ValueError("rows are %s, w is %s" % (x.dtype, w.dtype))
     t = _type_number(x, "rows")
     dev = _dev_index(x)
-    _check_same_device(x.device, (w, "w"))
-    n = x.shape[0]
-    _check_groups(offsets, order, n, groups, x.device)
+    if w.get_device() != dev:
+        raise ValueError("w lives on %s, expected %s" % (w.device, x.device))
+    _check_groups(offsets, order, n, groups, dev)
     y, yt = _result(out, out_dtype, (n, cols), x, "the result")
-    ld_y = _check_rows(y, "out")
+    ld_y = cols if out is None else _check_rows(y, "out")
     lib = _lib.load()
     rc = getattr(lib, fn_name)(_lib.handle(dev), _addr(x), ld_x, _addr(w), _addr(y), ld_y, _addr(offsets),
                                _addr(order), n, groups, k, o, t, yt, _stream_of(dev))
@@ -1077,7 +1082,7 @@ def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
     if not 1 <= groups <= MAX_GROUPS:
         raise ValueError("offsets must be int64 [n_groups + 1]")
     n, o, k = x.shape[0], dy.shape[1], x.shape[1]
-    _check_groups(offsets, order, n, groups, x.device)
+    _check_groups(offsets, order, n, groups, dev)
     dw, yt = _result(out, out_dtype, (groups, o, k), x, "the result")
     if not dw.is_contiguous():
         raise ValueError("out must be contiguous")
@@ -1190,6 +1195,9 @@ def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=Non
 # param_dtype and grad_dtype of struct ic_adamw_tensor (int32 each) as one little-endian word
 _ADAMW_TYPES = {(p, g): pt | gt << 32 for p, pt in _TYPE_NUMBER.items() for g, gt in _TYPE_NUMBER.items()}
 ADAMW_BLOCK = _lib.IC_ADAMW_BLOCK
+_numel, _get_device, _is_contiguous, _data_ptr = (
+    torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr)
+_dtype = operator.attrgetter("dtype")
 
 
 def adamw_state_size(params):
@@ -1243,20 +1251,19 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
             or exp_avg_sq.shape != exp_avg.shape or not exp_avg.is_contiguous() \
             or not exp_avg_sq.is_contiguous():
         raise ValueError("exp_avg and exp_avg_sq must be flat, contiguous and alike")
-    table = []      # struct ic_adamw_tensor, the two type numbers as one integer
-    at = 0
-    for p, g in zip(params, grads):
-        n = p.numel()
-        if g.numel() != n or p.get_device() != dev or g.get_device() != dev:
-            raise ValueError("a gradient must match its parameter, on the states' device")
-        if not (p.is_contiguous() and g.is_contiguous()):
-            raise ValueError("parameters and gradients must be contiguous")
-        try:
-            kinds = _ADAMW_TYPES[p.dtype, g.dtype]
-        except KeyError:
-            raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
-        table += (p.data_ptr(), g.data_ptr(), n, at, kinds)
-        at += -(-n // ADAMW_BLOCK) * ADAMW_BLOCK
+    # (column by column: a list of many small tensors is bound by what Python does for each)
+    sizes = list(map(_numel, params))
+    if list(map(_numel, grads)) != sizes or \
+            (set(map(_get_device, params)) | set(map(_get_device, grads))) - {dev}:
+        raise ValueError("a gradient must match its parameter, on the states' device")
+    if not (all(map(_is_contiguous, params)) and all(map(_is_contiguous, grads))):
+        raise ValueError("parameters and gradients must be contiguous")
+    try:
+        kinds = [_ADAMW_TYPES[pair] for pair in zip(map(_dtype, params), map(_dtype, grads))]
+    except KeyError:
+        raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
+    starts = list(itertools.accumulate([-(-n // ADAMW_BLOCK) * ADAMW_BLOCK for n in sizes], initial=0))
+    at = starts.pop()
     size = exp_avg.shape[0]
     if at != size:
         raise ValueError("the states have %d elements, these tensors need %d" % (size, at))
@@ -1265,7 +1272,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
         raise ValueError("uint8 states need contiguous float32 scales [2, %d]" % (size // ADAMW_BLOCK))
     if count == 0:
         return
-    table = array.array("q", table)
+    table = array.array("q", bytes(40 * count))     # struct ic_adamw_tensor, the two type numbers as one integer
+    for column, values in enumerate((map(_data_ptr, params), map(_data_ptr, grads), sizes, starts, kinds)):
+        table[column::5] = array.array("q", values)
     lr_t = step_t = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
