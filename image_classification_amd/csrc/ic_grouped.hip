@@ -704,6 +704,7 @@ struct RowsArgs {
   int cols;            // columns of the result
   int col_tiles;
   int y_f32, y_vec;    // y_vec: four columns can be stored at once
+  int64_t id0;         // the first tile of this launch
 };
 
 // A lane's sixteen results of one row, v[j] those of fragment j, in the 64 columns from c on; the row
@@ -759,7 +760,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   __shared__ unsigned box[3];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t id = a.id0 + xcd_run(blockIdx.x, gridDim.x);
   const int64_t tile = id / a.col_tiles;
   const int c0 = (int)(id % a.col_tiles) * BN;
   const Found f = find_group_once(a.g, tile, BM, wave, lane, box);
@@ -908,7 +909,7 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t id = a.id0 + xcd_run(blockIdx.x, gridDim.x);
   const int64_t tile = id / a.col_tiles;
   const int c0 = (int)(id % a.col_tiles) * BN;
   // (what still loads goes before what multiplies: 3 %)
@@ -992,8 +993,9 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
   __shared__ f32x4 sums[BYDEPTH ? 4 : 1][CF][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tile = (int64_t)blockIdx.x / a.col_tiles;
-  const int c0 = (int)(blockIdx.x % a.col_tiles) * kCols + (BYDEPTH ? 0 : wave * 16);
+  const int64_t id = a.id0 + blockIdx.x;
+  const int64_t tile = id / a.col_tiles;
+  const int c0 = (int)(id % a.col_tiles) * kCols + (BYDEPTH ? 0 : wave * 16);
   __shared__ unsigned box[3];
   const Found f = find_group_once(a.g, tile, 16, wave, lane, box);
   const int64_t e = f.e, o0 = f.o0, o1 = f.o1;
@@ -1382,14 +1384,24 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
 template <int BM, int BN>
 constexpr int rows_lds() { return 2 * (BM + BN) * kStageBytes + (BM > 128 ? BM : 128) * 4; }
 
+// `tiles` workgroups, in more than one launch where their threads pass 32 bits.
+template <typename Kernel>
+hipError_t launch_tiles(Kernel kernel, RowsArgs a, int64_t tiles, int threads, int lds, hipStream_t s) {
+  const int64_t most = 0xffffffffll / threads;
+  for (a.id0 = 0; a.id0 < tiles; a.id0 += most) {
+    const int64_t now = tiles - a.id0 < most ? tiles - a.id0 : most;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)now), dim3(threads), lds, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 hipError_t rows_launch(RowsArgs a, hipStream_t s) {
   a.col_tiles = (a.cols + BN - 1) / BN;
-  const int64_t grid = (a.g.n / BM + a.g.groups + 1) * a.col_tiles;
-  if (grid * (WM * WN * 64) > 0xffffffffll) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_grouped_rows<T, BM, BN, WM, WN, QALONG, ALIGNED>), dim3((unsigned)grid),
-                     dim3(WM * WN * 64), (rows_lds<BM, BN>()), s, a);
-  return hipGetLastError();
+  return launch_tiles(k_grouped_rows<T, BM, BN, WM, WN, QALONG, ALIGNED>, a,
+                      (a.g.n / BM + a.g.groups + 1) * a.col_tiles, WM * WN * 64, rows_lds<BM, BN>(), s);
 }
 
 // The tile sizes: workgroups of 256 x 256 (8 waves of 128 x 64, one workgroup a CU), 128 x 128 (4 waves
@@ -1421,10 +1433,7 @@ int pick_tile(int type, F tiles) {
 template <typename T, int NS, bool QALONG>
 hipError_t short_launch(RowsArgs a, hipStream_t s) {
   a.col_tiles = (a.cols + 63) / 64;
-  const int64_t grid = (a.g.n / 64 + a.g.groups + 1) * a.col_tiles;
-  if (grid * 256 > 0xffffffffll) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_grouped_short<T, NS, QALONG>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_tiles(k_grouped_short<T, NS, QALONG>, a, (a.g.n / 64 + a.g.groups + 1) * a.col_tiles, 256, 0, s);
 }
 
 // Up to 8 rows a group on average (or hardly any rows at all), forward.
@@ -1432,11 +1441,9 @@ template <typename T>
 hipError_t few_launch(RowsArgs a, hipStream_t s) {
   const bool by_depth = a.depth >= 512;
   a.col_tiles = by_depth ? (a.cols + 31) / 32 : (a.cols + 63) / 64;
-  const int64_t grid = (a.g.n / 16 + a.g.groups + 1) * a.col_tiles;
-  if (grid * 256 > 0xffffffffll) return hipErrorInvalidValue;
-  if (by_depth) hipLaunchKernelGGL((k_grouped_few<T, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_grouped_few<T, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  return hipGetLastError();
+  const int64_t tiles = (a.g.n / 16 + a.g.groups + 1) * a.col_tiles;
+  return by_depth ? launch_tiles(k_grouped_few<T, true>, a, tiles, 256, 0, s)
+                  : launch_tiles(k_grouped_few<T, false>, a, tiles, 256, 0, s);
 }
 
 template <typename T, bool QALONG>

@@ -41,7 +41,7 @@ struct AdamArgs {
   double lr, b1, b2, omb1, omb2, eps, wd, c1, c2;   // omb = 1 - b; c = 1 - b^t
   double lr1, root2;         // lr / c1, sqrt(1 / c2): the usual step has no division in the kernel
   const float* lr_dev;       // not NULL: the learning rate is read here
-  const int64_t* step_dev;   // not NULL: t is read here
+  const int64_t* step_dev;   // not NULL: t is read here; below 1 counts as 1
   float grad_scale;
 };
 
@@ -111,7 +111,7 @@ __device__ __forceinline__ void corrections(const AdamArgs& a, double* lr, doubl
     if (a.lr_dev) *lr = (double)*a.lr_dev;
     double c1 = a.c1;
     if (a.step_dev) {
-      const int64_t t = *a.step_dev;
+      const int64_t t = *a.step_dev < 1 ? 1 : *a.step_dev;   // (counted from 1)
       c1 = 1.0 - power(a.b1, t);
       *root2 = sqrt(1.0 / (1.0 - power(a.b2, t)));
     }

@@ -968,6 +968,31 @@ def _scratch(nbytes, like):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
+def _columns_of(t):
+    """(first byte, bytes from row to row, bytes of a row, one behind the last byte) of a matrix of rows;
+    of any other contiguous tensor as one row."""
+    size = t.element_size()
+    if t.dim() == 2 and t.shape[0] > 1:
+        ld, width = t.stride(0) * size, t.shape[1] * size
+        return t.data_ptr(), ld, width, t.data_ptr() + (t.shape[0] - 1) * ld + width
+    return t.data_ptr(), 0, t.numel() * size, t.data_ptr() + t.numel() * size
+
+
+def _check_apart(out, *inputs):
+    """`out` may share no memory with what the same launch reads; different columns of one wide matrix
+    are apart."""
+    a, ld, width, a_end = _columns_of(out)
+    for t in inputs:
+        b, ld_t, width_t, b_end = _columns_of(t)
+        if a_end <= b or b_end <= a or width == 0 or width_t == 0:
+            continue
+        if ld and ld == ld_t:
+            gap = (b - a) % ld
+            if gap >= width and gap + width_t <= ld:
+                continue
+        raise ValueError("out must share no memory with the inputs")
+
+
 def group_rows(codes, n_groups):
     """(order int32 [n], offsets int64 [n_groups + 1]): the rows of each code one after the other,
     in their order; group g is order[offsets[g]:offsets[g + 1]].  Rows whose code is outside
@@ -1039,7 +1064,10 @@ def _grouped_rows(fn_name, x, w, offsets, order, out, out_dtype, dx):
         raise ValueError("w lives on %s, expected %s" % (w.device, x.device))
     _check_groups(offsets, order, n, groups, dev)
     y, yt = _result(out, out_dtype, (n, cols), x, "the result")
-    ld_y = cols if out is None else _check_rows(y, "out")
+    ld_y = cols
+    if out is not None:
+        ld_y = _check_rows(y, "out")
+        _check_apart(y, x, w)
     lib = _lib.load()
     rc = getattr(lib, fn_name)(_lib.handle(dev), _addr(x), ld_x, _addr(w), _addr(y), ld_y, _addr(offsets),
                                _addr(order), n, groups, k, o, t, yt, _stream_of(dev))
@@ -1051,8 +1079,8 @@ def grouped_matmul(x, w, offsets, order=None, out=None, out_dtype=None):
     """y[i] = w[g] @ x[i] for every row i of group g, zeros for rows of no group.
 
     x [n, k], w [n_groups, out, k] of the same type (float32, bfloat16, float16; sums are float32);
-    (order, offsets) as group_rows returns them -- order=None: the rows lie group by group, row i in
-    group g when offsets[g] <= i < offsets[g + 1].  Returns y [n, out] of x's type or `out_dtype`
+    (order, offsets) as group_rows returns them (offsets ascend from 0 to at most n) -- order=None: the
+    rows lie group by group, row i in group g when offsets[g] <= i < offsets[g + 1].  Returns y [n, out] of x's type or `out_dtype`
     (float32); `out`: a tensor to write to, which must share no memory with x or w.  Rows may lie
     apart (a column slice of a wider matrix); order must name every row once."""
     return _grouped_rows("ic_grouped_matmul", x, w, offsets, order, out, out_dtype, False)
@@ -1086,6 +1114,8 @@ def grouped_matmul_dw(dy, x, offsets, order=None, out=None, out_dtype=None):
     dw, yt = _result(out, out_dtype, (groups, o, k), x, "the result")
     if not dw.is_contiguous():
         raise ValueError("out must be contiguous")
+    if out is not None:
+        _check_apart(dw, dy, x)
     lib = _lib.load()
     nbytes = lib.ic_grouped_matmul_dw_scratch(n, groups, k, o, t)
     scratch = _scratch(nbytes, x)
@@ -1185,6 +1215,8 @@ def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=Non
     elif out.dtype != logits.dtype or tuple(out.shape) != (n, v) or out.device != device:
         raise ValueError("out must be a %s %s tensor on %s" % (logits.dtype, (n, v), device))
     ld_out = _check_rows(out, "out")
+    if out.data_ptr() != logits.data_ptr() or ld_out != ld:
+        _check_apart(out, logits)
     rc = _lib.load().ic_label_logprobs_grad(
         _lib.handle(dev), _addr(logits), ld, n, v, t, _addr(labels), l64, inv, _addr(lse), _addr(entropy),
         _addr(d_logp), _addr(d_entropy), _addr(out), ld_out, _stream_of(dev))
@@ -1233,7 +1265,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
     exp_avg_sq, scales: flat states as adamw_states makes them, for this list in this order.  With
     uint8 states, ADAMW_BLOCK elements share a scale (adamw_state_values gives their values).
     lr: a number, or a float32 device tensor of one element; step: a number counted from 1, or an
-    int64 device tensor of one element -- a captured step reads them at every replay."""
+    int64 device tensor of one element (a value below 1 counts as 1) -- a captured step reads them at
+    every replay."""
     count = len(params)
     if len(grads) != count:
         raise ValueError("%d parameters, %d gradients" % (count, len(grads)))

@@ -399,8 +399,9 @@ typedef struct ic_adamw_tensor {
  *   tensors [count] (HOST).  state_bits 32: exp_avg, exp_avg_sq [state_elements] f32.  state_bits 8:
  *   they are codes [state_elements] uint8 with scales [2][state_elements / IC_ADAMW_BLOCK] f32
  *   (all zeros to begin with); ic_adamw_state_values gives the values that they stand for.
- *   lr_dev (f32) and step_dev (int64), device, are read instead of lr and step when they are not NULL
- *   (a captured step then follows them).  step >= 1.  No two tensors may share memory. */
+ *   lr_dev (f32) and step_dev (int64; a value below 1 counts as 1), device, are read instead of lr and
+ *   step when they are not NULL (a captured step then follows them).  step >= 1.  No two tensors may
+ *   share memory. */
 int ic_adamw_step(void* handle, const ic_adamw_tensor* tensors, int64_t count, int state_bits,
                   void* exp_avg, void* exp_avg_sq, float* scales, int64_t state_elements, double lr,
                   const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,

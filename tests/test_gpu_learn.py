@@ -251,6 +251,46 @@ def test_bad_orders_and_offsets_stay_inside():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, groups, k, out", [(9000, 1, 128, 100), (20_000, 2, 16, 24), (7001, 1, 33, 65)])
+def test_tiles_cut_into_many_pieces(n, groups, k, out, t):
+    # few tiles under many rows: a tile's pieces come from dozens of workgroups; the bits repeat
+    codes, x, dy, w = group_case(n, groups, k, out, t, 11)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    a = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+    close(a, *ref["dw"], n, "dw")
+    b = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+    assert torch.equal(a, b)
+
+
+def test_results_share_no_memory_with_the_inputs():
+    codes, x, dy, w = group_case(64, 2, 16, 16, torch.float32, 4)
+    wide = torch.zeros(64, 48, device=DEV)
+    wide[:, :16] = x
+    xs, w = wide[:, :16], w.to(DEV)
+    order, offsets = ops.group_rows(codes.to(DEV), 2)
+    y = ops.grouped_matmul(xs, w, offsets, order, out=wide[:, 16:32])          # other columns: fine
+    assert torch.equal(y, ops.grouped_matmul(x.to(DEV), w, offsets, order))
+    for out in (wide[:, 8:24], wide[:, :16]):
+        with pytest.raises(ValueError, match="share no memory"):
+            ops.grouped_matmul(xs, w, offsets, order, out=out)
+        with pytest.raises(ValueError, match="share no memory"):
+            ops.grouped_matmul_dx(xs, w, offsets, order, out=out)
+    flat = torch.zeros(64 * 16, device=DEV)
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.grouped_matmul_dw(flat.view(64, 16), x.to(DEV), offsets, order, out=flat[:512].view(2, 16, 16))
+    logits = torch.randn(8, 40, device=DEV)
+    labels = torch.zeros(8, dtype=torch.int32, device=DEV)
+    logp, h, lse, _, _ = ops.label_logprobs(logits[:, :32], labels)
+    ones = torch.ones(8, device=DEV)
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.label_logprobs_grad(logits[:, :32], labels, lse, h, ones, out=logits[:, 4:36])
+    want = ops.label_logprobs_grad(logits[:, :32], labels, lse, h, ones)
+    got = ops.label_logprobs_grad(logits[:, :32], labels, lse, h, ones, out=logits[:, :32])
+    assert torch.equal(got, want)
+
+
 # -- label_logprobs ---------------------------------------------------------------------------------------
 def score_reference(z, labels, temperature):
     z = z.double() / temperature
@@ -587,6 +627,22 @@ def test_adamw_many_tensors_and_device_scalars(bits):
         assert float((p - q).abs().max()) <= 4 * U * float(p.abs().max() + 0.02)
     rp, rm, rv = flat_f64([t.cpu() for t in ps2]) * 0, 0, 0
     assert rp.size == a[0].numel()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_a_device_step_below_one_counts_as_one(bits):
+    results = []
+    for step in (1, torch.tensor([0], device=DEV), torch.tensor([-7], device=DEV)):
+        p = [torch.linspace(-1, 1, 700, device=DEV)]
+        g = [torch.linspace(2, -3, 700, device=DEV)]
+        m, v, scales = ops.adamw_states(p, bits)
+        ops.adamw_step(p, g, m, v, lr=0.5, step=step, scales=scales)
+        results.append(p[0])
+    assert bool(torch.isfinite(results[0]).all())
+    # (the corrections are worked out on the host for a number, on the device for a tensor)
+    for q in results[1:]:
+        assert float((q - results[0]).abs().max()) <= 4 * U * 2.0
+    assert torch.equal(results[1], results[2])
 
 
 @pytest.mark.parametrize("bits", [32, 8])

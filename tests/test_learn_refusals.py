@@ -166,3 +166,64 @@ def test_the_line_of_a_weight_gradient_is_covered_once(seed):
         joined.add((e, t))
     assert not pieces and not (whole & joined)
     assert whole | joined == {(e, t) for e in range(groups) for t in range(tiles)}
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_the_ends_inside_a_cut_tile_share_its_join(seed):
+    # the join's workgroups: every element of a cut tile is taken by exactly one of the ends that lie
+    # inside the tile, whatever the runs (empty ones among them), and all agree on the tile's workgroups
+    import numpy as np
+    rng = np.random.default_rng(100 + seed)
+    kk = int(rng.choice([32, 64]))
+    groups, tiles, wgs = int(rng.integers(1, 6)), int(rng.integers(1, 4)), int(rng.integers(2, 60))
+    each, chunks = int(rng.choice([1, 4, 16])), 16
+    sizes = rng.choice([0, 1, kk, kk + 1, int(rng.integers(0, 4000))], groups)
+    off = [int(o) for o in np.concatenate([[0], np.cumsum(sizes)])]
+    first = [off[e] // kk + e for e in range(groups + 1)]
+    line = first[groups] * tiles
+    run_of = {}
+    for w in range(wgs):
+        for u in range(line * w // wgs, line * (w + 1) // wgs):
+            run_of[u] = w
+    begins, u = {}, 0
+    for e in range(groups):
+        stages = off[e + 1] // kk + 1 - off[e] // kk
+        for _ in range(tiles):
+            for q in range(u, u + stages):
+                begins[q] = (u, u + stages)
+            u += stages
+    assert u == line
+    taken = {}
+    for w in range(wgs - 1):
+        u1 = line * (w + 1) // wgs
+        if u1 >= line or begins[u1][0] == u1:
+            continue
+        begin, end = begins[u1]
+        lo, hi = ((begin + 1) * wgs - 1) // line, (end * wgs - 1) // line
+        assert lo == run_of[begin] and hi == run_of[end - 1] and lo <= w < hi
+        for x in range(each):
+            mine = (w - lo) * each + x
+            assert 0 <= mine < (hi - lo) * each
+            for at in range(mine, chunks, (hi - lo) * each):
+                assert (begin, at) not in taken
+                taken[begin, at] = w
+    cut = {b for b, end in begins.values() if run_of[b] != run_of[end - 1]}
+    assert set(taken) == {(b, at) for b in cut for at in range(chunks)}
+
+
+def test_memory_that_is_shared():
+    wide = z(6, 40)
+    apart = [(wide[:, :8], wide[:, 8:20]), (wide[:, 30:], wide[:, :30]), (wide[:3], wide[3:]),
+             (z(4, 8), z(4, 8)), (wide[0:1, :8], wide[0:1, 8:]), (z(0, 8), z(0, 8))]
+    for a, b in apart:
+        ops._check_apart(a, b)
+        ops._check_apart(b, a)
+    shared = [(wide, wide), (wide[:, :8], wide[:, 7:20]), (wide[:4], wide[3:]), (wide[:, 4:12], wide),
+              (z(30).as_strided((4, 3), (6, 1)), None)]
+    flat = shared.pop()[0]
+    shared.append((flat, flat.as_strided((3, 3), (7, 1))))      # other row strides: refused unless apart
+    for a, b in shared:
+        with pytest.raises(ValueError, match="share no memory"):
+            ops._check_apart(a, b)
+        with pytest.raises(ValueError, match="share no memory"):
+            ops._check_apart(b, a)
