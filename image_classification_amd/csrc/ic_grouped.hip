@@ -60,8 +60,9 @@ __device__ __forceinline__ unsigned rank_in_wave(Count* cnt, unsigned d, bool in
   return old + __popcll(same & below);
 }
 
-// Few rows: one workgroup, everything in LDS (bitonic sorting took 18.6 us for 1000 rows: 66 steps of a
-// barrier each).
+// Few rows: one workgroup, everything in LDS.  Bound by latency: 6.6 us for 1000 rows of 1000 groups
+// (bitonic sorting took 18.6 us: 66 steps of a barrier each), 4.0 for 16 rows of 64; up to 8192 rows one
+// such workgroup is faster than the launches below (5003 rows of 37 groups: 8.3 us against 23).
 constexpr int kSmallRows = 8192, kSmallBits = 8;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restrict__ codes, int n,
@@ -165,6 +166,8 @@ __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restri
 }
 
 // Many rows: a pass over a digit is three launches (counts per block of rows, prefixes, scatter).
+// Bound by the launches' latency: 42 000 rows of 21 groups take 5 + 5 + 8 us and the offsets 5, a
+// million rows of 10 000 groups (two passes) 52 us in all, of which 12 MB read and written would be 5.
 constexpr int kSortRows = 4096;     // rows of a workgroup
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
@@ -745,6 +748,14 @@ __device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, in
 }
 
 // forward (QALONG: W_g [cols][depth]) and dx (W_g [depth][cols])
+// 65 536 rows, 16 groups of 2048 x 2048 bf16, 256 x 256 tiles: 600 us forward and 625 dx, 920 and 880
+// TFLOP/s (a large library product reaches 1280).  The products alone, with neither loads nor LDS reads,
+// take 440 us (the clock falls to about 2.2 GHz under them, and some 2100 tiles make 9 rounds of 256 CUs
+// where 8.2 would do); the LDS reads cost 80 us more, the loads as much again.
+// 42 000 rows, 21 groups, 1000 -> 256 float32: 239 us forward (64 x 64 tiles) and 245 dx (128 x 128), 90
+// TFLOP/s where a large library product reaches 154; the products alone 190 and 220 us, because 2.6 and
+// 5.5 rounds of the card take 3 and 6.
+// Rows that are not 16-byte pieces (ALIGNED false): 5003 rows, 37 groups, 193 -> 317 fp16 13 us each.
 template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
@@ -898,7 +909,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 // of 64 x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
 // goes to LDS, shared by the four waves; each wave's 16 rows go straight to the registers that the
 // products take them from.  One barrier, one memory latency behind the search for the group.
-// (1M rows x 128 float32, 10 000 groups of 64 x 128: staged like the longer ones 355 us.)
+// 1M rows x 128 float32, 10 000 groups of 64 x 128: 343 us, 3.2 TB/s of rows, matrices and results and
+// 48 TFLOP/s (staged like the longer ones 355 us).  Neither is at its limit (memory 0.21 ms, products
+// 0.11 ms): a workgroup loads, multiplies and stores once, and what five of them a CU overlap is part
+// of it.
 // Five workgroups share a CU: 32 KB of LDS and 96 registers each.
 template <typename T, int NS, bool QALONG>
 __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
@@ -983,6 +997,8 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
 // shared, so nothing goes through LDS on the way.  BYDEPTH: the four waves share the depth of the same
 // 32 columns and add their sums in LDS, in wave order; otherwise (short rows) each wave takes 16 columns
 // of its own.  A lane's granules of a chunk are neighbours (32 bytes), four lanes read 128 bytes.
+// 16 rows, 64 groups of 2048 x 2048 bf16 (about 14 of them met, 118 MB): 28.8 us, 4.1 TB/s (through LDS 36 us);
+// 1000 rows, 1000 groups of 64 x 128 float32 (21 MB): 10.6 us.
 template <typename T, bool BYDEPTH>
 __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
   constexpr int kV = Elem<T>::kVec;
@@ -1077,6 +1093,8 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
 // stored at once; the pieces of one that is cut go to float32 partial results -- at most two a
 // workgroup: of the tile its run begins inside (number 2 w) and of the one it ends inside (2 w + 1) --
 // and k_grouped_dw_join adds them in the order of the line.
+// 65 536 rows, 16 groups of 2048 x 2048 bf16: 737 us and 41 to join, 710 TFLOP/s together; without loads
+// 510 us, without LDS reads either 475.  42 000 rows, 21 groups of 256 x 1000 float32: 237 + 21 us.
 struct DwArgs {
   const void* dy;
   const void* x;
@@ -1286,7 +1304,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
 // Adds the pieces of the tiles that are cut.  Workgroup row y stands for the end of run y of the line:
 // if it lies inside a tile, the rows y of all the ends inside that tile share its elements, 64 f32x4 at a
 // time, so that a tile cut into many pieces has as many workgroups to read them (100 000 rows, 1 group
-// of 100 x 128 float32, 256 pieces a tile: 467 us with one, 22 us).  Few pieces: each wave adds all
+// of 100 x 128 float32, 256 pieces a tile: 22 us, 467 with one).  Few pieces: each wave adds all
 // of its 64, in the order of the line.  Many: the four waves share the pieces of the same 64, every
 // fourth each, and their sums are added in the waves' order.  Either way the order depends on the sizes
 // alone.

@@ -19,7 +19,8 @@
 // given away both of its two looks for its next ones in its part of the row again (seldom: three
 // of the t best in one of 64 lanes).
 //
-// What bounds it: reading the row once.  See the figures at each kernel.
+// What bounds it: reading the row once, and the instructions that rank it; the figures stand at each
+// kernel.
 #include "ic_wave.h"
 
 namespace ic {
@@ -251,7 +252,8 @@ template <> __device__ __forceinline__ float value16<f16_t>(unsigned k) {
 template <> __device__ __forceinline__ float value16<float>(unsigned) { return 0.0f; }
 
 // Rows of up to 64 * NC granules: one wave a row, the row stays in registers between the maximum,
-// the sums and the ranking.
+// the sums and the ranking.  100 000 rows of 1000 bf16 scores with the best five: 87 us, 2.4 TB/s: bound by
+// its vector instructions (reading the row is 40 us; ranked as 32-bit words with an index each 111 us).
 template <typename T, int NC, bool TOP>
 __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
   constexpr int kV = Elem<T>::kVec;
@@ -375,7 +377,9 @@ constexpr int kPieceThreads = 256;
 constexpr int kPieceWaves = kPieceThreads / 64;
 
 // Longer rows: a workgroup streams one of `pieces` pieces of a row (pieces > 1 where there are too
-// few rows to fill the card; k_score_join then joins them).
+// few rows to fill the card; k_score_join then joins them).  4096 rows of 65 536 bf16 scores: 125 to 138 us,
+// 3.9 to 4.3 TB/s (a sum over 1 GiB by the library reads 3.9); 8 rows of 65 536 float32 scores with the
+// best ten: 8.8 us and 4.6 for the join, latency.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kPieceThreads) void k_score_pieces(ScoreArgs a, int pieces,
                                                                 unsigned* part) {
@@ -558,7 +562,8 @@ struct GradArgs {
 // dL/dx_j = ( g (delta_{j,label} - p_j) - h p_j (log p_j + H) ) / T with g = dL/dlogp (0 for a row
 // without a label) and h = dL/dH.  One read of the scores, one write of the gradient (out may be
 // the scores themselves: an element is read before it is written, by the same lane).  A row of few
-// granules is taken by 2^lanes_log2 lanes, 256 >> lanes_log2 rows a workgroup.
+// granules is taken by 2^lanes_log2 lanes, 256 >> lanes_log2 rows a workgroup.  4096 rows of 65 536 bf16
+// scores: 190 us, 5.7 TB/s (a copy of 1 GiB: 5.2): bound by memory.
 template <typename T>
 __global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, int span) {
   constexpr int kV = Elem<T>::kVec;
