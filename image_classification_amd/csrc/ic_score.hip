@@ -15,9 +15,9 @@
 //
 // The best alternatives: values are ranked as integers (a monotone map of the float bits, -0 as
 // +0), ties to the lowest index.  A lane keeps its own two best while it streams; the t best of a
-// wave are then t rounds of a 64-lane maximum, in which only the winner moves on.  A lane that has
-// given away both of its two looks for its next ones in its part of the row again (seldom: three
-// of the t best in one of 64 lanes).
+// wave are then t rounds of a 64-lane maximum, in which only the winner moves on.  Where a lane has
+// given away both of its two, its part of the row is looked through again for what follows (and, where
+// the row is in registers, every lane's for its best two of the rest: about every tenth round).
 //
 // What bounds it: reading the row once, and the instructions that rank it; the figures stand at each
 // kernel.
@@ -108,8 +108,8 @@ __device__ __forceinline__ int best_lane(unsigned k, int i, unsigned* kb) {
   return __builtin_amdgcn_readfirstlane(__ffsll(who) - 1);
 }
 
-// t rounds over the lanes' lists; lane r returns with the r-th best.  refill(lane, k, i) gives the
-// lane's next element after (k, i) to that lane.
+// t rounds over the lanes' lists; lane r returns with the r-th best.  refill(w, k, i, b, left), called where
+// lane w has given away both of its two, brings the lists up to date with (k, i) taken last.
 template <typename Refill>
 __device__ __forceinline__ void take_best(Best2 b, int t, int lane, unsigned* out_k, int* out_i,
                                           Refill refill) {
@@ -131,14 +131,7 @@ __device__ __forceinline__ void take_best(Best2 b, int t, int lane, unsigned* ou
       --left;
     }
     if (r + 1 < t && __builtin_amdgcn_readlane(left, w) == 0) {
-      unsigned nk;
-      int ni;
-      refill(w, kb, ib, &nk, &ni);
-      if (lane == w) {
-        b.k1 = nk;
-        b.i1 = ni;
-        left = 1;
-      }
+      refill(w, kb, ib, &b, &left);
     }
   }
   *out_k = rk;
@@ -328,15 +321,15 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
         const unsigned kb = wave_max_u32(k1);
         mine = lane == r ? kb : mine;
         const bool won = k1 == kb;
-        // a lane that gives away its second looks for its next two
+        // where a lane gives away its second, all look for their best two of what is left
         const bool spent = won && k2 == 0u;
         k1 = won ? k2 : k1;
         k2 = won ? 0u : k2;
         if (r + 1 < a.top && __ballot(spent)) {
           unsigned n1, n2;
           best2(kb, &n1, &n2);
-          k1 = spent ? n1 : k1;
-          k2 = spent ? n2 : k2;
+          k1 = n1;
+          k2 = n2;
         }
       }
       ri = 65535 - (int)(mine & 0xffffu);
@@ -359,15 +352,93 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
         }
         return q;
       };
-      take_best(best2(0u, 0, true), a.top, lane, &rk, &ri,
-                [&](int, unsigned k0, int i0, unsigned* nk, int* ni) {
-                  const Best2 q = best2(k0, i0, false);
-                  *nk = q.k1;
-                  *ni = q.i1;
-                });
+      take_best(best2(0u, 0, true), a.top, lane, &rk, &ri, [&](int, unsigned k0, int i0, Best2* b, int* left) {
+        *b = best2(k0, i0, false);     // all lanes' best two of what is left
+        *left = 2;
+      });
     }
   }
   write_row<T>(a, row, xr, st, lane, rk, ri);
+}
+
+// Rows of up to 64 scores: 2^LOG lanes a row, a score a lane, so that a wave takes up to 16 rows; what a
+// row's lanes reduce is left in all of them.
+template <int X>
+__device__ __forceinline__ unsigned from_lane_xor(unsigned v) {
+  if constexpr (X == 1) return dpp_u32<0xb1>(v, v);                     // quad_perm 1 0 3 2
+  else if constexpr (X == 2) return dpp_u32<0x4e>(v, v);                // quad_perm 2 3 0 1
+  else if constexpr (X == 4) {
+    const unsigned w = dpp_u32<0x141>(v, v);                            // row_half_mirror: xor 7
+    return dpp_u32<0x1b>(w, w);                                         // quad_perm 3 2 1 0: xor 3
+  } else if constexpr (X == 8) return dpp_u32<0x128>(v, v);             // row_ror 8
+  else return (unsigned)__shfl_xor((int)v, X, 64);
+}
+__device__ __forceinline__ uint64_t pair64(unsigned high, unsigned low) { return (uint64_t)high << 32 | low; }
+template <int X>
+__device__ __forceinline__ uint64_t from_lane_xor(uint64_t v) {
+  return pair64(from_lane_xor<X>((unsigned)(v >> 32)), from_lane_xor<X>((unsigned)v));
+}
+template <int X, int L, typename F>
+__device__ __forceinline__ float lanes_fold(float v, F op) {
+  if constexpr (X < L) {
+    v = op(v, __uint_as_float(from_lane_xor<X>(__float_as_uint(v))));
+    return lanes_fold<2 * X, L>(v, op);
+  } else {
+    return v;
+  }
+}
+// Bitonic sort of the keys of L lanes, descending: blocks of K lanes, partners J apart.
+template <int K, int J, int L, typename Key>
+__device__ __forceinline__ Key lanes_sort(Key k, int lane) {
+  if constexpr (K > L) {
+    return k;
+  } else {
+    const Key other = from_lane_xor<J>(k);
+    const bool larger = ((lane & J) == 0) == ((lane & K) == 0 || K == L);
+    k = (k > other) == larger ? k : other;     // (equal keys: either)
+    if constexpr (J > 1) return lanes_sort<K, J / 2, L>(k, lane);
+    else return lanes_sort<2 * K, K, L>(k, lane);
+  }
+}
+
+// Bound by instructions and, up to a few thousand rows, by latency: 54 184 rows of 18 bf16 scores with the best
+// eleven 14 us (a wave a row 58), 50 000 rows of 60 float32 with the best thirty 28 us (99).
+template <typename T, int LOG, bool TOP>
+__global__ __launch_bounds__(256) void k_score_small(ScoreArgs a) {
+  constexpr int L = 1 << LOG;
+  const int lane = threadIdx.x & 63, sub = lane & (L - 1);
+  int64_t row = a.row0 + (int64_t)blockIdx.x * (256 / L) + (threadIdx.x >> LOG);
+  const bool ours = row < a.n;
+  if (!ours) row = a.n - 1;          // (its lanes take part and write nothing)
+  const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
+  const bool in = sub < a.v;
+  const float x = in ? Elem<T>::load(xr + sub) : -__builtin_inff();
+  const float c = a.inv_t * kLog2e;
+  auto most = [](float p, float q) { return fmaxf(p, q); };
+  auto sum = [](float p, float q) { return p + q; };
+  Stats st;
+  st.m = lanes_fold<1, L>(fmaxf(x, kLowest), most);
+  const float d = x - st.m;
+  const float e = __builtin_amdgcn_exp2f(d * c);
+  st.s = lanes_fold<1, L>(e, sum);
+  st.u = lanes_fold<1, L>(e * fmaxf(d, kFar), sum);
+  unsigned rk = 0;
+  int ri = -1;
+  if constexpr (TOP) {
+    // keys differ, ties rank by index; lanes behind the row come last
+    if constexpr (sizeof(T) == 2) {
+      const unsigned bits = reinterpret_cast<const unsigned short*>(xr)[in ? sub : 0];
+      const unsigned r16 = x != x ? 0xffffu : rank16x2<T>(bits) & 0xffffu;
+      const unsigned key = lanes_sort<2, 1, L>(in ? r16 << 16 | (unsigned)(65535 - sub) : 0u, lane);
+      ri = 65535 - (int)(key & 0xffffu);
+      rk = rank_of(value16<T>(key >> 16));
+    } else {
+      const uint64_t key = lanes_sort<2, 1, L>(in ? pair64(rank_of(x), 0xffffffffu - (unsigned)sub) : (uint64_t)0, lane);
+      ri = (int)(0xffffffffu - (unsigned)key);
+      rk = (unsigned)(key >> 32);
+    }
+  }
+  if (ours) write_row<T>(a, row, xr, st, sub, rk, ri);
 }
 
 // A piece of a row as k_score_pieces leaves it: 4 words, then top (rank, index) pairs
@@ -434,7 +505,7 @@ __global__ __launch_bounds__(kPieceThreads) void k_score_pieces(ScoreArgs a, int
     unsigned rk;
     int ri;
     const int t0 = g0 + (wave << 6);
-    take_best(b, a.top, lane, &rk, &ri, [&](int w, unsigned k0, int i0, unsigned* nk, int* ni) {
+    take_best(b, a.top, lane, &rk, &ri, [&](int w, unsigned k0, int i0, Best2* lists, int* left) {
       // lane w's granules are t0 + w, + kPieceThreads, ...: the 64 lanes look through them
       Best2 q = {0u, 0u, -1, -1};
       for (int64_t h = (int64_t)t0 + w + (int64_t)lane * kPieceThreads; h < g1;
@@ -451,8 +522,12 @@ __global__ __launch_bounds__(kPieceThreads) void k_score_pieces(ScoreArgs a, int
       }
       unsigned kb;
       const int from = best_lane(q.k1, q.i1, &kb);
-      *nk = kb;
-      *ni = __builtin_amdgcn_readlane(q.i1, from);
+      const int ib = __builtin_amdgcn_readlane(q.i1, from);
+      if (lane == w) {
+        lists->k1 = kb;
+        lists->i1 = ib;
+        *left = 1;
+      }
     });
     if (lane < a.top) {
       lk[wave][lane] = rk;
@@ -614,6 +689,9 @@ __global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, 
 // rows of one launch: the launch's threads are counted in 32 bits
 constexpr int64_t kRowsPerLaunch = (int64_t)1 << 22;
 
+// So many rows fill the card with a wave each.
+constexpr int64_t kManyRows = 2048;
+
 template <typename T, bool TOP>
 hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) {
   // the longest row a wave keeps in registers: 8 granules a lane (one more than the row's length
@@ -624,7 +702,18 @@ hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) 
     const int64_t rows = n - a.row0 < kRowsPerLaunch ? n - a.row0 : kRowsPerLaunch;
     a.n = a.row0 + rows;
     const dim3 by4((unsigned)((rows + 3) / 4));
-    if (granules <= 64) {
+    if (a.v <= 64) {
+      int log2 = 2;
+      while ((1 << log2) < a.v) ++log2;
+      const dim3 by((unsigned)((rows + (256 >> log2) - 1) / (256 >> log2)));
+      switch (log2) {
+        case 2: hipLaunchKernelGGL((k_score_small<T, 2, TOP>), by, dim3(256), 0, s, a); break;
+        case 3: hipLaunchKernelGGL((k_score_small<T, 3, TOP>), by, dim3(256), 0, s, a); break;
+        case 4: hipLaunchKernelGGL((k_score_small<T, 4, TOP>), by, dim3(256), 0, s, a); break;
+        case 5: hipLaunchKernelGGL((k_score_small<T, 5, TOP>), by, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((k_score_small<T, 6, TOP>), by, dim3(256), 0, s, a); break;
+      }
+    } else if (granules <= 64) {
       hipLaunchKernelGGL((k_score_wave<T, 1, TOP>), by4, dim3(256), 0, s, a);
     } else if (granules <= 128) {
       hipLaunchKernelGGL((k_score_wave<T, 2, TOP>), by4, dim3(256), 0, s, a);
@@ -632,6 +721,12 @@ hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) 
       hipLaunchKernelGGL((k_score_wave<T, 4, TOP>), by4, dim3(256), 0, s, a);
     } else if (granules <= 512) {
       hipLaunchKernelGGL((k_score_wave<T, 8, TOP>), by4, dim3(256), 0, s, a);
+    } else if (TOP && sizeof(T) == 4 && granules <= 1024 && n >= kManyRows) {
+      // (ranking by one wave instead of four and a join: 17 852 rows of 2151 with the best thirty 187 ->
+      // 149 us, 20 000 of 4000 with the best five 94 -> 77; 16-bit rows of twice the length would need
+      // 360 registers: 3000 rows of 5000 fp16, best sixteen, 34 -> 36 us)
+      if constexpr (sizeof(T) == 4)
+        hipLaunchKernelGGL((k_score_wave<T, 16, TOP>), by4, dim3(256), 0, s, a);
     } else {
       hipLaunchKernelGGL((k_score_pieces<T, TOP>), dim3((unsigned)rows, (unsigned)pieces),
                          dim3(kPieceThreads), 0, s, a, pieces, part);

@@ -393,6 +393,46 @@ def test_label_logprobs_special_rows(t, v):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("v", [1, 2, 4, 5, 8, 9, 16, 17, 31, 32, 33, 63, 64, 65])
+def test_short_rows_of_scores_with_ties(t, v):
+    # a wave holds several such rows; the last workgroup is not full, rows lie apart
+    g = torch.Generator().manual_seed(v)
+    n = 131
+    z = torch.round(torch.randn(n, v, generator=g) * 1.5)
+    z[torch.rand(n, v, generator=g) < 0.3] = -math.inf
+    z[3] = -math.inf
+    z[4] = -0.0
+    z[4, ::2] = 0.0
+    z = z.to(t)
+    labels = torch.randint(-1, v + 1, (n,), generator=g)
+    wide = torch.full((n, v + 3), 7.0, dtype=t, device=DEV)
+    wide[:, 1:1 + v] = z
+    for top in sorted({0, 1, min(v, 3), min(v, 32)}):
+        check_scores(z, labels, top, 1.0)
+        check_scores(z, labels, top, 0.5, zd=wide[:, 1:1 + v])
+    bad = z.clone()
+    bad[n - 1, v - 1] = math.nan
+    bad[n - 3, 0] = math.inf
+    logp, ent, lse, tl, ti = ops.label_logprobs(bad.to(DEV), torch.zeros(n, dtype=torch.int32, device=DEV), top=1)
+    rows = torch.zeros(n, dtype=torch.bool, device=DEV)
+    rows[n - 1] = rows[n - 3] = True
+    for q in (ent, lse, tl[:, 0]):
+        assert torch.equal(torch.isnan(q), rows)
+    assert int(ti[n - 1, 0]) == v - 1 and int(ti[n - 3, 0]) == 0
+    logp2, ent2, lse2, _, ti2 = ops.label_logprobs(z.to(DEV), torch.zeros(n, dtype=torch.int32, device=DEV), top=1)
+    assert torch.equal(lse[~rows], lse2[~rows]) and torch.equal(ti[~rows], ti2[~rows])
+
+
+def test_many_rows_of_float32_scores_a_wave_each():
+    # rows long enough for sixteen pieces a lane, with ties, so that lanes give away many
+    g = torch.Generator().manual_seed(8)
+    for v, top in ((2046, 32), (3333, 20), (4090, 3)):
+        z = torch.round(torch.randn(2050, v, generator=g) * 40) / 16
+        labels = torch.randint(0, v, (2050,), generator=g)
+        check_scores(z, labels, top, 1.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 def test_best_alternatives_that_lie_in_one_lane(t):
     # the best scores 64 or 256 granules apart, and ties everywhere: a lane gives away many
     vec = 4 if t == torch.float32 else 8
