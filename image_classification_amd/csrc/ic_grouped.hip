@@ -25,6 +25,7 @@
 // the lane, so the layouts are not padded: 16-byte granules are exchanged inside a row by an
 // exclusive-or with bits of the row number, chosen so that the lanes of one LDS access fall into
 // different banks.  Granules outside the operands are fetched from a granule of zeros.
+#include <cmath>
 #include <type_traits>
 
 #include "ic_wave.h"
@@ -999,12 +1000,16 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
 // of its own.  A lane's granules of a chunk are neighbours (32 bytes), four lanes read 128 bytes.
 // 16 rows, 64 groups of 2048 x 2048 bf16 (about 14 of them met, 118 MB): 28.8 us, 4.1 TB/s (through LDS 36 us);
 // 1000 rows, 1000 groups of 64 x 128 float32 (21 MB): 10.6 us.
-template <typename T, bool BYDEPTH>
+// QALONG false (dx of float32, by depth only): the matrix's granules are gathered from four of its rows, 16
+// neighbouring columns a load; for launches that latency bounds (18 rows, 3 groups of 1336 x 184: 39.6 -> 13.4
+// us; 128 rows, 1 group of 1024 x 1024: 30.5 -> 10.1).
+template <typename T, bool BYDEPTH, bool QALONG, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
   constexpr int kV = Elem<T>::kVec;
   constexpr int kChunk = 8 * kV;                 // of the depth: 2 granules in each quarter wave
   constexpr int CF = BYDEPTH ? 2 : 1;            // fragments of 16 columns a wave
   constexpr int kCols = BYDEPTH ? 32 : 64;       // of a workgroup
+  static_assert(QALONG || (BYDEPTH && sizeof(T) == 4), "dx: float32 by depth");
   constexpr int kAhead = BYDEPTH ? 4 : 2;        // chunks whose loads are in flight together
   __shared__ f32x4 sums[BYDEPTH ? 4 : 1][CF][64];
   const int lane = threadIdx.x & 63;
@@ -1034,8 +1039,16 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
     for (int j = 0; j < CF; ++j) {
       int c = c0 + j * 16 + (lane & 15);
       if (c >= a.cols) c = a.cols - 1;           // (its products are not stored)
-      q[j] = static_cast<const T*>(a.q) + e * a.q_stride + (int64_t)c * a.ld_q + kq;
+      q[j] = static_cast<const T*>(a.q) + e * a.q_stride + (QALONG ? (int64_t)c * a.ld_q + kq : (int64_t)c);
     }
+    // four elements of a column from row k on
+    auto across = [&](const T* col, int k) {
+      u32x4 w = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        if (k + i < a.depth) w[i & 3] = *reinterpret_cast<const unsigned*>(col + (int64_t)(k + i) * a.ld_q);
+      return w;
+    };
     const int chunks = (a.depth + kChunk - 1) / kChunk;
     const int first = BYDEPTH ? (int)((int64_t)chunks * wave / 4) : 0;
     const int last = BYDEPTH ? (int)((int64_t)chunks * (wave + 1) / 4) : chunks;
@@ -1046,11 +1059,23 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int k = (c + i) * kChunk + h * kV;
-          const bool in = c + i < last && k + kq < a.depth;
-          pv[i][h] = in ? *reinterpret_cast<const u32x4*>(p + k) : u32x4{0u, 0u, 0u, 0u};
+          if constexpr (!QALONG) {
+            const bool in = c + i < last;
+            pv[i][h] = granule_of<T>(p, k, in ? a.depth - kq : 0);
 #pragma unroll
-          for (int j = 0; j < CF; ++j)
-            qv[i][j][h] = in ? *reinterpret_cast<const u32x4*>(q[j] + k) : u32x4{0u, 0u, 0u, 0u};
+            for (int j = 0; j < CF; ++j) qv[i][j][h] = across(q[j], in ? k + kq : a.depth);
+          } else if constexpr (ALIGNED) {
+            const bool in = c + i < last && k + kq < a.depth;
+            pv[i][h] = in ? *reinterpret_cast<const u32x4*>(p + k) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < CF; ++j)
+              qv[i][j][h] = in ? *reinterpret_cast<const u32x4*>(q[j] + k) : u32x4{0u, 0u, 0u, 0u};
+          } else {
+            const int width = c + i < last ? a.depth - kq : 0;    // of what begins at this lane's pointers
+            pv[i][h] = granule_of<T>(p, k, width);
+#pragma unroll
+            for (int j = 0; j < CF; ++j) qv[i][j][h] = granule_of<T>(q[j], k, width);
+          }
         }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
@@ -1106,6 +1131,7 @@ struct DwArgs {
   int out, k;
   int tiles, k_tiles;
   int wgs;
+  int whole;           // runs begin and end with tiles
   int y_f32, y_vec;
 };
 
@@ -1134,6 +1160,17 @@ __device__ __forceinline__ DwPlace dw_place(const DwArgs& a, int64_t u, int64_t 
   return p;
 }
 
+// The unit that workgroup w's run begins with (and w - 1's ends before).  Whole tiles: the first unit of a
+// tile, an equal number of tiles each.
+__device__ __forceinline__ int64_t dw_begin(const DwArgs& a, int64_t line, int64_t w, int64_t kk) {
+  if (!a.whole) return line * w / a.wgs;
+  const int64_t t = a.g.groups * a.tiles * w / a.wgs, e = t / a.tiles;
+  if (e >= a.g.groups) return line;
+  const int64_t o0 = uniform(a.g.at(e)), o1 = uniform(a.g.at(e + 1));
+  const int64_t stages = (o1 < o0 ? o0 : o1) / kk + 1 - o0 / kk;
+  return (o0 / kk + e) * a.tiles + t % a.tiles * stages;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
@@ -1150,8 +1187,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   // neighbours in the line share rows: they run on one XCD
   const int64_t w = xcd_run(blockIdx.x, gridDim.x);
   const int64_t line = dw_line(a, kK);
-  int64_t u = line * w / a.wgs;
-  const int64_t u1 = line * (w + 1) / a.wgs;
+  int64_t u = dw_begin(a, line, w, kK);
+  const int64_t u1 = dw_begin(a, line, w + 1, kK);
   const int wm = wave % WM, wn = wave / WM;
   const int pc = wm * (BM / WM), qc = wn * (BN / WN);
   const int pplace = across_place<T, BM, false>(pc, lane);
@@ -1282,7 +1319,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       __syncthreads();   // the buffers are free for the next run's loads
     }
     done += run;
-    const bool whole = pl.stage == 0 && run == pl.stages;
+    // (a.whole: always, unless the offsets do not ascend; there is no scratch then)
+    const bool whole = a.whole || (pl.stage == 0 && run == pl.stages);
     if (whole) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
@@ -1454,20 +1492,32 @@ hipError_t short_launch(RowsArgs a, hipStream_t s) {
   return launch_tiles(k_grouped_short<T, NS, QALONG>, a, (a.g.n / 64 + a.g.groups + 1) * a.col_tiles, 256, 0, s);
 }
 
-// Up to 8 rows a group on average (or hardly any rows at all), forward.
-template <typename T>
+// Few rows.
+template <typename T, bool QALONG, bool ALIGNED>
 hipError_t few_launch(RowsArgs a, hipStream_t s) {
-  const bool by_depth = a.depth >= 512;
+  const bool by_depth = !QALONG || a.depth >= 512;
   a.col_tiles = by_depth ? (a.cols + 31) / 32 : (a.cols + 63) / 64;
   const int64_t tiles = (a.g.n / 16 + a.g.groups + 1) * a.col_tiles;
-  return by_depth ? launch_tiles(k_grouped_few<T, true>, a, tiles, 256, 0, s)
-                  : launch_tiles(k_grouped_few<T, false>, a, tiles, 256, 0, s);
+  if (by_depth) return launch_tiles(k_grouped_few<T, true, QALONG, ALIGNED>, a, tiles, 256, 0, s);
+  if constexpr (QALONG) return launch_tiles(k_grouped_few<T, false, true, ALIGNED>, a, tiles, 256, 0, s);
+  return hipErrorInvalidValue;
 }
 
 template <typename T, bool QALONG>
 hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) {
+  // rows in tiles of 16, without stages: few rows a group or in all; and where the depth is long and tiles
+  // would leave most of the card idle (128 rows, 1 group of 1024 x 1024 float32: 28.5 -> 10.4 us, 250 rows,
+  // 3 groups of 1001 -> 100 38 -> 9.4; but 256 rows, 4 groups of 2048 x 2048 bf16, 256 tiles: 24 -> 30)
+  const int64_t tiles64 = (a.g.n / 64 + a.g.groups) * ((a.cols + 63) / 64);
+  const bool idle = a.g.n <= 256 && tiles64 < 128;
+  // (dx: 16-bit columns gathered element by element take longer than the stages do: 16 rows, 4 groups of
+  // 2000 x 128 fp16 16.6 -> 29 us; float32 from a depth of 256 on: 2 rows, 410 -> 943, 19.7 -> 8.5 us)
+  if constexpr (!QALONG && sizeof(T) == 4)
+    if (idle && a.depth >= 256) return few_launch<T, false, false>(a, s);
+  if constexpr (QALONG)
+    if (a.g.n <= 8 * a.g.groups || a.g.n <= 32 || (idle && a.depth >= 512))
+      return aligned ? few_launch<T, true, true>(a, s) : few_launch<T, true, false>(a, s);
   if (!aligned) return rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
-  if (QALONG && (a.g.n <= 8 * a.g.groups || a.g.n <= 32)) return few_launch<T>(a, s);
   // rows of at most 512 bytes whose tiles would be 64 x 64 anyway (fewer columns, or short groups)
   const int64_t row_bytes = (int64_t)a.depth * (int)sizeof(T);
   if (row_bytes <= 512 && (a.cols <= 64 || a.g.n < 128 * a.g.groups)) {
@@ -1498,12 +1548,16 @@ bool grouped_aligned(const GroupedCall& c, bool dw) {
 struct DwPlan {
   int tile;
   int wgs;
+  bool whole;
 };
 DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned) {
   const int kk = kStageBytes / (type == IC_F32 ? 4 : 2);
   const double* rate = type == IC_F32 ? kRate32 : kRate16;
-  DwPlan best = {2, 1};
+  DwPlan best = {2, 1, false};
   double least = 1e300;
+  // So few rows that a tile has at most five stages: whole tiles, nothing cut and nothing joined (128 rows,
+  // 1 group of 1024 x 1024 float32: 21 -> 10 us with the call).
+  const bool whole = n <= 4 * kk;
   for (int i = aligned ? 0 : 2; i < 3; ++i) {
     const int size = kTileSize[i];
     const double tiles = (double)((out + size - 1) / size) * ((k + size - 1) / size);
@@ -1513,17 +1567,26 @@ DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned
     // pipeline, the time of about six units
     double wgs = line / 4;
     const double slots = (double)kCUs * kPerCu[i];
+    if (whole) {
+      const double all = tiles * groups, rounds = std::ceil(all / slots);
+      const double t = rounds * kPerCu[i] * size * size / rate[i];
+      if (t < least) {
+        least = t;
+        best = DwPlan{i, (int)(all < 8 * slots ? all : 8 * slots), whole};
+      }
+      continue;
+    }
     wgs = wgs < 1 ? 1 : wgs > slots ? slots : wgs;
     const double t = (line / wgs + 6) * kPerCu[i] * size * size / rate[i];
     if (t < least) {
       least = t;
-      best = DwPlan{i, (int)wgs};
+      best = DwPlan{i, (int)wgs, false};
     }
   }
   return best;
 }
 size_t dw_scratch_of(const DwPlan& p) {
-  return (size_t)2 * p.wgs * kTileSize[p.tile] * kTileSize[p.tile] * 4;
+  return p.whole ? 0 : (size_t)2 * p.wgs * kTileSize[p.tile] * kTileSize[p.tile] * 4;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool ALIGNED>
@@ -1534,7 +1597,7 @@ hipError_t dw_launch(DwArgs a, hipStream_t s) {
   a.tiles = (int)tiles;
   hipLaunchKernelGGL((k_grouped_dw<T, BM, BN, WM, WN, ALIGNED>), dim3((unsigned)a.wgs), dim3(WM * WN * 64),
                      (rows_lds<BM, BN>()), s, a);
-  if (a.wgs > 1) {
+  if (a.wgs > 1 && !a.whole) {
     // a workgroup for each 4096 elements and each end of a run; four where that makes few (2000 rows,
     // 8 groups of 64 x 128 float32, both kernels: 14.8 -> 12.5 us; with many, most find nothing to add and
     // more of them cost time: 4096 rows, 16 groups of 512 x 512 bf16, 23.7 us with one, 27.1 with four)
@@ -1658,6 +1721,7 @@ hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s)
   a.ld_x = c.ld_x;
   const DwPlan plan = dw_plan(c.n, c.groups, c.k, c.out, c.type, al);
   a.wgs = plan.wgs;
+  a.whole = plan.whole;
   a.out = c.out;
   a.k = c.k;
   a.y_f32 = c.y_f32 || c.type == IC_F32;

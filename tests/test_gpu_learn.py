@@ -243,12 +243,39 @@ def test_bad_orders_and_offsets_stay_inside():
     far[-1] = 10 ** 12
     all_rows = ops.grouped_matmul(x.to(DEV), w.to(DEV), far, order)
     assert torch.equal(all_rows[codes.to(DEV) >= 0], good[codes.to(DEV) >= 0])
-    for off in ([0, 150, 20, 200], [-5, -9, 300, 100], [10 ** 15, 0, 0, -10 ** 15]):
+    for off in ([0, 150, 20, 200], [-5, -9, 300, 100], [10 ** 15, 0, 0, -10 ** 15], [0, 90, 10, 60], [0, 70, 70, 3]):
         o = torch.tensor(off, device=DEV)
+        for few in (1, 100):       # (whole tiles of the weight gradient)
+            few_order = torch.arange(few, dtype=torch.int32, device=DEV)
+            ops.grouped_matmul(x.to(DEV)[:few], w.to(DEV), o, few_order)
+            ops.grouped_matmul_dx(dy.to(DEV)[:few], w.to(DEV), o, few_order)
+            ops.grouped_matmul_dw(dy.to(DEV)[:few], x.to(DEV)[:few], o, few_order)
         ops.grouped_matmul(x.to(DEV), w.to(DEV), o, order)
         ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), o, order)
         ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), o, order)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 2, 31, 100, 128, 129, 256, 257])
+@pytest.mark.parametrize("groups, k, out", [(1, 943, 41), (7, 64, 72), (300, 40, 33), (2500, 24, 8), (2, 64, 520),
+                                            (3, 33, 1031)])
+def test_few_rows_forward_and_back(n, groups, k, out, t):
+    # from rows read without a tile and whole tiles of the weight gradient to the general forms
+    codes, x, dy, w = group_case(n, groups, k, out, t, n + groups)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    y = ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+    dx = ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+    dw = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+    close(y, *ref["y"], k, "y")
+    close(dx, *ref["dx"], out, "dx")
+    close(dw, *ref["dw"], n, "dw")
+    # one row further on in memory: another alignment, the same sums
+    shifted = torch.zeros(n * k + 1, dtype=t, device=DEV)
+    shifted[1:] = x.to(DEV).flatten()
+    y2 = ops.grouped_matmul(shifted[1:].view(n, k), w.to(DEV), offsets, order, out_dtype=torch.float32)
+    close(y2, *ref["y"], k, "y")
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)

@@ -79,7 +79,8 @@ def test_scratch_sizes():
     assert lib.ic_group_rows_scratch(1_000_000, 10_000) >= 12_000_000   # pairs and sorted codes
     # two partial tiles a workgroup: at most 256 x 2 x 256 x 256 floats, little for little work
     for t in (0, 1, 2):
-        assert 0 < lib.ic_grouped_matmul_dw_scratch(0, 1, 8, 8, t) <= 2 * 64 * 64 * 4
+        assert lib.ic_grouped_matmul_dw_scratch(0, 1, 8, 8, t) == 0          # nothing is cut
+        assert lib.ic_grouped_matmul_dw_scratch(100, 50, 800, 80, t) == 0
         for n, e, k, out in ((1_000_000, 10_000, 128, 64), (65536, 16, 2048, 2048), (3_000_000, 1, 2048, 16),
                              (4097, 3, 8, 8)):
             assert 0 < lib.ic_grouped_matmul_dw_scratch(n, e, k, out, t) <= 2 * 256 * 256 * 256 * 4
@@ -227,3 +228,34 @@ def test_memory_that_is_shared():
             ops._check_apart(a, b)
         with pytest.raises(ValueError, match="share no memory"):
             ops._check_apart(b, a)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_whole_tiles_of_a_weight_gradient_are_dealt_once(seed):
+    # few rows: runs that begin and end with tiles (the unit a run begins with, worked out from its tile)
+    import numpy as np
+    rng = np.random.default_rng(200 + seed)
+    kk = int(rng.choice([32, 64]))
+    groups, tiles = int(rng.integers(1, 9)), int(rng.integers(1, 6))
+    wgs = int(rng.integers(1, groups * tiles + 1))
+    sizes = rng.choice([0, 0, 1, kk, int(rng.integers(0, 4 * kk))], groups)
+    off = [int(o) for o in np.concatenate([[0], np.cumsum(sizes)])]
+    line = (off[groups] // kk + groups) * tiles
+
+    def begin(w):
+        t = groups * tiles * w // wgs
+        e = t // tiles
+        if e >= groups:
+            return line
+        stages = off[e + 1] // kk + 1 - off[e] // kk
+        return (off[e] // kk + e) * tiles + t % tiles * stages
+
+    assert begin(0) == 0 and begin(wgs) == line
+    starts, u = set(), 0
+    for e in range(groups):
+        for _ in range(tiles):
+            starts.add(u)
+            u += off[e + 1] // kk + 1 - off[e] // kk
+    assert u == line
+    at = [begin(w) for w in range(wgs + 1)]
+    assert at == sorted(at) and set(at[:-1]) <= starts and len(set(at)) == wgs + 1
