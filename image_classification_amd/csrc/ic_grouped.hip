@@ -707,22 +707,21 @@ struct RowsArgs {
   int depth;           // length of the contraction
   int cols;            // columns of the result
   int col_tiles;
-  int y_f32, y_vec;    // y_vec: four columns can be stored at once
+  int y_f32;
   int64_t id0;         // the first tile of this launch
 };
 
 // A lane's sixteen results of one row, v[j] those of fragment j, in the 64 columns from c on; the row
 // begins at `at` and has `cols` columns.  vec: 16 bytes can be stored at once.
 template <typename T>
-__device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, int lane, bool f32, bool vec,
-                                        const f32x4* v) {
+__device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, int lane, bool f32, const f32x4* v) {
   if (sizeof(T) == 4 || f32) {
     float* d = static_cast<float*>(y) + at;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int cj = c + spread_row<T>((lane >> 4) * 4) + spread_step<T>(j);
-      if (vec && cj + 4 <= cols) {
-        *reinterpret_cast<f32x4*>(d + cj) = v[j];
+      if (cj + 4 <= cols) {
+        __builtin_memcpy(d + cj, &v[j], 16);     // (a 16-byte store: memory may be written at any address)
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -737,8 +736,9 @@ __device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, in
       float f[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = v[2 * h + (i >> 2)][i & 3];
-      if (vec && cj + 8 <= cols) {
-        *reinterpret_cast<u32x4*>(d + cj) = Elem<T>::pack(f);
+      if (cj + 8 <= cols) {
+        const u32x4 w = Elem<T>::pack(f);
+        __builtin_memcpy(d + cj, &w, 16);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -902,7 +902,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int row = rows[pr + i * 16 + (lane & 15)];
-    if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y, c0 + qc, a.cols, lane, a.y_f32, a.y_vec, acc[i]);
+    if (row >= 0) store16<T>(a.y, (int64_t)row * a.ld_y, c0 + qc, a.cols, lane, a.y_f32, acc[i]);
   }
 }
 
@@ -990,7 +990,7 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
       }
     }
   }
-  if (row >= 0) store16<T>(a.y, row * a.ld_y, c0, a.cols, lane, a.y_f32, a.y_vec, acc);
+  if (row >= 0) store16<T>(a.y, row * a.ld_y, c0, a.cols, lane, a.y_f32, acc);
 }
 
 // Few rows a group (single rows to serve): the matrices are the traffic, so a workgroup takes 16 rows
@@ -1132,7 +1132,7 @@ struct DwArgs {
   int tiles, k_tiles;
   int wgs;
   int whole;           // runs begin and end with tiles
-  int y_f32, y_vec;
+  int y_f32;
 };
 
 // A place in the line.
@@ -1325,7 +1325,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int o = m0 + pc + i * 16 + (lane & 15);
-        if (o < a.out) store16<T>(a.dw, (pl.e * a.out + o) * a.k, n0 + qc, a.k, lane, a.y_f32, a.y_vec, acc[i]);
+        if (o < a.out) store16<T>(a.dw, (pl.e * a.out + o) * a.k, n0 + qc, a.k, lane, a.y_f32, acc[i]);
       }
     } else {
       // 16 bytes a lane, lanes side by side; the join undoes the order
@@ -1384,8 +1384,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
     const int left = a.k - c;
     if (a.y_f32 || sizeof(T) == 4) {
       float* d = static_cast<float*>(a.dw) + to;
-      if (a.y_vec && left >= 4) {
-        *reinterpret_cast<f32x4*>(d) = s;
+      if (left >= 4) {
+        __builtin_memcpy(d, &s, 16);
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -1393,15 +1393,15 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_grouped_dw_join(DwArgs a) {
       }
     } else if constexpr (sizeof(T) == 2) {
       T* d = static_cast<T*>(a.dw) + to;
-      T h[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) Elem<T>::store(&h[q], s[q]);
-      if (a.y_vec && left >= 4) {
-        *reinterpret_cast<u32x2*>(d) = *reinterpret_cast<u32x2*>(h);
+      if (left >= 4) {
+        const float f[8] = {s[0], s[1], s[2], s[3], 0.f, 0.f, 0.f, 0.f};
+        const u32x4 w = Elem<T>::pack(f);
+        const u32x2 h = {w[0], w[1]};
+        __builtin_memcpy(d, &h, 8);
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (q < left) d[q] = h[q];
+          if (q < left) Elem<T>::store(d + q, s[q]);
       }
     }
   };
@@ -1694,8 +1694,6 @@ hipError_t launch_grouped_rows(const GroupedCall& c, bool dx, hipStream_t s) {
   a.depth = dx ? c.out : c.k;
   a.cols = dx ? c.k : c.out;
   a.y_f32 = c.y_f32 || c.type == IC_F32;
-  const int yb = a.y_f32 ? 4 : 2;
-  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && (c.ld_y * yb) % 16 == 0;
   const bool al = grouped_aligned(c, false);
   if (c.type == IC_F32) return dx ? rows_typed<float, false>(a, c.type, al, s) : rows_typed<float, true>(a, c.type, al, s);
   if (c.type == IC_BF16) return dx ? rows_typed<bf16_t, false>(a, c.type, al, s) : rows_typed<bf16_t, true>(a, c.type, al, s);
@@ -1725,8 +1723,6 @@ hipError_t launch_grouped_dw(const GroupedCall& c, void* scratch, hipStream_t s)
   a.out = c.out;
   a.k = c.k;
   a.y_f32 = c.y_f32 || c.type == IC_F32;
-  const int yb = a.y_f32 ? 4 : 2;
-  a.y_vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && ((int64_t)c.k * yb) % 16 == 0;
   if (c.type == IC_F32) return dw_typed<float>(a, plan.tile, al, s);
   if (c.type == IC_BF16) return dw_typed<bf16_t>(a, plan.tile, al, s);
   return dw_typed<f16_t>(a, plan.tile, al, s);
