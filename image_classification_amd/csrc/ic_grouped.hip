@@ -907,17 +907,17 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 }
 
 // Short rows (a contraction of at most NS stages, 512 bytes: the 128 float32 of a local descriptor), tiles
-// of 64 x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
-// goes to LDS, shared by the four waves; each wave's 16 rows go straight to the registers that the
+// of 64 R x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
+// goes to LDS, shared by the four waves; each wave's 16 R rows go straight to the registers that the
 // products take them from.  One barrier, one memory latency behind the search for the group.
-// 1M rows x 128 float32, 10 000 groups of 64 x 128: 343 us, 3.2 TB/s of rows, matrices and results and
+// 1M rows x 128 float32, 10 000 groups of 64 x 128: 321 us (R = 1: 343), 3.4 TB/s of rows, matrices and results and
 // 48 TFLOP/s (staged like the longer ones 355 us).  Neither is at its limit (memory 0.21 ms, products
-// 0.11 ms): a workgroup loads, multiplies and stores once, and what five of them a CU overlap is part
+// 0.11 ms): a workgroup loads, multiplies and stores once, and what four of them a CU overlap is part
 // of it.
-// Five workgroups share a CU: 32 KB of LDS and 96 registers each.
-template <typename T, int NS, bool QALONG>
-__global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
-  constexpr int BN = 64, kWaves = 4, FN = 4;
+// Five workgroups share a CU (R = 2: four): 32 KB of LDS and 96 (128) registers each.
+template <typename T, int NS, int R, bool QALONG>
+__global__ __launch_bounds__(256, R == 1 ? 5 : 3) void k_grouped_short(RowsArgs a) {
+  constexpr int BN = 64, kWaves = 4, FN = 4, BM = 64 * R;
   constexpr int kV = Elem<T>::kVec, kK = Mma<T>::kK;
   constexpr int kQRow = BN * (int)sizeof(T) / 16;
   constexpr int kStage = BN * kStageBytes;
@@ -929,31 +929,39 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
   const int c0 = (int)(id % a.col_tiles) * BN;
   // (what still loads goes before what multiplies: 3 %)
   __builtin_amdgcn_s_setprio(3);
-  const Found f = find_group_once(a.g, tile, 64, wave, lane, reinterpret_cast<unsigned*>(smem));
+  const Found f = find_group_once(a.g, tile, BM, wave, lane, reinterpret_cast<unsigned*>(smem));
   __syncthreads();   // (the box is read: its place may be filled)
-  const int64_t t = tile - (f.o0 / 64 + f.e);
-  const int64_t r0 = f.o0 + t * 64;
+  const int64_t t = tile - (f.o0 / BM + f.e);
+  const int64_t r0 = f.o0 + t * BM;
   if (t < 0 || r0 >= f.o1) return;
   // the last tile of a group leaves waves without rows: not the same ones in every tile
   const int quarter = (wave + (int)tile) & 3;
-  const int64_t pos = r0 + quarter * 16 + (lane & 15);
-  int64_t row = -1;
-  if (pos < f.o1) {
-    row = a.order ? (int64_t)a.order[pos] : pos;
-    if (row < 0 || row >= a.g.n) row = -1;
-  }
-  f32x4 acc[FN];
+  int64_t row[R];
 #pragma unroll
-  for (int j = 0; j < FN; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < R; ++r) {
+    const int64_t pos = r0 + (r * 4 + quarter) * 16 + (lane & 15);
+    row[r] = -1;
+    if (pos < f.o1) {
+      row[r] = a.order ? (int64_t)a.order[pos] : pos;
+      if (row[r] < 0 || row[r] >= a.g.n) row[r] = -1;
+    }
+  }
+  f32x4 acc[R][FN];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (f.e < a.g.groups) {
-    const bool busy = r0 + quarter * 16 < f.o1;
-    const T* p = static_cast<const T*>(a.p) + (row < 0 ? 0 : row) * a.ld_p + (lane >> 4) * kV;
-    u32x4 pf[2 * NS];
-    if (busy) {
+    u32x4 pf[R][2 * NS];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool busy = r0 + (r * 4 + quarter) * 16 < f.o1;
+      const T* p = static_cast<const T*>(a.p) + (row[r] < 0 ? 0 : row[r]) * a.ld_p + (lane >> 4) * kV;
 #pragma unroll
       for (int i = 0; i < 2 * NS; ++i) {
         const int k = i * 4 * kV;
-        pf[i] = k + (lane >> 4) * kV < a.depth ? *reinterpret_cast<const u32x4*>(p + k) : u32x4{0u, 0u, 0u, 0u};
+        pf[r][i] = busy && k + (lane >> 4) * kV < a.depth ? *reinterpret_cast<const u32x4*>(p + k)
+                                                          : u32x4{0u, 0u, 0u, 0u};
       }
     }
     const T* qb = static_cast<const T*>(a.q) + f.e * a.q_stride;
@@ -978,6 +986,7 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
     all_landed();
     __syncthreads();
     __builtin_amdgcn_s_setprio(0);
+    const bool busy = r0 + quarter * 16 < f.o1, second = R > 1 && r0 + (4 + quarter) * 16 < f.o1;
     if (busy) {
 #pragma unroll
       for (int i = 0; i < 2 * NS; ++i) {
@@ -986,11 +995,20 @@ __global__ __launch_bounds__(256, 5) void k_grouped_short(RowsArgs a) {
 #pragma unroll
         for (int part = 0; part < Mma<T>::kParts; ++part)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[j] = Mma<T>::mul(part, qf[j], pf[i], acc[j]);
+          for (int j = 0; j < FN; ++j) acc[0][j] = Mma<T>::mul(part, qf[j], pf[0][i], acc[0][j]);
+        if constexpr (R > 1) {
+          if (second)
+#pragma unroll
+            for (int part = 0; part < Mma<T>::kParts; ++part)
+#pragma unroll
+              for (int j = 0; j < FN; ++j) acc[R - 1][j] = Mma<T>::mul(part, qf[j], pf[R - 1][i], acc[R - 1][j]);
+        }
       }
     }
   }
-  if (row >= 0) store16<T>(a.y, row * a.ld_y, c0, a.cols, lane, a.y_f32, acc);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (row[r] >= 0) store16<T>(a.y, row[r] * a.ld_y, c0, a.cols, lane, a.y_f32, acc[r]);
 }
 
 // Few rows a group (single rows to serve): the matrices are the traffic, so a workgroup takes 16 rows
@@ -1489,7 +1507,12 @@ int pick_tile(int type, F tiles) {
 template <typename T, int NS, bool QALONG>
 hipError_t short_launch(RowsArgs a, hipStream_t s) {
   a.col_tiles = (a.cols + 63) / 64;
-  return launch_tiles(k_grouped_short<T, NS, QALONG>, a, (a.g.n / 64 + a.g.groups + 1) * a.col_tiles, 256, 0, s);
+  // 128 rows a workgroup where there are many of them: the matrix is fetched and read from LDS for twice the
+  // rows (1M rows, 2000 groups of 64 x 128 float32: 261 -> 246 us, 200 000 rows, 2000 groups of 200 x 64
+  // bf16 45 -> 40); with few (20 000 rows, 200 groups: 11.4 -> 16.5) or narrow results (32 columns: 70 -> 74) 64
+  const int64_t twice = (a.g.n / 128 + a.g.groups + 1) * a.col_tiles;
+  if (twice >= 8192 && a.cols > 32) return launch_tiles(k_grouped_short<T, NS, 2, QALONG>, a, twice, 256, 0, s);
+  return launch_tiles(k_grouped_short<T, NS, 1, QALONG>, a, (a.g.n / 64 + a.g.groups + 1) * a.col_tiles, 256, 0, s);
 }
 
 // Few rows.

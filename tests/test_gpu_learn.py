@@ -291,6 +291,24 @@ def test_tiles_cut_into_many_pieces(n, groups, k, out, t):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, groups, k, out", [(30_000, 700, 32, 600), (40_000, 8000, 24, 40), (3000, 8200, 16, 33)])
+def test_many_short_rows(n, groups, k, out, t):
+    # workgroups of 128 short rows: groups that end in their first, second or no half
+    codes, x, dy, w = group_case(n, groups, k, out, t, 21)
+    xd, dd, wd = x.double(), dy.double(), w.double()
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    y = ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+    dx = ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+    none = codes < 0
+    assert bool((y.cpu()[none] == 0).all()) and bool((dx.cpu()[none] == 0).all())
+    at = torch.nonzero(~none)[:, 0]
+    at = at[torch.randperm(at.numel(), generator=torch.Generator().manual_seed(1))[:1500]]
+    wr = wd[codes[at].long()]
+    close(y.cpu()[at], (wr * xd[at][:, None, :]).sum(2), (wr * xd[at][:, None, :]).abs().sum(2), k, "y")
+    close(dx.cpu()[at], (wr * dd[at][:, :, None]).sum(1), (wr * dd[at][:, :, None]).abs().sum(1), out, "dx")
+
+
 def test_results_share_no_memory_with_the_inputs():
     codes, x, dy, w = group_case(64, 2, 16, 16, torch.float32, 4)
     wide = torch.zeros(64, 48, device=DEV)
