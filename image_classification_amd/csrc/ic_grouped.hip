@@ -167,16 +167,20 @@ __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restri
 }
 
 // Many rows: a pass over a digit is three launches (counts per block of rows, prefixes, scatter).
-// Bound by the launches' latency: 42 000 rows of 21 groups take 5 + 5 + 8 us and the offsets 5, a
-// million rows of 10 000 groups (two passes) 52 us in all, of which 12 MB read and written would be 5.
-constexpr int kSortRows = 4096;     // rows of a workgroup
+// Bound by the launches' latency: 42 000 rows of 21 groups take 12.6 us in a captured graph, a million rows of
+// 10 000 groups (two passes) 43, of which 12 MB read and written would be 5.
+// A workgroup takes 4096 rows, or 2048 up to 2M rows, where a pass has few workgroups (42 000 rows 15.1 ->
+// 12.6 us in a captured graph, 200 000 of 4000 groups 30 -> 25, 1M of 10 000 equal; 5M of 1000: 94 -> 104).
+constexpr int64_t kSortFew = 2 << 20;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
+static_assert(kSortThreads >= 1 << kMaxDigitBits, "a thread holds the first place of a digit");
 
 struct SortPlan {
   int bits;        // of the key: groups + 1 values, the last for rows of no group
   int passes;
   int digit_bits;
+  int rows;        // of a workgroup
   int64_t blocks;
   size_t o_tab, o_total, o_pairs0, o_pairs1, o_codes, bytes;
 };
@@ -186,7 +190,8 @@ SortPlan sort_plan(int64_t n, int64_t groups) {
   while (((int64_t)1 << p.bits) < groups + 1) ++p.bits;
   p.passes = (p.bits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digit_bits = (p.bits + p.passes - 1) / p.passes;
-  p.blocks = (n + kSortRows - 1) / kSortRows;
+  p.rows = n <= kSortFew ? 2048 : 4096;
+  p.blocks = (n + p.rows - 1) / p.rows;
   size_t off = 0;
   auto take = [&off](size_t b) {
     const size_t o = off;
@@ -215,6 +220,7 @@ __device__ __forceinline__ unsigned key_of(const int32_t* codes, const Pair* pai
 }
 
 // tab[digit][block] = rows of the block with that digit
+template <int ROWS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int32_t* codes, const Pair* pairs,
                                                              int64_t n, int64_t groups, int shift,
                                                              int digit_bits, unsigned* tab) {
@@ -222,9 +228,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int32_t* code
   const int digits = 1 << digit_bits;
   for (int d = threadIdx.x; d < digits; d += kSortThreads) cnt[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortRows;
+  const int64_t base = (int64_t)blockIdx.x * ROWS;
 #pragma unroll
-  for (int r = 0; r < kSortRows / kSortThreads; ++r) {
+  for (int r = 0; r < ROWS / kSortThreads; ++r) {
     const int64_t i = base + r * kSortThreads + threadIdx.x;
     if (i < n) atomicAdd(&cnt[(key_of(codes, pairs, i, groups) >> shift) & (digits - 1)], 1u);
   }
@@ -259,6 +265,7 @@ __global__ __launch_bounds__(256) void k_sort_scan(unsigned* tab, int64_t blocks
 // Rows to their places of this digit, keeping the order of equal digits: a wave takes 64
 // consecutive rows at a time (rank among equal digits from ballots), the waves' counts are summed
 // in wave order.
+template <int ROWS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
     const int32_t* codes, const Pair* pairs, int64_t n, int64_t groups, int shift, int digit_bits,
     const unsigned* tab, const unsigned* total, Pair* out_pairs, int32_t* out_order,
@@ -284,8 +291,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
   for (int w = 0; w < wave; ++w) before += wave_sum[w];
   if (threadIdx.x < (unsigned)digits)
     first[threadIdx.x] = before + inc - v + tab[(size_t)threadIdx.x * gridDim.x + blockIdx.x];
-  constexpr int kR = kSortRows / kSortThreads;   // rounds of 64 rows a wave
-  const int64_t base = (int64_t)blockIdx.x * kSortRows + wave * (64 * kR);
+  constexpr int kR = ROWS / kSortThreads;   // rounds of 64 rows a wave
+  const int64_t base = (int64_t)blockIdx.x * ROWS + wave * (64 * kR);
   unsigned key[kR], rank[kR];
   const unsigned long long below = (1ull << lane) - 1ull;
 #pragma unroll
@@ -1690,12 +1697,13 @@ hipError_t launch_group_rows(const int32_t* codes, int64_t n, int64_t groups, in
   const Pair* in = nullptr;
   for (int i = 0; i < p.passes; ++i) {
     const int shift = i * p.digit_bits;
-    hipLaunchKernelGGL(k_sort_count, dim3((unsigned)p.blocks), dim3(kSortThreads), 0, s, codes, in, n, groups,
-                       shift, p.digit_bits, tab);
+    const bool few = p.rows == 2048;
+    hipLaunchKernelGGL(few ? k_sort_count<2048> : k_sort_count<4096>, dim3((unsigned)p.blocks), dim3(kSortThreads), 0,
+                       s, codes, in, n, groups, shift, p.digit_bits, tab);
     hipLaunchKernelGGL(k_sort_scan, dim3(1u << p.digit_bits), dim3(256), 0, s, tab, p.blocks, total);
     Pair* out = i + 1 < p.passes ? pairs[i & 1] : nullptr;
-    hipLaunchKernelGGL(k_sort_scatter, dim3((unsigned)p.blocks), dim3(kSortThreads), 0, s, codes, in, n,
-                       groups, shift, p.digit_bits, tab, total, out, order, sorted);
+    hipLaunchKernelGGL(few ? k_sort_scatter<2048> : k_sort_scatter<4096>, dim3((unsigned)p.blocks), dim3(kSortThreads),
+                       0, s, codes, in, n, groups, shift, p.digit_bits, tab, total, out, order, sorted);
     in = out;
   }
   hipLaunchKernelGGL(k_group_offsets, dim3((unsigned)((n + 1 + 255) / 256)), dim3(256), 0, s, sorted, n, groups,

@@ -30,7 +30,8 @@ def grouping(codes, groups):
 @pytest.mark.parametrize("n,groups", [
     (0, 1), (0, 5000), (1, 1), (1, 70000), (2, 3), (63, 7), (64, 64), (65, 1000), (511, 2), (512, 9),
     (513, 300), (2047, 5), (4096, 4096), (4096, 1), (4097, 1), (4097, 511), (5000, 512), (8192, 70000),
-    (12289, 10000), (100003, 37), (300000, 300000), (70000, 1 << 20)])
+    (12289, 10000), (100003, 37), (300000, 300000), (70000, 1 << 20),
+    (2_200_001, 3000)])
 @pytest.mark.parametrize("kind", ["even", "skewed", "one", "none"])
 def test_group_rows(n, groups, kind):
     rng = np.random.default_rng(n * 31 + groups)
