@@ -289,8 +289,8 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
   int ri = -1;
   if (TOP) {
     if (sizeof(T) == 2 && a.v <= kPackedMost && st.s == st.s) {
-      // word (i, w, h): element 2 w + h of granule i.  `floor_`: only words below it count.
-      auto best2 = [&](unsigned floor_, unsigned* k1, unsigned* k2) {
+      // word (i, w, h): element 2 w + h of granule i.  Unless `all`, only words below floor_ count.
+      auto best2 = [&](bool all, unsigned floor_, unsigned* k1, unsigned* k2) {
         unsigned b1 = 0, b2 = 0;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -303,11 +303,11 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
               const unsigned at = (unsigned)(low - 2 * w - h);
               unsigned k = h ? (pair & 0xffff0000u) | (at & 0xffffu) : (pair << 16) | (at & 0xffffu);
               // (elements before the row lie in granule 0)
-              if (i == 0) k = at > 65535u ? 0u : k;
-              k = k < floor_ ? k : 0u;
-              const unsigned lesser = b1 < k ? b1 : k;
+              if (i == 0 && rv.head) k = at > 65535u ? 0u : k;
+              if (!all) k = k < floor_ ? k : 0u;
+              // the median of the best two and a third is the new second
+              asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b2) : "v"(b1), "v"(b2), "v"(k));
               b1 = b1 > k ? b1 : k;
-              b2 = b2 > lesser ? b2 : lesser;
             }
           }
         }
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
         *k2 = b2;
       };
       unsigned k1, k2;
-      best2(0xffffffffu, &k1, &k2);
+      best2(true, 0u, &k1, &k2);
       unsigned mine = 0;
       for (int r = 0; r < a.top; ++r) {
         const unsigned kb = wave_max_u32(k1);
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
         k2 = won ? 0u : k2;
         if (r + 1 < a.top && __ballot(spent)) {
           unsigned n1, n2;
-          best2(kb, &n1, &n2);
+          best2(false, kb, &n1, &n2);
           k1 = n1;
           k2 = n2;
         }
