@@ -603,9 +603,20 @@ template <typename T>
 __device__ __forceinline__ u32x4 granule_of(const T* row, int64_t c, int64_t cols) {
   constexpr int kV = Elem<T>::kVec;
   u32x4 w = {0u, 0u, 0u, 0u};
-  if (row && c + kV <= cols) {
+  if (!row || c >= cols) return w;
+  if (c + kV <= cols) {
     __builtin_memcpy(&w, row + c, 16);   // (a 16-byte load: memory may be read at any address)
-  } else if (row) {
+  } else if (cols >= kV) {
+    // the row's last granule, without what lies before c (element by element, the workgroups of a matrix's
+    // last columns took several times as long as the others)
+    u32x4 q;
+    __builtin_memcpy(&q, row + cols - kV, 16);
+    const unsigned drop = (unsigned)(c + kV - cols) * 8 * (unsigned)sizeof(T);   // bits, 16 to 112
+    const uint64_t low = (uint64_t)q[1] << 32 | q[0], high = (uint64_t)q[3] << 32 | q[2];
+    const uint64_t a = drop >= 64 ? high >> (drop - 64) : low >> drop | high << 1 << (63 - drop);
+    const uint64_t b = drop >= 64 ? 0 : high >> drop;
+    w = u32x4{(unsigned)a, (unsigned)(a >> 32), (unsigned)b, (unsigned)(b >> 32)};
+  } else {
 #pragma unroll
     for (int i = 0; i < kV; ++i)
       if (c + i < cols) {
@@ -636,13 +647,12 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
 // The freed buffer is refilled with stage st + 2 one load per four products, during the last part of
 // st and (of four parts) the first of st + 1: issued in one go behind the barrier, the 8 waves' loads
 // would hold up the products behind them in every wave.
-// LOAD(i, stage, buffer) issues load i of kLoads (LOADS_EACH instructions), straight to the buffer if
-// ALIGNED, else to registers that PLACE(i, buffer) writes there a stage later; with PREPARES, NEXT(stage) fetches what the loads of
-// that stage need, and lands a barrier before them.
-#define MULTIPLY_STAGES(STAGES, LOAD, PLACE, NEXT, PREPARES, LOADS_EACH)                                          \
+// LOAD(i, stage, buffer) issues load i of kLoads (LOADS_EACH instructions) straight to the buffer; with
+// PREPARES, NEXT(stage) fetches what the loads of that stage need, and lands a barrier before them.
+#define MULTIPLY_STAGES(STAGES, LOAD, NEXT, PREPARES, LOADS_EACH)                     \
   {                                                                                  \
     constexpr int kStage = kPBytes + kQBytes;                                        \
-    constexpr int kFirst = kHalves == 2 && ALIGNED ? kLoads / 2 : kLoads;            \
+    constexpr int kFirst = kHalves == 2 ? kLoads / 2 : kLoads;                       \
     auto none = [](int) {};                                                          \
     if (PREPARES) {                                                                  \
       NEXT(0);                                                                       \
@@ -651,14 +661,8 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       __syncthreads();                                                               \
     }                                                                                \
     _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0, smem);             \
-    if (!ALIGNED) {                                                                  \
-      _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, smem);             \
-    }                                                                                \
     if (STAGES > 1) {                                                                \
       _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1, smem + kStage);  \
-      if (!ALIGNED) {                                                                \
-        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, smem + kStage);  \
-      }                                                                              \
       all_but<kLoads * LOADS_EACH>();                                                \
     } else {                                                                         \
       all_landed();                                                                  \
@@ -680,9 +684,6 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       mul(0, 0, 0, kLoads - kFirst, [&](int i) {                                     \
         if (more) LOAD(kFirst + i, st + 1, other);                                   \
       });                                                                            \
-      if (!ALIGNED && more) {                                                        \
-        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, other);          \
-      }                                                                              \
       if (PREPARES && st > 0) NEXT(st + 2);                                          \
       if (kHalves == 2) {                                                            \
         read_q(buf, 1, 1);                                                           \
@@ -701,6 +702,54 @@ __device__ __forceinline__ void fetch(const T* row, int64_t c, int64_t cols, cha
       mul(1, kLast, 1, kFirst, [&](int i) {                                          \
         if (refill) LOAD(i, st + 2, buf);                                            \
       });                                                                            \
+    }                                                                                \
+  }
+
+// The same for operands of any alignment, which go through registers: LOAD(i, stage) fetches load i into
+// them, PLACE(i, buffer) writes it to LDS a whole stage later, into the buffer that the barrier before has
+// freed.
+#define MULTIPLY_HELD(STAGES, LOAD, PLACE)                                           \
+  {                                                                                  \
+    constexpr int kStage = kPBytes + kQBytes;                                        \
+    auto none = [](int) {};                                                          \
+    _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 0);                   \
+    _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, smem);               \
+    if (STAGES > 1) {                                                                \
+      _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, 1);                 \
+    }                                                                                \
+    __syncthreads();                                                                 \
+    read_q(smem, 0, 0);                                                              \
+    read_p(smem, 0, 0, 0);                                                           \
+    for (int st = 0; st < STAGES; ++st) {                                            \
+      char* buf = smem + (st & 1) * kStage;                                          \
+      char* other = smem + ((st + 1) & 1) * kStage;                                  \
+      if (kHalves == 2) {                                                            \
+        read_p(buf, 0, 1, 1);                                                        \
+      } else {                                                                       \
+        read_q(buf, 1, 1);                                                           \
+        read_p(buf, 1, 0, 1);                                                        \
+      }                                                                              \
+      mul(0, 0, 0, 0, none);                                                         \
+      if (st + 1 < STAGES) {                                                         \
+        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) PLACE(i, other);          \
+      }                                                                              \
+      if (st + 2 < STAGES) {                                                         \
+        _Pragma("unroll") for (int i = 0; i < kLoads; ++i) LOAD(i, st + 2);          \
+      }                                                                              \
+      if (kHalves == 2) {                                                            \
+        read_q(buf, 1, 1);                                                           \
+        read_p(buf, 1, 0, 0);                                                        \
+        mul(0, 1, 1, 0, none);                                                       \
+        read_p(buf, 1, 1, 1);                                                        \
+        mul(1, 0, 0, 0, none);                                                       \
+      }                                                                              \
+      __syncthreads();                                                               \
+      if (st + 1 < STAGES) {                                                         \
+        read_q(other, 0, 0);                                                         \
+        read_p(other, 0, 0, 0);                                                      \
+      }                                                                              \
+      constexpr int kLast = kHalves == 2 ? 1 : 0;                                    \
+      mul(1, kLast, 1, 0, none);                                                     \
     }                                                                                \
   }
 
@@ -763,7 +812,9 @@ __device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, in
 // 42 000 rows, 21 groups, 1000 -> 256 float32: 239 us forward (64 x 64 tiles) and 245 dx (128 x 128), 90
 // TFLOP/s where a large library product reaches 154; the products alone 190 and 220 us, because 2.6 and
 // 5.5 rounds of the card take 3 and 6.
-// Rows that are not 16-byte pieces (ALIGNED false): 5003 rows, 37 groups, 193 -> 317 fp16 13 us each.
+// Rows that are not 16-byte pieces (ALIGNED false): 5003 rows, 37 groups, 193 -> 317 fp16 11 us each, 24 340 rows,
+// 3 groups, 423 -> 1566 fp16 96 us forward and 151 dx (of 424 -> 1568 columns 68 and 60): bound by the
+// instructions that put their pieces together.
 template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
   constexpr int kThreads = WM * WN * 64, kWaves = WM * WN;
@@ -902,7 +953,12 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     };
     auto next = [](int) {};
-    MULTIPLY_STAGES(stages, load, place, next, false, 1)
+    if constexpr (ALIGNED) {
+      MULTIPLY_STAGES(stages, load, next, false, 1)
+    } else {
+      auto fill = [&](int i, int st) { load(i, st, smem); };
+      MULTIPLY_HELD(stages, fill, place)
+    }
   } else {
     __syncthreads();
   }
@@ -1274,6 +1330,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
       // load i: dy's and x's granules of one row
       constexpr int kLoads = kPLoads;
       u32x4 held[ALIGNED ? 1 : 2 * kLoads];
+      const bool inside = m0 + BM <= a.out && n0 + BN <= a.k;
+      // (through registers: each lane fetches its rows' numbers itself, a stage ahead)
+      int rid[ALIGNED ? 1 : kLoads];
+      auto row_of = [&](int i, int64_t st) {
+        const int64_t pos = r0 + place_of(st) * kK + ((i * kWaves + wave) * 64 + lane) / kPRow;
+        if (st >= stages || pos >= r1) return -1;
+        return a.order ? a.order[pos] : (int)pos;
+      };
       auto load = [&](int i, int64_t st, char* buf) {
         const int q0 = (i * kWaves + wave) * 64;
         const int64_t first = r0 + place_of(st) * kK;
@@ -1293,7 +1357,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         asm volatile("" : "+v"(q));   // (worked out at each load: there are no registers to keep it in)
         const int k = q / kPRow, s = q % kPRow;
         int r = (int)first + k;
-        if (a.order) r = ids[(st & 1) * 64 + k];
+        if constexpr (!ALIGNED) r = rid[i];
+        else if (a.order) r = ids[(st & 1) * 64 + k];
         const bool in = k < r1 - first && (unsigned)r < (unsigned)a.g.n;
         const int cd = m0 + (s ^ across_swap_p<T, BM>(k)) * kV, cx = n0 + (s ^ across_swap_q<T, BN>(k)) * kV;
         const T* rd = static_cast<const T*>(a.dy) + (int64_t)r * a.ld_dy;
@@ -1301,6 +1366,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         if constexpr (ALIGNED) {
           fetch<T>(in ? rd : nullptr, cd, a.out, buf + q0 * 16);
           fetch<T>(in ? rx : nullptr, cx, a.k, buf + kPBytes + q0 * 16);
+        } else if (inside) {
+          __builtin_memcpy(&held[2 * i], in ? reinterpret_cast<const char*>(rd + cd) : zero, 16);
+          __builtin_memcpy(&held[2 * i + 1], in ? reinterpret_cast<const char*>(rx + cx) : zero, 16);
         } else {
           held[2 * i] = granule_of<T>(in ? rd : nullptr, cd, a.out);
           held[2 * i + 1] = granule_of<T>(in ? rx : nullptr, cx, a.k);
@@ -1340,7 +1408,17 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      MULTIPLY_STAGES(stages, load, place, look, true, 2)
+      if constexpr (ALIGNED) {
+        MULTIPLY_STAGES(stages, load, look, true, 2)
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) rid[i] = row_of(i, 0);
+        auto fill = [&](int i, int64_t st) {
+          load(i, st, smem);
+          rid[i] = row_of(i, st + 1);
+        };
+        MULTIPLY_HELD(stages, fill, place)
+      }
       __syncthreads();   // the buffers are free for the next run's loads
     }
     done += run;
@@ -1495,11 +1573,11 @@ constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.85};
 
 // The tile with the least time for `tiles(size)` tiles: rounds of the card times a round's work.
 template <typename F>
-int pick_tile(int type, F tiles) {
+int pick_tile(int type, bool aligned, F tiles) {
   const double* rate = type == IC_F32 ? kRate32 : kRate16;
   int best = 2;
   double least = 1e300;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = aligned ? 0 : 1; i < 3; ++i) {
     const int64_t slots = (int64_t)kCUs * kPerCu[i];
     const int64_t rounds = (tiles(kTileSize[i]) + slots - 1) / slots;
     const double t = (double)rounds * kPerCu[i] * kTileSize[i] * kTileSize[i] / rate[i];
@@ -1547,17 +1625,19 @@ hipError_t rows_typed(const RowsArgs& a, int type, bool aligned, hipStream_t s) 
   if constexpr (QALONG)
     if (a.g.n <= 8 * a.g.groups || a.g.n <= 32 || (idle && a.depth >= 512))
       return aligned ? few_launch<T, true, true>(a, s) : few_launch<T, true, false>(a, s);
-  if (!aligned) return rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
   // rows of at most 512 bytes whose tiles would be 64 x 64 anyway (fewer columns, or short groups)
   const int64_t row_bytes = (int64_t)a.depth * (int)sizeof(T);
-  if (row_bytes <= 512 && (a.cols <= 64 || a.g.n < 128 * a.g.groups)) {
+  if (aligned && row_bytes <= 512 && (a.cols <= 64 || a.g.n < 128 * a.g.groups)) {
     if (row_bytes <= 128) return short_launch<T, 1, QALONG>(a, s);
     if (row_bytes <= 256) return short_launch<T, 2, QALONG>(a, s);
     return short_launch<T, 4, QALONG>(a, s);
   }
-  const int tile = pick_tile(type, [&](int size) {
+  const int tile = pick_tile(type, aligned, [&](int size) {
     return (a.g.n / size + a.g.groups) * ((a.cols + size - 1) / size);
   });
+  if (!aligned)
+    return tile == 1 ? rows_launch<T, 128, 128, 2, 2, QALONG, false>(a, s)
+                     : rows_launch<T, 64, 64, 4, 1, QALONG, false>(a, s);
   if (tile == 0) return rows_launch<T, 256, 256, 2, 4, QALONG, true>(a, s);
   if (tile == 1) return rows_launch<T, 128, 128, 2, 2, QALONG, true>(a, s);
   return rows_launch<T, 64, 64, 4, 1, QALONG, true>(a, s);
@@ -1588,7 +1668,7 @@ DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned
   // So few rows that a tile has at most five stages: whole tiles, nothing cut and nothing joined (128 rows,
   // 1 group of 1024 x 1024 float32: 21 -> 10 us with the call).
   const bool whole = n <= 4 * kk;
-  for (int i = aligned ? 0 : 2; i < 3; ++i) {
+  for (int i = aligned ? 0 : 1; i < 3; ++i) {
     const int size = kTileSize[i];
     const double tiles = (double)((out + size - 1) / size) * ((k + size - 1) / size);
     const double line = ((double)(n / kk) + groups) * tiles;
@@ -1641,7 +1721,8 @@ hipError_t dw_launch(DwArgs a, hipStream_t s) {
 
 template <typename T>
 hipError_t dw_typed(const DwArgs& a, int tile, bool aligned, hipStream_t s) {
-  if (!aligned) return dw_launch<T, 64, 64, 4, 1, false>(a, s);
+  if (!aligned)
+    return tile == 1 ? dw_launch<T, 128, 128, 2, 2, false>(a, s) : dw_launch<T, 64, 64, 4, 1, false>(a, s);
   if (tile == 0) return dw_launch<T, 256, 256, 2, 4, true>(a, s);
   if (tile == 1) return dw_launch<T, 128, 128, 2, 2, true>(a, s);
   return dw_launch<T, 64, 64, 4, 1, true>(a, s);
@@ -1655,6 +1736,9 @@ hipError_t allow(Kernel kernel, int bytes) {
 template <typename T>
 hipError_t allow_typed() {
   hipError_t e = allow(k_grouped_rows<T, 128, 128, 2, 2, true, true>, rows_lds<128, 128>());
+  if (e == hipSuccess) e = allow(k_grouped_rows<T, 128, 128, 2, 2, true, false>, rows_lds<128, 128>());
+  if (e == hipSuccess) e = allow(k_grouped_rows<T, 128, 128, 2, 2, false, false>, rows_lds<128, 128>());
+  if (e == hipSuccess) e = allow(k_grouped_dw<T, 128, 128, 2, 2, false>, rows_lds<128, 128>());
   if (e == hipSuccess) e = allow(k_grouped_rows<T, 128, 128, 2, 2, false, true>, rows_lds<128, 128>());
   if (e == hipSuccess) e = allow(k_grouped_dw<T, 128, 128, 2, 2, true>, rows_lds<128, 128>());
   if (e == hipSuccess) e = allow(k_grouped_rows<T, 256, 256, 2, 4, true, true>, rows_lds<256, 256>());

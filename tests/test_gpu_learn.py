@@ -293,6 +293,20 @@ def test_tiles_cut_into_many_pieces(n, groups, k, out, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, groups, k, out", [(30_000, 3, 261, 385), (17_001, 2, 131, 258)])
+def test_large_tiles_of_rows_of_any_alignment(n, groups, k, out, t):
+    # widths that end inside a 16-byte piece, in tiles of 128 x 128; rows of no group hold NaN
+    codes, x, dy, w = group_case(n, groups, k, out, t, 31)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    none = codes < 0
+    x[none], dy[none] = math.nan, math.nan
+    close(ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32), *ref["y"], k, "y")
+    close(ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32), *ref["dx"], out, "dx")
+    close(ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32), *ref["dw"], n, "dw")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("n, groups, k, out", [(30_000, 700, 32, 600), (40_000, 8000, 24, 40), (3000, 8200, 16, 33)])
 def test_many_short_rows(n, groups, k, out, t):
     # workgroups of 128 short rows: groups that end in their first, second or no half
