@@ -1241,6 +1241,19 @@ __device__ __forceinline__ DwPlace dw_place(const DwArgs& a, int64_t u, int64_t 
   return p;
 }
 
+// From a place to the first stage of the next tile, without a search; false behind the last group.
+__device__ __forceinline__ bool dw_next(const DwArgs& a, DwPlace& p, int64_t kk) {
+  p.stage = 0;
+  if (++p.tile < a.tiles) return true;
+  p.tile = 0;
+  if (++p.e >= a.g.groups) return false;
+  p.o0 = uniform(a.g.at(p.e));
+  p.o1 = uniform(a.g.at(p.e + 1));
+  if (p.o1 < p.o0) p.o1 = p.o0;
+  p.stages = p.o1 / kk + 1 - p.o0 / kk;
+  return true;
+}
+
 // The unit that workgroup w's run begins with (and w - 1's ends before).  Whole tiles: the first unit of a
 // tile, an equal number of tiles each.
 __device__ __forceinline__ int64_t dw_begin(const DwArgs& a, int64_t line, int64_t w, int64_t kk) {
@@ -1275,8 +1288,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
   const int pplace = across_place<T, BM, false>(pc, lane);
   const int qplace = kPBytes + across_place<T, BN, true>(qc, lane);
   int* ids = reinterpret_cast<int*>(smem + 2 * (kPBytes + kQBytes));   // [2][kK] rows of a stage
-  for (int64_t done = 0; u < u1;) {
-    const DwPlace pl = dw_place(a, u, kK, lane);
+  if (u >= u1) return;
+  DwPlace pl = dw_place(a, u, kK, lane);
+  for (int64_t done = 0;;) {
     const int64_t run = pl.stages - pl.stage < u1 - u ? pl.stages - pl.stage : u1 - u;
     u += run;
     const int m0 = pl.tile / a.k_tiles * BM, n0 = pl.tile % a.k_tiles * BN;
@@ -1439,6 +1453,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_dw(DwArgs a) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) part[(i * FN + j) * kThreads] = acc[i][j];
     }
+    if (u >= u1 || !dw_next(a, pl, kK)) break;
   }
 }
 
