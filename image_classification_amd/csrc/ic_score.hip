@@ -245,7 +245,7 @@ template <> __device__ __forceinline__ float value16<f16_t>(unsigned k) {
 template <> __device__ __forceinline__ float value16<float>(unsigned) { return 0.0f; }
 
 // Rows of up to 64 * NC granules: one wave a row, the row stays in registers between the maximum,
-// the sums and the ranking.  100 000 rows of 1000 bf16 scores with the best five: 87 us, 2.4 TB/s: bound by
+// the sums and the ranking.  100 000 rows of 1000 bf16 scores with the best five: 69 us, 3.0 TB/s: bound by
 // its vector instructions (reading the row is 40 us; ranked as 32-bit words with an index each 111 us).
 template <typename T, int NC, bool TOP>
 __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
@@ -341,8 +341,12 @@ __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {
         Best2 q = {0u, 0u, -1, -1};
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
+          // (16 bits: rows with NaN.  Opaque: unpacked here, not kept in registers from the sums on, which
+          // would cost the usual path its waves)
+          u32x4 own = raw[i];
+          if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(own));
           float x[kV];
-          Elem<T>::unpack(raw[i], x);
+          Elem<T>::unpack(own, x);
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
             const int idx = index_at(i, j);
@@ -717,8 +721,14 @@ hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) 
       hipLaunchKernelGGL((k_score_wave<T, 1, TOP>), by4, dim3(256), 0, s, a);
     } else if (granules <= 128) {
       hipLaunchKernelGGL((k_score_wave<T, 2, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 192) {
+      hipLaunchKernelGGL((k_score_wave<T, 3, TOP>), by4, dim3(256), 0, s, a);
     } else if (granules <= 256) {
       hipLaunchKernelGGL((k_score_wave<T, 4, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 320) {
+      hipLaunchKernelGGL((k_score_wave<T, 5, TOP>), by4, dim3(256), 0, s, a);
+    } else if (granules <= 384) {
+      hipLaunchKernelGGL((k_score_wave<T, 6, TOP>), by4, dim3(256), 0, s, a);
     } else if (granules <= 512) {
       hipLaunchKernelGGL((k_score_wave<T, 8, TOP>), by4, dim3(256), 0, s, a);
     } else if (TOP && sizeof(T) == 4 && granules <= 1024 && n >= kManyRows) {

@@ -415,8 +415,8 @@ def check_scores(z, labels, top, temperature, zd=None, ld=None):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
-@pytest.mark.parametrize("n,v", [(1, 1), (5, 2), (3, 7), (9, 64), (4, 255), (7, 257), (33, 1000), (5, 1023),
-                                 (3, 2041), (2, 4090), (5, 4099), (3, 10007), (1, 65536), (2, 100001)])
+@pytest.mark.parametrize("n,v", [(1, 1), (5, 2), (3, 7), (9, 64), (4, 255), (7, 257), (9, 700), (33, 1000), (5, 1023),
+                                 (5, 1300), (3, 1500), (3, 2041), (3, 2500), (3, 3060), (2, 4090), (5, 4099), (3, 10007), (1, 65536), (2, 100001)])
 @pytest.mark.parametrize("top,masked,temperature", [(0, 0.0, 1.0), (1, 0.3, 0.7), (5, 0.0, 1.0), (32, 0.9, 2.0)])
 def test_label_logprobs(n, v, t, top, masked, temperature):
     z, labels = masked_scores(n, v, t, n * 13 + v, masked)
