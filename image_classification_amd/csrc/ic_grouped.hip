@@ -805,14 +805,14 @@ __device__ __forceinline__ void store16(void* y, int64_t at, int c, int cols, in
 }
 
 // forward (QALONG: W_g [cols][depth]) and dx (W_g [depth][cols])
-// 65 536 rows, 16 groups of 2048 x 2048 bf16, 256 x 256 tiles: 600 us forward and 625 dx, 920 and 880
+// 65 536 rows, 16 groups of 2048 x 2048 bf16, 256 x 256 tiles: 592 us forward and 611 dx, 930 and 900
 // TFLOP/s (a large library product reaches 1280).  The products alone, with neither loads nor LDS reads,
 // take 440 us (the clock falls to about 2.2 GHz under them, and some 2100 tiles make 9 rounds of 256 CUs
 // where 8.2 would do); the LDS reads cost 80 us more, the loads as much again.
-// 42 000 rows, 21 groups, 1000 -> 256 float32: 239 us forward (64 x 64 tiles) and 245 dx (128 x 128), 90
+// 42 000 rows, 21 groups, 1000 -> 256 float32: 237 us forward (64 x 64 tiles) and 243 dx (128 x 128), 90
 // TFLOP/s where a large library product reaches 154; the products alone 190 and 220 us, because 2.6 and
 // 5.5 rounds of the card take 3 and 6.
-// Rows that are not 16-byte pieces (ALIGNED false): 5003 rows, 37 groups, 193 -> 317 fp16 11 us each, 24 340 rows,
+// Rows that are not 16-byte pieces (ALIGNED false): 5003 rows, 37 groups, 193 -> 317 fp16 10.4 and 10.8 us, 24 340 rows,
 // 3 groups, 423 -> 1566 fp16 96 us forward and 151 dx (of 424 -> 1568 columns 68 and 60): bound by the
 // instructions that put their pieces together.
 template <typename T, int BM, int BN, int WM, int WN, bool QALONG, bool ALIGNED>
@@ -973,7 +973,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 // of 64 R x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
 // goes to LDS, shared by the four waves; each wave's 16 R rows go straight to the registers that the
 // products take them from.  One barrier, one memory latency behind the search for the group.
-// 1M rows x 128 float32, 10 000 groups of 64 x 128: 321 us (R = 1: 343), 3.4 TB/s of rows, matrices and results and
+// 1M rows x 128 float32, 10 000 groups of 64 x 128: 321 to 331 us (R = 1: 343), 3.4 TB/s of rows, matrices and results and
 // 48 TFLOP/s (staged like the longer ones 355 us).  Neither is at its limit (memory 0.21 ms, products
 // 0.11 ms): a workgroup loads, multiplies and stores once, and what four of them a CU overlap is part
 // of it.
@@ -1079,7 +1079,7 @@ __global__ __launch_bounds__(256, R == 1 ? 5 : 3) void k_grouped_short(RowsArgs 
 // shared, so nothing goes through LDS on the way.  BYDEPTH: the four waves share the depth of the same
 // 32 columns and add their sums in LDS, in wave order; otherwise (short rows) each wave takes 16 columns
 // of its own.  A lane's granules of a chunk are neighbours (32 bytes), four lanes read 128 bytes.
-// 16 rows, 64 groups of 2048 x 2048 bf16 (about 14 of them met, 118 MB): 28.8 us, 4.1 TB/s (through LDS 36 us);
+// 16 rows, 64 groups of 2048 x 2048 bf16 (about 14 of them met, 118 MB): 27.5 us, 4.3 TB/s (through LDS 36 us);
 // 1000 rows, 1000 groups of 64 x 128 float32 (21 MB): 10.6 us.
 // QALONG false (dx of float32, by depth only): the matrix's granules are gathered from four of its rows, 16
 // neighbouring columns a load; for launches that latency bounds (18 rows, 3 groups of 1336 x 184: 39.6 -> 13.4
@@ -1199,8 +1199,9 @@ __global__ __launch_bounds__(256) void k_grouped_few(RowsArgs a) {
 // stored at once; the pieces of one that is cut go to float32 partial results -- at most two a
 // workgroup: of the tile its run begins inside (number 2 w) and of the one it ends inside (2 w + 1) --
 // and k_grouped_dw_join adds them in the order of the line.
-// 65 536 rows, 16 groups of 2048 x 2048 bf16: 737 us and 41 to join, 710 TFLOP/s together; without loads
-// 510 us, without LDS reads either 475.  42 000 rows, 21 groups of 256 x 1000 float32: 237 + 21 us.
+// 65 536 rows, 16 groups of 2048 x 2048 bf16: 721 us and 46 to join, 720 TFLOP/s together; without loads
+// 510 us, without LDS reads either 475.  42 000 rows, 21 groups of 256 x 1000 float32: 236 + 21 us.  5003 rows,
+// 37 groups of 317 x 193 fp16: 18 + 9 us.
 struct DwArgs {
   const void* dy;
   const void* x;

@@ -245,7 +245,7 @@ template <> __device__ __forceinline__ float value16<f16_t>(unsigned k) {
 template <> __device__ __forceinline__ float value16<float>(unsigned) { return 0.0f; }
 
 // Rows of up to 64 * NC granules: one wave a row, the row stays in registers between the maximum,
-// the sums and the ranking.  100 000 rows of 1000 bf16 scores with the best five: 69 us, 3.0 TB/s: bound by
+// the sums and the ranking.  100 000 rows of 1000 bf16 scores with the best five: 69 to 74 us, 2.9 TB/s: bound by
 // its vector instructions (reading the row is 40 us; ranked as 32-bit words with an index each 111 us).
 template <typename T, int NC, bool TOP>
 __global__ __launch_bounds__(256) void k_score_wave(ScoreArgs a) {

@@ -1295,7 +1295,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
         kinds = [_ADAMW_TYPES[pair] for pair in zip(map(_dtype, params), map(_dtype, grads))]
     except KeyError:
         raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
-    starts = list(itertools.accumulate([-(-n // ADAMW_BLOCK) * ADAMW_BLOCK for n in sizes], initial=0))
+    starts = list(itertools.accumulate([n + ADAMW_BLOCK - 1 & -ADAMW_BLOCK for n in sizes], initial=0))
     at = starts.pop()
     size = exp_avg.shape[0]
     if at != size:
