@@ -307,7 +307,8 @@ def test_large_tiles_of_rows_of_any_alignment(n, groups, k, out, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
-@pytest.mark.parametrize("n, groups, k, out", [(30_000, 700, 32, 600), (40_000, 8000, 24, 40), (3000, 8200, 16, 33)])
+@pytest.mark.parametrize("n, groups, k, out", [(30_000, 700, 32, 600), (40_000, 8000, 24, 40), (3000, 8200, 16, 33),
+                                               (30_000, 8100, 40, 24)])
 def test_many_short_rows(n, groups, k, out, t):
     # workgroups of 128 short rows: groups that end in their first, second or no half
     codes, x, dy, w = group_case(n, groups, k, out, t, 21)
@@ -481,6 +482,13 @@ def test_short_rows_of_scores_with_ties(t, v):
     assert int(ti[n - 1, 0]) == v - 1 and int(ti[n - 3, 0]) == 0
     logp2, ent2, lse2, _, ti2 = ops.label_logprobs(z.to(DEV), torch.zeros(n, dtype=torch.int32, device=DEV), top=1)
     assert torch.equal(lse[~rows], lse2[~rows]) and torch.equal(ti[~rows], ti2[~rows])
+
+
+def test_more_rows_than_one_launch_takes():
+    n, v = (1 << 22) + 77, 3
+    g = torch.Generator().manual_seed(5)
+    z = torch.randn(n, v, generator=g)
+    check_scores(z, torch.randint(0, v, (n,), generator=g), 2, 1.0)
 
 
 def test_many_rows_of_float32_scores_a_wave_each():
