@@ -569,6 +569,23 @@ def test_label_logprobs_grad(n, v, t, temperature, masked):
     assert torch.equal(zd, got)
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_a_gradient_larger_than_half_the_last_level_cache(t):
+    # such gradients are stored past it; the rows do not depend on each other, so a few are checked
+    n = (1 << 27) // (2 if t != torch.float32 else 4) // 1001 + 3
+    g = torch.Generator().manual_seed(2)
+    z = (torch.randn(64, 1001, generator=g) * 3).to(t).to(DEV).repeat((n + 63) // 64, 1)[:n]
+    labels = (torch.arange(n) % 1001).int().to(DEV)
+    _, h, lse, _, _ = ops.label_logprobs(z, labels)
+    dl = torch.linspace(-1, 1, n, device=DEV)
+    dh = torch.linspace(2, 0, n, device=DEV)
+    dz = ops.label_logprobs_grad(z, labels, lse, h, dl, dh)
+    for lo in (0, n // 2, n - 70):
+        part = ops.label_logprobs_grad(z[lo:lo + 70], labels[lo:lo + 70], lse[lo:lo + 70], h[lo:lo + 70],
+                                       dl[lo:lo + 70], dh[lo:lo + 70])
+        assert torch.equal(dz[lo:lo + 70], part)
+
+
 def test_label_logprobs_gradient_against_differences():
     g = torch.Generator().manual_seed(8)
     n, v = 6, 50
