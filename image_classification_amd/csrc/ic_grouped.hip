@@ -1684,9 +1684,12 @@ DwPlan dw_plan(int64_t n, int64_t groups, int k, int out, int type, bool aligned
   const double* rate = type == IC_F32 ? kRate32 : kRate16;
   DwPlan best = {2, 1, false};
   double least = 1e300;
-  // So few rows that a tile has at most five stages: whole tiles, nothing cut and nothing joined (128 rows,
-  // 1 group of 1024 x 1024 float32: 21 -> 10 us with the call).
-  const bool whole = n <= 4 * kk;
+  // Whole tiles, nothing cut and nothing joined: where a tile has at most five stages (128 rows, 1 group of
+  // 1024 x 1024 float32: 21 -> 10 us with the call), and up to 128 where there are half as many groups as stages, so that
+  // few tiles are long (4000 rows, 300 groups of 16 x 136 fp16: 20.2 -> 10.4 us, 2000 rows, 20 groups of 64 x 64
+  // bf16 15.0 -> 12.5; but 8000 rows, 20 groups: 15.7 -> 26.4, and 1000 rows, 1 group: 13.7 -> 15.8).
+  const int64_t stages = n / kk;
+  const bool whole = stages <= 4 || (groups >= 4 && stages <= 128 && stages <= (groups > 8 ? 2 * groups : 16));
   for (int i = aligned ? 0 : 1; i < 3; ++i) {
     const int size = kTileSize[i];
     const double tiles = (double)((out + size - 1) / size) * ((k + size - 1) / size);

@@ -280,6 +280,16 @@ def test_few_rows_forward_and_back(n, groups, k, out, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("kind", ["ragged", "last", "none"])
+@pytest.mark.parametrize("n, groups, k, out", [(2000, 50, 72, 40), (1000, 5, 33, 130), (4000, 400, 24, 65)])
+def test_weight_gradients_in_whole_tiles(n, groups, k, out, kind, t):
+    codes, x, dy, w = group_case(n, groups, k, out, t, 41, kind)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    close(ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32), *ref["dw"], n, "dw")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("n, groups, k, out", [(9000, 1, 128, 100), (20_000, 2, 16, 24), (7001, 1, 33, 65)])
 def test_tiles_cut_into_many_pieces(n, groups, k, out, t):
     # few tiles under many rows: a tile's pieces come from dozens of workgroups; the bits repeat
