@@ -453,7 +453,8 @@ constexpr int kPieceWaves = kPieceThreads / 64;
 
 // Longer rows: a workgroup streams one of `pieces` pieces of a row (pieces > 1 where there are too
 // few rows to fill the card; k_score_join then joins them).  4096 rows of 65 536 bf16 scores: 125 to 138 us,
-// 3.9 to 4.3 TB/s (a sum over 1 GiB by the library reads 3.9); 8 rows of 65 536 float32 scores with the
+// 3.9 to 4.3 TB/s (a sum over 1 GiB by the library reads 3.9), 103 us where the last level cache still holds a
+// part of them; 8 rows of 65 536 float32 scores with the
 // best ten: 8.8 us and 4.6 for the join, latency.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kPieceThreads) void k_score_pieces(ScoreArgs a, int pieces,
@@ -645,7 +646,7 @@ struct GradArgs {
 // scores: 190 us by itself, 5.7 TB/s (a copy of 1 GiB: 5.2): bound by memory.
 // Rows are taken from the last to the first: what the pass over the scores read last may still be in the last
 // level cache (324 -> 317 us for both passes).  STREAM, for gradients that cache cannot hold: stores that do not
-// push the scores out of it (-> 298 us).
+// push the scores out of it (-> 298 us when both passes are repeated over the same scores).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, int span) {
   constexpr int kV = Elem<T>::kVec;
