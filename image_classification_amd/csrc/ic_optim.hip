@@ -16,7 +16,9 @@
 //      so the step never divides by eps alone where a gradient was seen.
 // Both roundings are to nearest, an exact middle to the even code, at most 2^-4 (m) and 2^-5
 // (sqrt v) of the value, and the codes are decided in float64 (see k_adamw8): which of two codes a
-// value takes then does not depend on the last bit of a float32 evaluation.
+// value takes then does not depend on the last bit of a float32 evaluation.  A scale that is a float32
+// subnormal (a block's maximum below 6e-36 for m, 6e-33 for sqrt v) is itself off by up to a half, and what
+// then lies above the largest code takes the largest code.
 // The update uses the new m and v before they are rounded.
 //
 // What bounds it: memory with 32-bit states, instructions with 8-bit ones; the figures stand at each
@@ -245,8 +247,11 @@ __device__ __forceinline__ float stepped(float p, float m, double r, const Lane8
 // adamw8_careful decides every code in float64 and handles what is not finite.
 // adamw8_quick is for finite values.  Its codes come from the float64 quotients rounded to float32
 // once: m's by the hardware's conversion to this format (e4m3), v's from the float32 bits.  That is the
-// same code except where the float32 is exactly a middle between two codes (one in 2^19 or so), in
-// which case it returns true and the wave takes the careful way instead.
+// same code except in two cases, in which it returns true and the wave takes the careful way instead:
+// where the float32 is exactly a middle between two codes (one in 2^19 or so), and where a new scale is a
+// float32 subnormal.  Rounding such a scale moves it by up to a half, so the largest quotient may pass the
+// largest code, and neither of these codes is bounded (e4m3 has no number above 464, v's bits run into the
+// next byte); a normal scale moves by 2^-24 at most, which float32 quotients do not see.
 __device__ __forceinline__ void adamw8_careful(const Lane8& s, u32x2 mc, u32x2 vc, const float* g, const float* p,
                                                float* p_out, u32x2* mo, u32x2* vo, float* out_sm, float* out_sv) {
   double m[8], r[8];
@@ -317,7 +322,7 @@ __device__ __forceinline__ bool adamw8_quick(const Lane8& s, u32x2 mc, u32x2 vc,
   const double im = new_sm > 0.0f ? inverse_of((double)new_sm) : 0.0;
   const double iv = new_sv > 0.0f ? inverse_of((double)new_sv) : 0.0;
   const double seen = new_sv > 0.0f ? kSeen : __builtin_inf();
-  bool doubt = false;
+  bool doubt = (new_sm > 0.0f && new_sm < 0x1p-126f) || (new_sv > 0.0f && new_sv < 0x1p-126f);
   float qm[8];
   *vo = u32x2{0u, 0u};
 #pragma unroll
