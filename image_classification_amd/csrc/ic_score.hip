@@ -21,6 +21,8 @@
 //
 // What bounds it: reading the row once, and the instructions that rank it; the figures stand at each
 // kernel.
+#include <climits>
+
 #include "ic_wave.h"
 
 namespace ic {
@@ -639,23 +641,56 @@ struct GradArgs {
   int64_t ld_out;
 };
 
-// dL/dx_j = ( g (delta_{j,label} - p_j) - h p_j (log p_j + H) ) / T with g = dL/dlogp (0 for a row
-// without a label) and h = dL/dH.  One read of the scores, one write of the gradient (out may be
-// the scores themselves: an element is read before it is written, by the same lane).  A row of few
-// granules is taken by 2^lanes_log2 lanes, 256 >> lanes_log2 rows a workgroup.  4096 rows of 65 536 bf16
-// scores: 190 us by itself, 5.7 TB/s (a copy of 1 GiB: 5.2): bound by memory.
-// Rows are taken from the last to the first: what the pass over the scores read last may still be in the last
-// level cache (324 -> 317 us for both passes).  STREAM, for gradients that cache cannot hold: stores that do not
-// push the scores out of it (-> 298 us when both passes are repeated over the same scores).
-template <typename T, bool STREAM>
-__global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, int span) {
+// p_j = e^(x_j / T - lse) is as good as lse is: rounded to float32 it is off by half its last bit, and p by as
+// much of itself.  Up to this size that is 2^-20 (float32 scores), and 2^-17 where p is rounded to 2^-9 or 2^-12
+// afterwards.  Beyond it (all scores of a row shifted far from zero, rows masked with the type's lowest value)
+// the row is "far": its maximum M and ln s are worked out once more, and log p = (x - M) / T - ln s as in
+// the pass over the scores.
+template <typename T>
+__device__ __forceinline__ bool far_from_zero(float lse) {
+  return fabsf(lse) > (sizeof(T) == 4 ? 32.0f : 256.0f);   // (and infinite; NaN is not)
+}
+// (M, s) of a row from its scores, in all of the row's lanes: lane `sub` of `lanes`, which are part of a wave or
+// the whole workgroup (in which every row is far, then).
+template <typename T, int THREADS>
+__device__ __forceinline__ Stats row_again(const RowView<T>& rv, int total, int sub, int lanes, float c) {
   constexpr int kV = Elem<T>::kVec;
-  const int lanes = 1 << lanes_log2;
-  const int64_t row = a.row0 + ((int64_t)(gridDim.x - 1 - blockIdx.x) << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
-  if (row >= a.n) return;
+  __shared__ float sm[THREADS / 64], ss[THREADS / 64];
+  Stats st = {kLowest, 0.0f, 0.0f};
+  for (int q = sub; q < total; q += lanes) {
+    float x[kV];
+    rv.get(q, x);
+    add_values<kV>(st, x, c);
+  }
+  const int within = lanes < 64 ? lanes : 64;
+  float m = st.m;
+  for (int o = 1; o < within; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  rescale(st, m, c);
+  for (int o = 1; o < within; o <<= 1) st.s += __shfl_xor(st.s, o, 64);
+  if (lanes > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      sm[threadIdx.x >> 6] = st.m;
+      ss[threadIdx.x >> 6] = st.s;
+    }
+    __syncthreads();   // (and no score is overwritten before all of the row have been read)
+    for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, sm[w]);
+    st.m = m;
+    st.s = 0.0f;
+    for (int w = 0; w < THREADS / 64; ++w) st.s += ss[w] * __builtin_amdgcn_exp2f(gap(sm[w], m) * c);
+  }
+  return st;
+}
+
+// dL/dx_j = ( g (delta_{j,label} - p_j) - h p_j (log p_j + H) ) / T with g = dL/dlogp (0 for a row
+// without a label) and h = dL/dH, for granules [g0, g1) of a row, by lane `sub` of `lanes`.  One read of the scores
+// (two where `again`: the row is far), one write of the gradient (out may be the scores themselves: an element is
+// read before it is written, by the same lane).
+template <typename T, bool STREAM, int THREADS>
+__device__ __forceinline__ void grad_row(const GradArgs& a, int64_t row, float lse, bool again, int sub, int lanes,
+                                         int g0, int span) {
+  constexpr int kV = Elem<T>::kVec;
   const T* xr = static_cast<const T*>(a.logits) + row * a.ld;
   T* yr = static_cast<T*>(a.out) + row * a.ld_out;
-  const float lse = a.lse[row];
   int64_t l = -1;
   if (a.labels && a.d_logp)
     l = a.labels64 ? static_cast<const int64_t*>(a.labels)[row]
@@ -664,21 +699,27 @@ __global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, 
   const float g = label >= 0 ? a.d_logp[row] : 0.0f;
   const float h = a.d_entropy ? a.d_entropy[row] : 0.0f;
   const float H = a.d_entropy ? a.entropy[row] : 0.0f;
-  const bool none = lse == -__builtin_inff();
   const RowView<T> rv(xr, a.v);
   const int total = rv.granules();
-  const int g0 = (int)blockIdx.y * span;
   const int g1 = total - g0 < span ? total : g0 + span;
+  float m0 = 0.0f, l0 = lse;           // log p = (x - m0) / T - l0
+  bool none = false;                   // nothing but -inf
+  if (again) {
+    const Stats st = row_again<T, THREADS>(rv, total, sub, lanes, a.inv_t * kLog2e);
+    none = st.s == 0.0f;
+    m0 = st.m;
+    l0 = none ? 0.0f : __builtin_amdgcn_logf(st.s) * kLn2;
+  }
   // the output row starts at the same place of a granule as the input row
   const bool same = (reinterpret_cast<uintptr_t>(yr) & 15) == (reinterpret_cast<uintptr_t>(xr) & 15);
   char* yb = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(yr) & ~(uintptr_t)15);
-  for (int q = g0 + ((int)threadIdx.x & (lanes - 1)); q < g1; q += lanes) {
+  for (int q = g0 + sub; q < g1; q += lanes) {
     float x[kV];
     rv.get(q, x);
     const int j0 = q * kV - rv.head;
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      const float lq = fmaxf(fmaf(x[i], a.inv_t, -lse), kFar) + 0.0f * lse;
+      const float lq = fmaxf(fmaf(x[i] - m0, a.inv_t, -l0), kFar) + 0.0f * l0;
       const float p = __builtin_amdgcn_exp2f(lq * kLog2e);
       float d = -p * fmaf(h, lq + H, g);
       d = (j0 + i == label ? d + g : d) * a.inv_t;
@@ -692,6 +733,48 @@ __global__ __launch_bounds__(256) void k_score_grad(GradArgs a, int lanes_log2, 
 #pragma unroll
       for (int i = 0; i < kV; ++i)
         if (j0 + i >= 0 && j0 + i < a.v) Elem<T>::store(yr + j0 + i, x[i]);
+    }
+  }
+}
+
+// Whole rows: 2^lanes_log2 lanes of a wave a row, or a workgroup.  Rows are taken from the last to the first, here
+// and below: what the pass over the scores read last may still be in the last level cache (4096 rows of 65 536 bf16
+// scores, 324 -> 317 us for both passes).  STREAM, for gradients that cache cannot hold: stores that do not push the
+// scores out of it (-> 298 us when both passes are repeated over the same scores).
+template <typename T, bool STREAM, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_score_grad(GradArgs a, int lanes_log2) {
+  constexpr int kThreadsLog2 = THREADS == 1024 ? 10 : 8;
+  const int lanes = 1 << lanes_log2;
+  const int64_t row = a.row0 + ((int64_t)(gridDim.x - 1 - blockIdx.x) << (kThreadsLog2 - lanes_log2)) +
+                      (threadIdx.x >> lanes_log2);
+  if (row >= a.n) return;
+  const float lse = a.lse[row];
+  grad_row<T, STREAM, THREADS>(a, row, lse, far_from_zero<T>(lse), (int)threadIdx.x & (lanes - 1), lanes, 0, INT_MAX);
+}
+
+// Long rows in pieces of `span` granules, a workgroup each.  It leaves far rows to k_score_grad_far, in a launch behind
+// it: none of several workgroups could read a row that the others already write to.  4096 rows of 65 536 bf16
+// scores: bound by memory; 190 to 209 us, 5.1 to 5.7 TB/s (a copy of 1 GiB: 5.2), by what the last level cache holds.
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(256) void k_score_grad_near(GradArgs a, int span) {
+  const int64_t row = a.row0 + (gridDim.x - 1 - blockIdx.x);
+  const float lse = a.lse[row];
+  if (far_from_zero<T>(lse)) return;
+  grad_row<T, STREAM, 256>(a, row, lse, false, threadIdx.x, 256, (int)blockIdx.y * span, span);
+}
+
+// The far rows among the long ones: a workgroup looks at every gridDim.x-th row, 64 at a time.
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(1024) void k_score_grad_far(GradArgs a) {
+  for (int64_t row0 = a.row0 + blockIdx.x; row0 < a.n; row0 += 64 * (int64_t)gridDim.x) {
+    const int64_t mine = row0 + (threadIdx.x & 63) * (int64_t)gridDim.x;
+    const float lse = mine < a.n ? a.lse[mine] : 0.0f;
+    unsigned long long far = __ballot(far_from_zero<T>(lse));   // (the same in every wave)
+    while (far) {
+      const int64_t row = row0 + (__ffsll(far) - 1) * (int64_t)gridDim.x;
+      far &= far - 1;
+      grad_row<T, STREAM, 1024>(a, row, 0.0f, true, threadIdx.x, 1024, 0, INT_MAX);
+      __syncthreads();   // (row_again's LDS is free)
     }
   }
 }
@@ -755,29 +838,49 @@ hipError_t score_launch(ScoreArgs a, int pieces, unsigned* part, hipStream_t s) 
   return hipSuccess;
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 hipError_t grad_launch(GradArgs a, hipStream_t s) {
   const int64_t granules = ((int64_t)a.v + 2 * Elem<T>::kVec - 2) / Elem<T>::kVec;
   int lanes_log2 = 1;
   while (lanes_log2 < 8 && (1 << lanes_log2) < granules) ++lanes_log2;
-  // a workgroup takes 2048 granules of a row, fewer when that leaves CUs without work
-  int64_t span = 2048;
-  while (span > 256 && a.n * ((granules + span - 1) / span) < 8 * (int64_t)kCUs) span /= 2;
-  while ((granules + span - 1) / span > 65535) span *= 2;
-  const unsigned y = (unsigned)((granules + span - 1) / span);
+  // (lanes of one wave, or the whole workgroup; 128 were slower anyway: 100 000 rows of 1000 bf16 74 -> 66 us)
+  if (lanes_log2 == 7) lanes_log2 = 6;
   const int64_t n = a.n;
-  // half of the last level cache: a smaller gradient is left there for who reads it next
-  const bool stream = n * a.v > ((int64_t)128 << 20) / (int64_t)sizeof(T);
+  const bool many = n >= kManyRows;
+  // A workgroup a row while a lane has few granules of it; of 1024 lanes where there are few rows (1000 rows of 16 384
+  // bf16: 13.0 us, with 256 lanes 14.5; 64 rows of 8192: 3.3, in pieces with the launch for the far ones 4.3)
+  const bool whole = granules <= 4096;
+  // else pieces (4096 rows of 65 536 bf16: 209 us, a workgroup a row 216) of 2048 granules, fewer when that leaves CUs
+  // without work
+  int64_t span = 2048;
+  while (span > 256 && n * ((granules + span - 1) / span) < 8 * (int64_t)kCUs) span /= 2;
+  while ((granules + span - 1) / span > 65535) span *= 2;
   for (a.row0 = 0; a.row0 < n; a.row0 += kRowsPerLaunch) {
     const int64_t rows = n - a.row0 < kRowsPerLaunch ? n - a.row0 : kRowsPerLaunch;
     a.n = a.row0 + rows;
-    const int64_t per_wg = 256 >> lanes_log2;
-    hipLaunchKernelGGL((stream ? k_score_grad<T, true> : k_score_grad<T, false>), dim3((unsigned)((rows + per_wg - 1) / per_wg), y), dim3(256), 0,
-                       s, a, lanes_log2, (int)span);
+    if (granules <= 256 || (whole && many)) {
+      const int64_t per_wg = 256 >> lanes_log2;
+      hipLaunchKernelGGL((k_score_grad<T, STREAM, 256>), dim3((unsigned)((rows + per_wg - 1) / per_wg)), dim3(256), 0,
+                         s, a, lanes_log2);
+    } else if (whole) {
+      hipLaunchKernelGGL((k_score_grad<T, STREAM, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, a, 10);
+    } else {
+      hipLaunchKernelGGL((k_score_grad_near<T, STREAM>), dim3((unsigned)rows, (unsigned)((granules + span - 1) / span)),
+                         dim3(256), 0, s, a, (int)span);
+      hipLaunchKernelGGL((k_score_grad_far<T, STREAM>), dim3((unsigned)(rows < 2 * kCUs ? rows : 2 * kCUs)), dim3(1024),
+                         0, s, a);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+template <typename T>
+hipError_t grad_typed(const GradArgs& a, hipStream_t s) {
+  // half of the last level cache: a smaller gradient is left there for who reads it next
+  const bool stream = a.n * a.v > ((int64_t)128 << 20) / (int64_t)sizeof(T);
+  return stream ? grad_launch<T, true>(a, s) : grad_launch<T, false>(a, s);
 }
 
 }  // namespace
@@ -817,9 +920,9 @@ hipError_t launch_label_logprobs_grad(const void* logits, int dtype, int64_t ld,
                                       const float* d_entropy, void* out, int64_t ld_out, hipStream_t s) {
   const GradArgs a{logits, ld, 0, n, (int)v, labels, labels64, inv_t, lse, entropy, d_logp, d_entropy, out,
                    ld_out};
-  if (dtype == IC_F32) return grad_launch<float>(a, s);
-  if (dtype == IC_BF16) return grad_launch<bf16_t>(a, s);
-  return grad_launch<f16_t>(a, s);
+  if (dtype == IC_F32) return grad_typed<float>(a, s);
+  if (dtype == IC_BF16) return grad_typed<bf16_t>(a, s);
+  return grad_typed<f16_t>(a, s);
 }
 
 }  // namespace ic

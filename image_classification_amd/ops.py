@@ -1194,7 +1194,9 @@ def label_logprobs_grad(logits, labels, lse, entropy, d_logp=None, d_entropy=Non
     """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to logits, in logits'
     type.  lse and entropy are what label_logprobs returned for the same logits and temperature;
     d_logp / d_entropy float32 [n] (None: zeros).  `out` may be logits itself.  Rows without a
-    label have no gradient through logp; rows of nothing but -inf have none at all."""
+    label have no gradient through logp; rows of nothing but -inf have none at all.  A row whose lse is
+    beyond 32 (float32; 256 for the 16-bit types) is read twice: a float32 lse no longer tells its
+    probabilities there."""
     ld = _check_rows(logits, "logits")
     n, v = logits.shape
     t = _type_number(logits, "logits")

@@ -376,7 +376,9 @@ int ic_label_logprobs(void* handle, const void* logits, int64_t ld, int64_t n, i
                       int64_t scratch_bytes, void* stream);
 /* dlogits = the gradient of sum_i d_logp[i] logp[i] + d_entropy[i] entropy[i], in the scores' type.
  * lse and entropy are what ic_label_logprobs returned; d_logp or d_entropy may be NULL (zeros).
- * out [n][v] with rows ld_out apart may be the scores themselves (same pointer and ld). */
+ * out [n][v] with rows ld_out apart may be the scores themselves (same pointer and ld).  Rows whose |lse| is
+ * above 32 (256 with 16-bit scores) are read twice: their maximum and sum are worked out again, because a
+ * float32 lse of that size does not tell their probabilities. */
 int ic_label_logprobs_grad(void* handle, const void* logits, int64_t ld, int64_t n, int64_t v, int dtype,
                            const void* labels, int labels64, float inv_temperature, const float* lse,
                            const float* entropy, const float* d_logp, const float* d_entropy, void* out,

@@ -74,3 +74,136 @@ def test_states_that_begin_with_subnormal_scales():
     p = torch.zeros(64 * 256, device=DEV)
     for step in range(3, 40):
         step8(p, torch.zeros_like(p), m, v, scales, step, (0.9, 0.9))
+
+
+# -- scores far from zero --------------------------------------------------------------------------------------
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# The exponent (x - M) / T of a term that does not vanish is below 130 and carries 3 roundings; a sum has at most
+# 300 in a row and 2 a join; the outer operations round values of at most 150 four times.
+ROW_TOL = U * (3 * 130 + 300 + 30 + 4 * 150)
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def far_rows(n, v, t, seed):
+    """Rows whose scores lie anywhere in the type's range, a few of each kind, and their labels."""
+    gen = torch.Generator().manual_seed(seed)
+    most = torch.finfo(t).max
+    z = torch.randn(n, v, generator=gen) * 3
+    for i in range(n):
+        kind = i % 9
+        if kind == 0:
+            z[i] = max(-1e9, -most)
+        elif kind == 1:
+            z[i] = -most
+        elif kind == 2:
+            z[i] += 1e4
+        elif kind == 3:
+            z[i] -= 1e4
+        elif kind == 4:
+            z[i] = z[i] * 10 + (1e6 if t != torch.float16 else 3e4)
+        elif kind == 5:
+            z[i] -= 300
+            z[i, torch.rand(v, generator=gen) < 0.5] = -float("inf")
+        elif kind == 6:
+            z[i] = -most
+            z[i, i % v] = 5.0
+        elif kind == 7:
+            z[i] = -float("inf")
+        # (8: ordinary)
+    labels = torch.randint(-1, v, (n,), generator=gen)
+    return z.to(t), labels
+
+
+def exact_rows(z, labels, temperature):
+    """float64: lse, entropy, label's log probability, log probabilities (of -inf: -inf)."""
+    x = z.double()
+    top = x.max(1, keepdim=True)[0]
+    none = torch.isinf(top)
+    d = (x - torch.where(none, torch.zeros_like(top), top)) / temperature
+    ln_s = torch.log(torch.exp(d).sum(1, keepdim=True))
+    lq = torch.where(none, torch.full_like(d, -float("inf")), d - ln_s)
+    p = torch.exp(lq)
+    h = -torch.where(p > 0, p * lq, torch.zeros_like(p)).sum(1)
+    has = (labels >= 0) & (labels < z.shape[1])
+    logp = torch.where(has, lq.gather(1, labels.clamp(min=0).long()[:, None])[:, 0], torch.zeros_like(h))
+    return (top / temperature + ln_s)[:, 0], h, logp, lq, p
+
+
+def check_far_grad(z, labels, a, b, temperature, got):
+    _, h, _, lq, p = exact_rows(z, labels, temperature)
+    has = (labels >= 0) & (labels < z.shape[1])
+    at = torch.nonzero(has)[:, 0]
+    g = a.double() * has
+    lqf = torch.where(p > 0, lq, torch.zeros_like(lq))
+    want = -p * (g[:, None] + b.double()[:, None] * (lqf + h[:, None]))
+    factor = g.abs()[:, None] + b.double().abs()[:, None] * (lqf.abs() + h[:, None] + 1)
+    size = p * factor
+    want[at, labels[at]] += g[at]
+    size[at, labels[at]] += g[at].abs()
+    none = torch.isinf(z.double().max(1)[0])
+    want[none] = 0
+    want, size = want / temperature, size / temperature
+    # (the hardware's exponential has no subnormals: a p below 2^-126 may be 0)
+    tol = (2 * ROW_TOL + 8 * U) * size + 2.0 ** -126 * factor / temperature + half_step(got.dtype) * want.abs() + \
+        (2.0 ** -25 if got.dtype == torch.float16 else 1e-37)
+    off = (got.double().cpu() - want).abs()
+    assert bool(torch.isfinite(got).all())
+    bad = (off > tol).any(1)
+    assert not bool(bad.any()), (torch.nonzero(bad)[:, 0].tolist(), float((off / tol).max()))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, v", [(300, 2), (18, 5), (45, 33), (27, 130), (90, 700), (21, 1000), (9, 1030), (18, 2500),
+                                  (9, 5001), (9, 20000), (9, 70001), (2300, 18001)])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_gradients_of_scores_far_from_zero(n, v, t, temperature):
+    if n * v > 1 << 22 and (t == torch.float16 or temperature != 1.0):
+        pytest.skip("covered by the other types and temperatures")
+    z, labels = far_rows(n, v, t, n + v)
+    gen = torch.Generator().manual_seed(9)
+    a, b = torch.randn(n, generator=gen), torch.randn(n, generator=gen)
+    zd, ld, ad, bd = z.to(DEV), labels.to(DEV), a.to(DEV), b.to(DEV)
+    _, ent, lse, _, _ = ops.label_logprobs(zd, ld, temperature=temperature)
+    got = ops.label_logprobs_grad(zd, ld, lse, ent, ad, bd, temperature)
+    check_far_grad(z, labels, a, b, temperature, got)
+    # rows that lie apart and begin anywhere, and in place
+    wide = torch.full((n, v + 7), 3.0, dtype=t, device=DEV)
+    wide[:, 3:3 + v] = zd
+    apart = ops.label_logprobs_grad(wide[:, 3:3 + v], ld, lse, ent, ad, bd, temperature)
+    check_far_grad(z, labels, a, b, temperature, apart)
+    ops.label_logprobs_grad(wide[:, 3:3 + v], ld, lse, ent, ad, bd, temperature, out=wide[:, 3:3 + v])
+    assert torch.equal(wide[:, 3:3 + v], apart)
+    assert bool((wide[:, :3] == 3).all()) and bool((wide[:, 3 + v:] == 3).all())
+
+
+def test_gradients_of_scores_far_from_zero_in_a_graph():
+    # the same launches whatever the rows hold: ordinary rows when captured, far ones when replayed
+    n, v = 18, 40_000
+    z, labels = far_rows(n, v, torch.float32, 4)
+    ones = torch.ones(n)
+    buf, ld, od = torch.zeros(n, v, device=DEV), labels.to(DEV), ones.to(DEV)
+
+    def both():
+        _, ent, lse, _, _ = ops.label_logprobs(buf, ld)
+        return ops.label_logprobs_grad(buf, ld, lse, ent, od, od)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for i in range(3):
+        rows = z.roll(i, 0)
+        buf.copy_(rows)
+        ld.copy_(labels.roll(i, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_far_grad(rows, labels.roll(i, 0), ones, ones, 1.0, got)
+        assert torch.equal(got, both())
