@@ -32,6 +32,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1.0e30f;      // x - M of a masked score: e^kFar is 0 and 0 * kFar is 0
+constexpr float kGone = -128.0f;      // the same for log p: a probability that small is 0, and times any weight stays 0
 constexpr float kLowest = -3.402823466e38f;
 
 // monotone in the value, 0 below everything (an absent element)
@@ -719,7 +720,7 @@ __device__ __forceinline__ void grad_row(const GradArgs& a, int64_t row, float l
     const int j0 = q * kV - rv.head;
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      const float lq = fmaxf(fmaf(x[i] - m0, a.inv_t, -l0), kFar) + 0.0f * l0;
+      const float lq = fmaxf(fmaf(x[i] - m0, a.inv_t, -l0), kGone) + 0.0f * l0;
       const float p = __builtin_amdgcn_exp2f(lq * kLog2e);
       float d = -p * fmaf(h, lq + H, g);
       d = (j0 + i == label ? d + g : d) * a.inv_t;

@@ -207,3 +207,33 @@ def test_gradients_of_scores_far_from_zero_in_a_graph():
         torch.cuda.synchronize()
         check_far_grad(rows, labels.roll(i, 0), ones, ones, 1.0, got)
         assert torch.equal(got, both())
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("v", [37, 1000, 40_000])
+@pytest.mark.parametrize("weight", [1e9, 2e30])
+def test_large_entropy_weights_beside_masked_scores(v, t, weight):
+    # a masked score has p = 0, so its gradient is 0 whatever the weight; the others' is weight times that of 1
+    gen = torch.Generator().manual_seed(v)
+    z = torch.randn(9, v, generator=gen)
+    z[:, 1::3] = -float("inf")
+    z[4] -= 3000                                # (a row that is read twice)
+    z = z.to(t).to(DEV)
+    labels = torch.zeros(9, dtype=torch.int32, device=DEV)
+    _, ent, lse, _, _ = ops.label_logprobs(z, labels)
+    one = torch.full((9,), 2.0 ** -10, device=DEV)
+    # (in float32: a float16 gradient below 2^-25 is 0, and weight times it need not be)
+    small = ops.label_logprobs_grad(z.float(), labels, lse, ent, None, one)
+    got = ops.label_logprobs_grad(z, labels, lse, ent, None, one * weight)
+    assert bool((got[:, 1::3] == 0).all())
+    # (float16 ends at 65504)
+    want = small.double() * float(torch.tensor(weight, dtype=torch.float32))
+    inside = want.abs() < float(torch.finfo(t).max) / 2
+    assert bool(inside.any())
+    # p lies within ROW_TOL (which both ways of reading a row keep), log p + H within as much of its two terms; the
+    # factor rounds twice, the result once
+    spread = (z.double() - z.double().max(1, keepdim=True)[0]).clamp(min=-200).abs() + 2 * ent.double()[:, None] + 1
+    p = torch.exp(torch.log_softmax(z.double(), 1))
+    tol = 2 * (ROW_TOL + 4 * U) * p * spread * weight * 2.0 ** -10 + 4 * U * want.abs() + half_step(t) * want.abs() + \
+        (2.0 ** -25 if t == torch.float16 else 0)
+    assert bool(((got.double() - want).abs() <= tol)[inside].all())
