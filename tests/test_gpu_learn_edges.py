@@ -237,3 +237,74 @@ def test_large_entropy_weights_beside_masked_scores(v, t, weight):
     tol = 2 * (ROW_TOL + 4 * U) * p * spread * weight * 2.0 ** -10 + 4 * U * want.abs() + half_step(t) * want.abs() + \
         (2.0 ** -25 if t == torch.float16 else 0)
     assert bool(((got.double() - want).abs() <= tol)[inside].all())
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, v, top", [(27, 2, 2), (40, 5, 5), (18, 64, 7), (18, 130, 32), (18, 700, 3), (18, 2500, 20),
+                                       (2060, 2500, 9), (9, 5001, 0), (9, 20000, 32), (9, 70001, 1)])
+@pytest.mark.parametrize("temperature", [1.0, 2.5])
+def test_log_probabilities_of_rows_anywhere_in_the_range(n, v, top, t, temperature):
+    """Each row held to its own size: what one row holds says nothing about another's error."""
+    z, labels = far_rows(n, v, t, 3 * n + v)
+    logp, ent, lse, tl, ti = ops.label_logprobs(z.to(DEV), labels.to(DEV), top=top, temperature=temperature)
+    rl, rh, rp, lq, _ = exact_rows(z, labels, temperature)
+    has = (labels >= 0) & (labels < v)
+    rp[has & torch.isinf(rl)] = -float("inf")
+
+    def held(got, want, scale, name):
+        got = got.double().cpu()
+        fine = torch.isfinite(want)
+        assert torch.equal(got[~fine], want[~fine]), name
+        off, tol = (got - want).abs()[fine], (ROW_TOL + scale)[fine]
+        assert bool((off <= tol).all()), (name, float((off / tol).max()))
+
+    # lse rounds M / T twice (1 / T and the product) and itself; a log probability the gap to M the same way
+    held(lse, rl, 4 * U * rl.abs(), "lse")
+    held(ent, rh, 4 * U * rh, "entropy")
+    held(logp, rp, 4 * U * rp.abs(), "logp")
+    if top:
+        order = torch.sort(z.double(), dim=1, descending=True, stable=True)[1][:, :top]
+        assert torch.equal(ti.cpu().long(), order)
+        want = lq.gather(1, order)
+        held(tl, want, 4 * U * want.abs(), "alternatives")
+
+
+def test_entropies_that_are_known():
+    # all equal: ln v; one left: 0; two left: ln 2 -- in every kernel's range of lengths, at any offset
+    for v in (2, 3, 64, 65, 1000, 2049, 4097, 30_001):
+        for base in (0.0, -1e9, torch.finfo(torch.float32).min, 3e38):
+            z = torch.full((3, v), base, device=DEV)
+            z[1:, 2:] = -float("inf")
+            z[1, 1] = -float("inf")
+            _, ent, lse, _, _ = ops.label_logprobs(z)
+            want = torch.tensor([np.log(v), 0.0, np.log(2.0)], dtype=torch.float64)
+            # s is a whole number, exact up to 2^24: the logarithm's roundings alone
+            assert bool(((ent.double().cpu() - want).abs() <= 4 * U * want).all()), (v, base, ent)
+            assert bool(((lse.double().cpu() - (z[0, 0].double().cpu() + want)).abs()
+                         <= 4 * U * (abs(base) + want)).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_hundred_tensors_against_their_formulas(bits):
+    # more than one launch's table: every tensor's parameters and states
+    gen = torch.Generator().manual_seed(1)
+    sizes = [int(q) for q in torch.randint(1, 700, (200,), generator=gen)]
+    ps = [torch.randn(n, generator=gen).to(DEV) for n in sizes]
+    gs = [torch.randn(n, generator=gen).to(DEV) for n in sizes]
+    m, v, scales = ops.adamw_states(ps, bits)
+    inside = np.concatenate([np.pad(np.ones(n, bool), (0, -n % 256)) for n in sizes])
+    hyper = dict(lr=0.01, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
+    for step in (1, 2, 3):
+        p0, g0 = flat_f64(ps), flat_f64(gs)
+        m0, v0 = (m.double().cpu().numpy(), v.double().cpu().numpy()) if bits == 32 else adam_values(m, v, scales)
+        ops.adamw_step(ps, gs, m, v, step=step, scales=scales, **hyper)
+        rp, rm, rv, upd = adam_reference(p0, g0, m0, v0, step, **hyper)
+        # the decay and the difference round twice, the step's factors about ten times
+        tol = 2 * U * (np.abs(p0) + upd) + 12 * U * upd + U * np.abs(rp)
+        assert (np.abs(flat_f64(ps) - rp) <= tol)[inside].all()
+        if bits == 32:
+            assert (np.abs(m.double().cpu().numpy() - rm) <= 4 * U * (np.abs(m0) + np.abs(g0)))[inside].all()
+            assert (np.abs(v.double().cpu().numpy() - rv) <= 6 * U * rv + 1e-44)[inside].all()
+        else:
+            check_codes(m, v, scales, rm * inside, np.sqrt(rv) * inside)
+        gs = [q * -0.5 for q in gs]
