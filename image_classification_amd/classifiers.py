@@ -436,8 +436,12 @@ class SoftmaxClassifier(object):
         return [b if gap >= min_prob_diff else -1 for b, gap in zip(best[:, 0].tolist(), lead)]
 
     def save_to_file(self, file_name):
-        """A numpy archive under exactly this name; nothing is pickled."""
+        """A numpy archive under exactly this name; nothing is pickled, so labels have to be numbers,
+        strings or bytes."""
         self._check_trained()
+        if self.classes_.dtype.hasobject:
+            raise ValueError("labels of type %s cannot be saved without pickling them"
+                             % type(self.labels_map[0]).__name__)
         arrays = {"weights_%d" % i: w.cpu().numpy() for i, w in enumerate(self._weights)}
         if self._centroids is not None:
             arrays["centroids"] = self._centroids
