@@ -1,0 +1,133 @@
+"""Calls that the documentation allows at the ends of sizes, strides and values."""
+import pytest
+import torch
+
+from image_classification_amd import ops
+from test_gpu_learn import close, reference
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("groups, k, out", [(1, 1, 1), (5, 64, 72), (3, 600, 33), (2, 1024, 1024)])
+def test_no_rows(groups, k, out, t):
+    codes = torch.empty(0, dtype=torch.int32, device=DEV)
+    order, offsets = ops.group_rows(codes, groups)
+    x, dy = torch.empty(0, k, dtype=t, device=DEV), torch.empty(0, out, dtype=t, device=DEV)
+    w = torch.ones(groups, out, k, dtype=t, device=DEV)
+    for o in (order, None):
+        assert ops.grouped_matmul(x, w, offsets, o).shape == (0, out)
+        assert ops.grouped_matmul_dx(dy, w, offsets, o).shape == (0, k)
+        dw = torch.full((groups, out, k), float("nan"), dtype=t, device=DEV)
+        ops.grouped_matmul_dw(dy, x, offsets, o, out=dw)
+        assert bool((dw == 0).all())
+    labels = torch.empty(0, dtype=torch.int64, device=DEV)
+    logp, ent, lse, tl, ti = ops.label_logprobs(x, labels, top=1)
+    assert logp.shape == ent.shape == lse.shape == (0,) and tl.shape == ti.shape == (0, 1)
+    assert ops.label_logprobs_grad(x, labels, lse, ent, logp, ent).shape == (0, k)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_of_nothing(bits):
+    empty = [torch.empty(0, device=DEV) for _ in range(3)]
+    m, v, scales = ops.adamw_states(empty, bits)
+    ops.adamw_step(empty, [torch.empty(0, device=DEV) for _ in empty], m, v, lr=0.1, step=1, scales=scales)
+    p = torch.ones(3, device=DEV)
+    some = [empty[0], p, empty[1]]
+    m, v, scales = ops.adamw_states(some, bits)
+    ops.adamw_step(some, [torch.zeros_like(q) for q in some], m, v, lr=0.1, step=1, weight_decay=0.5, scales=scales)
+    assert torch.allclose(p, torch.full((3,), 0.95, device=DEV))
+
+
+# (few rows, short rows, 64, 128 and 256 square tiles, rows of any alignment; whole and cut weight gradients)
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("n, groups, k, out", [(5, 3, 600, 40), (40, 9, 40, 24), (700, 3, 64, 64), (600, 2, 264, 72),
+                                               (600, 2, 263, 71), (9000, 2, 520, 520), (70_000, 1, 256, 512)])
+def test_subnormal_values_count(n, groups, k, out, t):
+    # products of the type's subnormals with powers of two that bring them back: exact sums of few bits
+    tiny = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[t]
+    back = {torch.float32: 2.0 ** 100, torch.bfloat16: 2.0 ** 100, torch.float16: 2.0 ** 14}[t]
+    gen = torch.Generator().manual_seed(n)
+    codes = torch.randint(0, groups, (n,), generator=gen, dtype=torch.int32)
+
+    def few(*shape):       # mostly zeros, so that a sum of 70 000 keeps its bits
+        return torch.randint(-3, 4, shape, generator=gen) * (torch.rand(shape, generator=gen) < 0.02)
+
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    for sx, sw in ((tiny, back), (back, tiny)):
+        x, dy, w = (few(n, k) * sx).to(t), (few(n, out) * sw).to(t), (few(groups, out, k) * sw).to(t)
+        ref = reference(codes, x, dy, w)
+        y = ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+        assert torch.equal(y.double().cpu(), ref["y"][0])
+        dw = ops.grouped_matmul_dw(dy.to(DEV), x.to(DEV), offsets, order, out_dtype=torch.float32)
+        assert torch.equal(dw.double().cpu(), ref["dw"][0])
+        dy = (few(n, out) * sx).to(t)
+        dx = ops.grouped_matmul_dx(dy.to(DEV), w.to(DEV), offsets, order, out_dtype=torch.float32)
+        assert torch.equal(dx.double().cpu(), reference(codes, x, dy, w)["dx"][0])
+
+
+@pytest.mark.parametrize("t, stride", [(torch.float32, (1 << 29) + 4), (torch.float32, (1 << 30) + 4),
+                                       (torch.bfloat16, (1 << 30) + 8), (torch.float16, (1 << 30) + 1)], ids=str)
+@pytest.mark.parametrize("n, groups, k, out", [(5, 2, 64, 72), (5, 1, 600, 33)])
+def test_rows_whose_offsets_pass_32_bits(n, groups, k, out, t, stride):
+    gen = torch.Generator().manual_seed(3)
+    codes = torch.tensor([0, groups - 1, 0, -1, groups - 1], dtype=torch.int32)
+    buf = torch.empty(4 * stride + 700, dtype=t, device=DEV)
+
+    def apart(q):
+        view = buf.as_strided((q.shape[0], q.shape[1]), (stride, 1))
+        view.copy_(q)
+        return view
+
+    x, dy = torch.randn(n, k, generator=gen).to(t), torch.randn(n, out, generator=gen).to(t)
+    w = torch.randn(groups, out, k, generator=gen).to(t)
+    ref = reference(codes, x, dy, w)
+    order, offsets = ops.group_rows(codes.to(DEV), groups)
+    close(ops.grouped_matmul(apart(x), w.to(DEV), offsets, order), *ref["y"], k, "y")
+    close(ops.grouped_matmul_dw(dy.to(DEV), apart(x), offsets, order), *ref["dw"], n, "dw")
+    close(ops.grouped_matmul_dx(apart(dy), w.to(DEV), offsets, order), *ref["dx"], out, "dx")
+    far = buf.as_strided((n, out), (stride, 1))
+    ops.grouped_matmul(x.to(DEV), w.to(DEV), offsets, order, out=far)
+    close(far, *ref["y"], k, "y, written apart")
+    z = apart(x)
+    logp, ent, lse, tl, ti = ops.label_logprobs(z, codes.to(DEV), top=3)
+    wl = ops.label_logprobs(x.to(DEV), codes.to(DEV), top=3)
+    # (rows that begin elsewhere in a granule are summed in another order)
+    for a, b in zip((logp, ent, lse, tl), wl):
+        assert float((a - b).abs().max()) <= 1e-5
+    assert torch.equal(ti, wl[4])
+    want = ops.label_logprobs_grad(x.to(DEV), codes.to(DEV), lse, ent, lse, ent)
+    assert torch.equal(ops.label_logprobs_grad(z, codes.to(DEV), lse, ent, lse, ent, out=z), want)
+
+
+def test_more_scores_than_32_bits_count():
+    # 70 000 rows of 65 000 bf16 scores, the last ones looked at
+    n, v = 70_000, 65_000
+    row = torch.randn(1, v, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(DEV)
+    z = row.expand(n, v).contiguous()
+    z[-1] = row.flip(1)[0]
+    labels = (torch.arange(n, device=DEV) % v).int()
+    logp, ent, lse, _, _ = ops.label_logprobs(z, labels)
+    one = ops.label_logprobs(z[-3:].clone(), labels[-3:])
+    assert float((logp[-3:] - one[0]).abs().max()) <= 1e-4 and float((ent[-3:] - one[1]).abs().max()) <= 1e-4
+    want = ops.label_logprobs_grad(z[-3:].clone(), labels[-3:], lse[-3:], ent[-3:], logp[-3:], ent[-3:])
+    ops.label_logprobs_grad(z, labels, lse, ent, logp, ent, out=z)
+    assert torch.equal(z[-3:], want)
+
+
+def test_a_product_of_more_values_than_32_bits_count():
+    # 3 million rows of 800 fp16: the rows of the far end against their own
+    n, k, out, groups = 3_000_000, 800, 16, 3
+    x = torch.ones(n, k, dtype=torch.float16, device=DEV)
+    x[-4:] = torch.arange(4, device=DEV)[:, None].half()
+    codes = (torch.arange(n, device=DEV) % groups).int()
+    w = (torch.arange(groups, device=DEV)[:, None, None] + 1).expand(groups, out, k).half().contiguous() / 1024
+    order, offsets = ops.group_rows(codes, groups)
+    y = ops.grouped_matmul(x, w, offsets, order, out_dtype=torch.float32)
+    want = (codes[-4:].float() + 1)[:, None] * torch.arange(4, device=DEV)[:, None] * (k / 1024)
+    assert bool((y[-4:] == want).all())
+    assert bool((y[:5] == (codes[:5].float() + 1)[:, None] * (k / 1024)).all())
+    dx = ops.grouped_matmul_dx(y[:, :16].half().contiguous(), w, offsets, order)
+    assert bool((dx[-4] == 0).all()) and bool((dx[-1] > 0).all())
