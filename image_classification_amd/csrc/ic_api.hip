@@ -896,11 +896,19 @@ int check_scratch(const char* who, const void* scratch, int64_t have, size_t nee
   return IC_OK;
 }
 
+constexpr int64_t kMostRows = 0x7ffffffeLL, kMostGroups = (int64_t)1 << 26, kMostScores = 0x7fffff00LL;
+constexpr int kMostWidth = 1 << 24;
+bool grouped_range(int64_t n, int64_t groups, int k, int out) {
+  return n >= 0 && n <= kMostRows && groups >= 1 && groups <= kMostGroups && k >= 1 && k <= kMostWidth && out >= 1 &&
+         out <= kMostWidth;
+}
+bool score_range(int64_t n, int64_t v) { return n >= 0 && n <= kMostRows && v >= 1 && v <= kMostScores; }
+
 int check_grouped(const char* who, int64_t n, int64_t groups, int k, int out, int dtype, int y_dtype) {
-  if (n < 0 || n >= 0x7fffffffLL || groups < 1 || groups > ((int64_t)1 << 26))
-    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 and 1 <= n_groups <= 2^26 (n=%lld n_groups=%lld)", who,
+  if (!grouped_range(n, groups, 1, 1))
+    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 - 1 and 1 <= n_groups <= 2^26 (n=%lld n_groups=%lld)", who,
                 (long long)n, (long long)groups);
-  if (k < 1 || out < 1 || k > (1 << 24) || out > (1 << 24))
+  if (!grouped_range(n, groups, k, out))
     return fail(IC_EINVAL, "%s: widths must be in [1, 2^24] (k=%d out=%d)", who, k, out);
   if (bad_type(dtype) || (y_dtype != dtype && y_dtype != IC_F32))
     return fail(IC_EINVAL, "%s: unsupported element types %d -> %d", who, dtype, y_dtype);
@@ -936,8 +944,8 @@ int grouped_rows_call(void* handle, const char* who, bool dx, const void* x, int
 }
 
 int check_scores(const char* who, int64_t n, int64_t v, int dtype, int64_t ld, float inv_t) {
-  if (n < 0 || n >= 0x7fffffffLL || v < 1 || v > 0x7fffff00LL)
-    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 and 1 <= v <= 2^31 - 256 (n=%lld v=%lld)", who,
+  if (!score_range(n, v))
+    return fail(IC_EINVAL, "%s: need 0 <= n < 2^31 - 1 and 1 <= v <= 2^31 - 256 (n=%lld v=%lld)", who,
                 (long long)n, (long long)v);
   if (bad_type(dtype)) return fail(IC_EINVAL, "%s: unknown element type %d", who, dtype);
   if (ld < v) return fail(IC_EINVAL, "%s: rows overlap (row stride %lld)", who, (long long)ld);
@@ -948,8 +956,9 @@ int check_scores(const char* who, int64_t n, int64_t v, int dtype, int64_t ld, f
 
 }  // namespace
 
+// (arguments that the call itself refuses need no scratch)
 int64_t ic_group_rows_scratch(int64_t n, int64_t n_groups) {
-  if (n < 0 || n_groups < 1) return 0;
+  if (!grouped_range(n, n_groups, 1, 1)) return 0;
   return (int64_t)ic::group_rows_scratch(n, n_groups);
 }
 
@@ -985,7 +994,7 @@ int ic_grouped_matmul_dx(void* handle, const void* dy, int64_t ld_dy, const void
 }
 
 int64_t ic_grouped_matmul_dw_scratch(int64_t n, int64_t n_groups, int k, int out, int dtype) {
-  if (n < 0 || n_groups < 1 || k < 1 || out < 1 || bad_type(dtype)) return 0;
+  if (!grouped_range(n, n_groups, k, out) || bad_type(dtype)) return 0;
   return (int64_t)ic::grouped_dw_scratch(n, n_groups, k, out, dtype);
 }
 
@@ -1014,7 +1023,7 @@ int ic_grouped_matmul_dw(void* handle, const void* dy, int64_t ld_dy, const void
 }
 
 int64_t ic_label_logprobs_scratch(int64_t n, int64_t v, int dtype, int top) {
-  if (n < 0 || v < 1 || bad_type(dtype) || top < 0) return 0;
+  if (!score_range(n, v) || bad_type(dtype) || top < 0 || top > ic::kMaxTop) return 0;
   return (int64_t)ic::score_scratch_bytes(n, ic::score_pieces(n, v, dtype), top);
 }
 

@@ -331,7 +331,7 @@ int ic_host_gather_f32(float* dst, const void* const* src, const int64_t* elems,
 
 /* Groups rows by code: order [n] int32 = the rows with codes[i] == 0, then 1, ..., ascending inside a
  * group; rows whose code is outside [0, n_groups) come last.  offsets [n_groups + 1] int64: group g is
- * order[offsets[g]] .. order[offsets[g + 1] - 1].  0 <= n < 2^31, 1 <= n_groups <= 2^26. */
+ * order[offsets[g]] .. order[offsets[g + 1] - 1].  0 <= n < 2^31 - 1, 1 <= n_groups <= 2^26. */
 int64_t ic_group_rows_scratch(int64_t n, int64_t n_groups);
 int ic_group_rows(void* handle, const int32_t* codes, int64_t n, int64_t n_groups, int32_t* order,
                   int64_t* offsets, void* scratch, int64_t scratch_bytes, void* stream);
@@ -342,7 +342,7 @@ int ic_group_rows(void* handle, const int32_t* codes, int64_t n, int64_t n_group
  *   ic_group_rows writes it, or is NULL: the rows lie group by group.  An entry of order that is no
  *   row is passed over; offsets are used as if clamped to [0, n].
  *   dtype: of x and w; y_dtype: the same, or IC_F32.
- * 1 <= k, out; 0 <= n < 2^31.  Rows and matrices that are 16-byte aligned, with widths of a
+ * 1 <= k, out <= 2^24; 0 <= n < 2^31 - 1.  Rows and matrices that are 16-byte aligned, with widths of a
  * multiple of 16 bytes, take the fast path. */
 int ic_grouped_matmul(void* handle, const void* x, int64_t ld_x, const void* w, void* y, int64_t ld_y,
                       const int64_t* offsets, const int32_t* order, int64_t n, int64_t n_groups, int k,

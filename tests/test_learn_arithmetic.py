@@ -74,3 +74,23 @@ def test_the_quick_codes_of_subnormal_scales_leave_their_range():
             assert careful(q * unit, mant, top).max() <= top
             past[name] += int(quick(q)[0].max() > top)
     assert past["m"] > 0 and past["v"] > 0
+
+
+def test_sizes_beyond_the_limits_ask_for_no_scratch():
+    # sizes that the calls refuse; some of them are not even representable a step further on
+    from image_classification_amd import _lib
+    lib = _lib.load()
+    big = [1 << 62, (1 << 63) - 1, (1 << 62) + 1]
+    for n, groups in [(1000, (1 << 26) + 1), (9000, 1 << 40), ((1 << 31) - 1, 5)] + [(9000, b) for b in big] + \
+            [(b, 5) for b in big] + [(-1, 5), (5, 0), (5, -(1 << 63))]:
+        assert lib.ic_group_rows_scratch(n, groups) == 0
+        assert lib.ic_grouped_matmul_dw_scratch(n, groups, 64, 64, 0) == 0
+    for k, out in (((1 << 24) + 1, 8), (8, (1 << 31) - 1), ((1 << 31) - 1, (1 << 31) - 1), (0, 8)):
+        assert lib.ic_grouped_matmul_dw_scratch(100_000, 3, k, out, 1) == 0
+    for n, v, top in [(b, 70_000, 3) for b in big] + [(4, b, 3) for b in big] + [(4, 70_000, 33), (4, 70_000, -1),
+                                                                              (4, 0, 0), (4, (1 << 31) - 255, 3)]:
+        assert lib.ic_label_logprobs_scratch(n, v, 0, top) == 0
+    # the largest sizes that are taken
+    assert lib.ic_group_rows_scratch((1 << 31) - 2, 1 << 26) > 0
+    assert lib.ic_grouped_matmul_dw_scratch((1 << 31) - 2, 1, 1 << 24, 1, 0) > 0
+    assert lib.ic_label_logprobs_scratch(4, (1 << 31) - 256, 0, 32) > 0
