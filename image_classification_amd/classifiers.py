@@ -226,8 +226,9 @@ class SoftmaxClassifier(object):
     """Linear softmax classifier over histograms or descriptors, with routed experts.
 
     logits = W_g [x, 1] for the nearest of `experts` centroids g (k-means over the training rows;
-    one expert: an ordinary linear classifier), W_g classes x columns.  `rank`: W_g is a product
-    B_g A_g through that many columns, for wide histograms with many classes.  Training minimises
+    one expert: an ordinary linear classifier; several: rows of at most 2048 columns), W_g classes x
+    columns.  `rank`: W_g is a product B_g A_g through that many columns, for wide histograms with many
+    classes.  Training minimises
     the mean negative log probability of the labels minus `entropy_weight` times the mean entropy,
     with AdamW steps over `epochs` passes in batches of `batch_size`; `state_bits=8` keeps the
     optimizer states in 8 bits.  Everything between the upload of the rows and the download of the

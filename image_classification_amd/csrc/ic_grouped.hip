@@ -62,8 +62,11 @@ __device__ __forceinline__ unsigned rank_in_wave(Count* cnt, unsigned d, bool in
 }
 
 // Few rows: one workgroup, everything in LDS.  Bound by latency: 6.6 us for 1000 rows of 1000 groups
-// (bitonic sorting took 18.6 us: 66 steps of a barrier each), 4.0 for 16 rows of 64; up to 8192 rows one
-// such workgroup is faster than the launches below (5003 rows of 37 groups: 8.3 us against 23).
+// (bitonic sorting took 18.6 us: 66 steps of a barrier each), 4.0 for 16 rows of 64; up to 8192 rows of as many
+// groups at most one such workgroup is about as fast as the launches below, or faster (5003 rows of 37 groups: 8.8 us
+// against 23; 8192 rows of 8192 groups 25 against 24).  It also writes the offsets, with a search of the sorted keys
+// for each, and that is what many more groups than rows cost: 1000 rows of 32 768 groups 30 us, of 2^20 730 (8193 rows
+// of 2^20 groups, by the launches below: 45).
 constexpr int kSmallRows = 8192, kSmallBits = 8;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_group_small(const int32_t* __restrict__ codes, int n,
@@ -973,8 +976,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_grouped_rows(RowsArgs a) {
 // of 64 R x 64: there are too few stages to pipeline, so everything is fetched at once.  The matrix's part
 // goes to LDS, shared by the four waves; each wave's 16 R rows go straight to the registers that the
 // products take them from.  One barrier, one memory latency behind the search for the group.
-// 1M rows x 128 float32, 10 000 groups of 64 x 128: 321 to 331 us (R = 1: 343), 3.4 TB/s of rows, matrices and results and
-// 48 TFLOP/s (staged like the longer ones 355 us).  Neither is at its limit (memory 0.21 ms, products
+// 1M rows x 128 float32, 10 000 groups of 64 x 128: 301 us in a captured graph, 3.7 TB/s of rows, matrices and results and
+// 54 TFLOP/s (310 to 337 under a kernel trace, where R = 1 takes 343 and staging like the longer ones 355).  Neither is at its limit (memory 0.21 ms, products
 // 0.11 ms): a workgroup loads, multiplies and stores once, and what four of them a CU overlap is part
 // of it.
 // Five workgroups share a CU (R = 2: four): 32 KB of LDS and 96 (128) registers each.
@@ -1584,7 +1587,11 @@ hipError_t rows_launch(RowsArgs a, hipStream_t s) {
 constexpr int kTileSize[3] = {256, 128, 64};
 constexpr int kPerCu[3] = {1, 2, 4};
 // Rate of a full CU relative to 256 x 256 tiles (a smaller tile reads more of LDS and L2 a product;
-// float32 products are eight to sixteen times slower and do not notice)
+// float32 products are eight to sixteen times slower and do not notice).  Measured with whole rounds of the card,
+// TFLOP/s with tiles of 256, 128 and 64: bf16 forward 976, 748, 477, dw 1003, 660, 371; float32 forward
+// 123, 122, 121, dw 124, 112, 100 (in dw both operands are read 4 bytes a lane, and a small tile reads more of
+// them).  256 x 256 of float32 are held back because a group's last tile wastes more (16 groups of 1024 x 1024,
+// forward: 108, 117, 118).
 constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.85};
 
 // The tile with the least time for `tiles(size)` tiles: the most tiles that a CU gets times a tile's work, over
@@ -1592,6 +1599,7 @@ constexpr double kRate16[3] = {1.0, 0.8, 0.5}, kRate32[3] = {0.7, 1.0, 0.85};
 // 16 groups of 2048 x 512 float32, dx, took 128 x 128 tiles: 275 us, with 64 x 64 199).
 template <typename F>
 int pick_tile(int type, bool aligned, F tiles) {
+  // (not kRate32: 64 x 64 tiles of float32 lose 1 to 3 % of the rate of 128 x 128 here, 11 % in dw)
   static const double kRows32[3] = {0.7, 1.0, 0.97};
   const double* rate = type == IC_F32 ? kRows32 : kRate16;
   int best = 2;

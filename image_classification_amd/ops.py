@@ -915,6 +915,8 @@ def ransac_homography(pts, offsets, n_iter, th, samples=None, seed=0, min_inlier
 # -- what is learned on top of the codes -------------------------------------------------------------
 # Launches only: memory a call needs for itself is allocated here, from torch's allocator on the
 # current stream, so these calls may be captured into a graph and used on any stream.
+# None of them records anything for autograd: a result never requires a gradient, whatever its inputs do, and
+# the gradients are calls of their own (grouped_matmul_dx, grouped_matmul_dw, label_logprobs_grad).
 # (A small call is bound by what Python does around it: addresses go to ctypes as plain integers, and
 # the stream is asked for once, without a Stream object.)
 def _addr(t):
@@ -1080,9 +1082,10 @@ def grouped_matmul(x, w, offsets, order=None, out=None, out_dtype=None):
 
     x [n, k], w [n_groups, out, k] of the same type (float32, bfloat16, float16; sums are float32);
     (order, offsets) as group_rows returns them (offsets ascend from 0 to at most n) -- order=None: the
-    rows lie group by group, row i in group g when offsets[g] <= i < offsets[g + 1].  Returns y [n, out] of x's type or `out_dtype`
-    (float32); `out`: a tensor to write to, which must share no memory with x or w.  Rows may lie
-    apart (a column slice of a wider matrix); order must name every row once."""
+    rows lie group by group, row i in group g when offsets[g] <= i < offsets[g + 1].  Returns y [n, out]
+    of x's type or `out_dtype` (float32); `out`: a tensor to write to, which must share no memory with x
+    or w.  Rows may lie apart (a column slice of a wider matrix); order must name every row once.
+    Autograd does not see the product: its gradients are grouped_matmul_dx and grouped_matmul_dw."""
     return _grouped_rows("ic_grouped_matmul", x, w, offsets, order, out, out_dtype, False)
 
 
@@ -1153,7 +1156,8 @@ def label_logprobs(logits, labels=None, top=0, temperature=1.0):
     at most 32).  logits [n, v] float32, bfloat16 or float16, rows may lie apart.
 
     Scores of -inf have probability 0; a row of nothing else gives lse = -inf, logp = -inf and
-    entropy = 0.  NaN or +inf in a row makes its results NaN."""
+    entropy = 0.  NaN or +inf in a row makes its results NaN.  Autograd does not see any of it: the
+    gradient of logp and entropy is label_logprobs_grad."""
     ld = _check_rows(logits, "logits")
     n, v = logits.shape
     t = _type_number(logits, "logits")
@@ -1268,7 +1272,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
     uint8 states, ADAMW_BLOCK elements share a scale (adamw_state_values gives their values).
     lr: a number, or a float32 device tensor of one element; step: a number counted from 1, or an
     int64 device tensor of one element (a value below 1 counts as 1) -- a captured step reads them at
-    every replay."""
+    every replay.  Autograd does not see the step: parameters that require a gradient are updated in place
+    all the same, without a new version."""
     count = len(params)
     if len(grads) != count:
         raise ValueError("%d parameters, %d gradients" % (count, len(grads)))
