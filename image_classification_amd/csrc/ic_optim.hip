@@ -366,7 +366,8 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamTable tab, AdamArgs a) {
   double lr, lr1d, root;
   corrections(a, &lr, &lr1d, &root);
   // (the step itself is float32: only what becomes a code has to be decided in float64)
-  const float lr1 = (float)lr1d, lrwd = (float)(lr * a.wd), eps = (float)a.eps;
+  // (an eps whose reciprocal is no float32 would turn a step of 0 / eps into NaN)
+  const float lr1 = (float)lr1d, lrwd = (float)(lr * a.wd), eps = fmaxf((float)a.eps, 0x1p-124f);
   unsigned char* mp = static_cast<unsigned char*>(a.m) + t.state0 + i;
   unsigned char* vp = static_cast<unsigned char*>(a.v) + t.state0 + i;
   const int64_t block = (t.state0 + i) / kStateBlock;

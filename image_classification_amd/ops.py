@@ -1269,7 +1269,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, lr, step, betas=(0.9, 0.999),
     params / grads: contiguous float32, bfloat16 or float16 tensors in any mix, one gradient per
     parameter of the same number of elements; no two parameters may share memory.  exp_avg,
     exp_avg_sq, scales: flat states as adamw_states makes them, for this list in this order.  With
-    uint8 states, ADAMW_BLOCK elements share a scale (adamw_state_values gives their values).
+    uint8 states, ADAMW_BLOCK elements share a scale (adamw_state_values gives their values), and an eps
+    below 2^-124 counts as that.
     lr: a number, or a float32 device tensor of one element; step: a number counted from 1, or an
     int64 device tensor of one element (a value below 1 counts as 1) -- a captured step reads them at
     every replay.  Autograd does not see the step: parameters that require a gradient are updated in place

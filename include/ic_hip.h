@@ -400,7 +400,8 @@ typedef struct ic_adamw_tensor {
  *   p -= lr weight_decay p + lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
  *   tensors [count] (HOST).  state_bits 32: exp_avg, exp_avg_sq [state_elements] f32.  state_bits 8:
  *   they are codes [state_elements] uint8 with scales [2][state_elements / IC_ADAMW_BLOCK] f32
- *   (all zeros to begin with); ic_adamw_state_values gives the values that they stand for.
+ *   (all zeros to begin with); ic_adamw_state_values gives the values that they stand for; an eps below 2^-124
+ *   counts as that.
  *   lr_dev (f32) and step_dev (int64; a value below 1 counts as 1), device, are read instead of lr and
  *   step when they are not NULL (a captured step then follows them).  step >= 1.  No two tensors may
  *   share memory. */

@@ -309,3 +309,22 @@ def test_two_hundred_tensors_against_their_formulas(bits):
         else:
             check_codes(m, v, scales, rm * inside, np.sqrt(rv) * inside)
         gs = [q * -0.5 for q in gs]
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-46, 1e-40, 1e-38])
+def test_an_eps_that_no_reciprocal_can_take(eps):
+    # in 8 bits an eps below 2^-124 counts as that: what has no state does not move, the rest moves as it should
+    gen = torch.Generator().manual_seed(2)
+    p = torch.randn(512, generator=gen).to(DEV)
+    g = torch.randn(512, generator=gen).to(DEV)
+    g[::2] = 0
+    p0 = p.clone()
+    m, v, scales = ops.adamw_states([p], 8)
+    hyper = dict(lr=1e-3, betas=(0.9, 0.999), weight_decay=0.0)
+    for step in (1, 2, 3):
+        before, m0, v0 = flat_f64([p]), *adam_values(m, v, scales)
+        ops.adamw_step([p], [g], m, v, step=step, eps=eps, scales=scales, **hyper)
+        rp, rm, rv, upd = adam_reference(before, flat_f64([g]), m0, v0, step, eps=2.0 ** -124, **hyper)
+        assert (np.abs(flat_f64([p]) - rp) <= 2 * U * (np.abs(before) + upd) + 12 * U * upd + U * np.abs(rp)).all()
+        check_codes(m, v, scales, rm, np.sqrt(rv))
+    assert torch.equal(p[::2], p0[::2]) and bool((p[1::2] != p0[1::2]).all())
