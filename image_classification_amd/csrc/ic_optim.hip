@@ -238,8 +238,13 @@ struct Lane8 {
   float lr1, lrwd, eps;
 };
 
+// WIDE: for divisors up to the largest float32.  The hardware's reciprocal flushes what is below 2^-126, so a quarter
+// of the divisor is inverted (none of a float32 has so small a reciprocal, none of an eps from 2^-124 on too large a one).
+template <bool WIDE>
 __device__ __forceinline__ float stepped(float p, float m, double r, const Lane8& s) {
-  return fmaf(-s.lrwd, p, p) - m * s.lr1 * __builtin_amdgcn_rcpf((float)(r * s.root) + s.eps);
+  if (!WIDE) return fmaf(-s.lrwd, p, p) - m * s.lr1 * __builtin_amdgcn_rcpf((float)(r * s.root) + s.eps);
+  const float quarter = 0.25f * __builtin_amdgcn_rcpf((float)(0.25 * (r * s.root)) + 0.25f * s.eps);
+  return fmaf(-s.lrwd, p, p) - m * s.lr1 * quarter;
 }
 
 // A block of 256 elements is held by 32 lanes, eight elements each, from the codes to the new codes.
@@ -247,11 +252,11 @@ __device__ __forceinline__ float stepped(float p, float m, double r, const Lane8
 // adamw8_careful decides every code in float64 and handles what is not finite.
 // adamw8_quick is for finite values.  Its codes come from the float64 quotients rounded to float32
 // once: m's by the hardware's conversion to this format (e4m3), v's from the float32 bits.  That is the
-// same code except in two cases, in which it returns true and the wave takes the careful way instead:
-// where the float32 is exactly a middle between two codes (one in 2^19 or so), and where a new scale is a
-// float32 subnormal.  Rounding such a scale moves it by up to a half, so the largest quotient may pass the
-// largest code, and neither of these codes is bounded (e4m3 has no number above 464, v's bits run into the
-// next byte); a normal scale moves by 2^-24 at most, which float32 quotients do not see.
+// same code except in two cases: where the float32 is exactly a middle between two codes (one in 2^19 or so), and
+// where a new scale is a float32 subnormal.  Rounding such a scale moves it by up to a half, so the largest quotient
+// may pass the largest code, and neither of these codes is bounded (e4m3 has no number above 464, v's bits run into
+// the next byte); a normal scale moves by 2^-24 at most, which float32 quotients do not see.  In both, and where a
+// divisor of the step is above 2^122 (stepped), it returns true and the wave takes the careful way instead.
 __device__ __forceinline__ void adamw8_careful(const Lane8& s, u32x2 mc, u32x2 vc, const float* g, const float* p,
                                                float* p_out, u32x2* mo, u32x2* vo, float* out_sm, float* out_sv) {
   double m[8], r[8];
@@ -268,7 +273,7 @@ __device__ __forceinline__ void adamw8_careful(const Lane8& s, u32x2 mc, u32x2 v
     m[q] = fma(s.b1, (double)fm * s.sm, s.omb1 * gq);
     const double v = fma(s.b2, r0 * r0, s.omb2 * (gq * gq));
     r[q] = root_of(v > kTiny ? v : v + kTiny);   // (NaN stays)
-    p_out[q] = stepped(p[q], (float)m[q], r[q], s);
+    p_out[q] = stepped<true>(p[q], (float)m[q], r[q], s);
     top_m = fmax(top_m, finite_size(m[q]));
     top_r = fmax(top_r, finite_size(r[q]));
   }
@@ -313,7 +318,7 @@ __device__ __forceinline__ bool adamw8_quick(const Lane8& s, u32x2 mc, u32x2 vc,
     m[q] = fma((double)fm, b1sm, s.omb1 * gq);
     const double v = fma(fr * fr, b2sv2, s.omb2 * (gq * gq));
     r[q] = root_of(fmax(v, kTiny));
-    p_out[q] = stepped(p[q], (float)m[q], r[q], s);
+    p_out[q] = stepped<false>(p[q], (float)m[q], r[q], s);
     top_m = fmax(top_m, fabs(m[q]));
     top_r = fmax(top_r, r[q]);
   }
@@ -322,7 +327,8 @@ __device__ __forceinline__ bool adamw8_quick(const Lane8& s, u32x2 mc, u32x2 vc,
   const double im = new_sm > 0.0f ? inverse_of((double)new_sm) : 0.0;
   const double iv = new_sv > 0.0f ? inverse_of((double)new_sv) : 0.0;
   const double seen = new_sv > 0.0f ? kSeen : __builtin_inf();
-  bool doubt = (new_sm > 0.0f && new_sm < 0x1p-126f) || (new_sv > 0.0f && new_sv < 0x1p-126f);
+  bool doubt = (new_sm > 0.0f && new_sm < 0x1p-126f) || (new_sv > 0.0f && new_sv < 0x1p-126f) ||
+               new_sv * (491520.0f * (float)s.root) > 0x1p122f;
   float qm[8];
   *vo = u32x2{0u, 0u};
 #pragma unroll

@@ -328,3 +328,13 @@ def test_an_eps_that_no_reciprocal_can_take(eps):
         assert (np.abs(flat_f64([p]) - rp) <= 2 * U * (np.abs(before) + upd) + 12 * U * upd + U * np.abs(rp)).all()
         check_codes(m, v, scales, rm, np.sqrt(rv))
     assert torch.equal(p[::2], p0[::2]) and bool((p[1::2] != p0[1::2]).all())
+
+
+@pytest.mark.parametrize("largest", [1e37, 8e37, 1e38, 3.4e38])
+def test_gradients_near_the_largest_float32(largest):
+    # a first step is lr times the sign, whatever the size
+    g = torch.from_numpy(np.float32(largest) * np.linspace(-1, 1, 512, dtype=np.float32)).to(DEV)
+    p = torch.zeros(512, device=DEV)
+    m, v, scales = ops.adamw_states([p], 8)
+    for step in (1, 2, 3):
+        step8(p, g, m, v, scales, step, (0.9, 0.999))
