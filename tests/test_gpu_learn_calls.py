@@ -131,3 +131,47 @@ def test_a_product_of_more_values_than_32_bits_count():
     assert bool((y[:5] == (codes[:5].float() + 1)[:, None] * (k / 1024)).all())
     dx = ops.grouped_matmul_dx(y[:, :16].half().contiguous(), w, offsets, order)
     assert bool((dx[-4] == 0).all()) and bool((dx[-1] > 0).all())
+
+
+def test_several_threads_at_once():
+    # the calls keep nothing in the handle: each thread on a stream of its own, all results as one after the other
+    import threading
+
+    def work(seed):
+        gen = torch.Generator().manual_seed(seed)
+        n, groups, k, v = 9000 + 500 * seed, 20, 72, 700
+        x = torch.randn(n, k, generator=gen).to(DEV)
+        w = torch.randn(groups, v, k, generator=gen).to(DEV) * 0.2
+        codes = torch.randint(-1, groups, (n,), generator=gen, dtype=torch.int32).to(DEV)
+        labels = torch.randint(-1, v, (n,), generator=gen).to(DEV)
+        step = [torch.ones(n, device=DEV)]
+        m, s, scales = ops.adamw_states([w], 8)
+        for t in range(1, 4):
+            order, offsets = ops.group_rows(codes, groups)
+            z = ops.grouped_matmul(x, w, offsets, order)
+            logp, ent, lse, tl, ti = ops.label_logprobs(z, labels, top=4)
+            ops.label_logprobs_grad(z, labels, lse, ent, step[0], out=z)
+            dw = ops.grouped_matmul_dw(z, x, offsets, order)
+            ops.adamw_step([w], [dw], m, s, lr=1e-3, step=t, scales=scales)
+        torch.cuda.current_stream().synchronize()
+        return logp, ent, tl, ti, z, dw, w, m, s, scales
+
+    want = [work(i) for i in range(4)]
+    got, errors = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = work(i)
+        except Exception as e:          # (a thread's exception would only be printed)
+            errors.append(e)
+
+    for _ in range(3):
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors, errors
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
